@@ -697,7 +697,7 @@ __global__ __launch_bounds__(BS) void fps_coop_kernel(int B, int N, int m, int L
       if (active) {
       float best = -1.f;
       if constexpr (PPT % 2 == 0) {
-        // two points per packed instruction (v_pk_add/mul/fma_f32): the same IEEE operations in the same order as
+        // two points per float2 operation: the same IEEE operations in the same order as
         // pn2_sq3 — fma(dz, dz, fma(dx, dx, dy * dy)) — on both halves
         typedef float f2 __attribute__((ext_vector_type(2)));
         const f2 o2x = {ox[0], ox[0]}, o2y = {oy[0], oy[0]}, o2z = {oz[0], oz[0]};
@@ -1070,7 +1070,7 @@ __global__ __launch_bounds__(1024) void fps_multi_kernel(int B, int N, int m, in
         const int sl = bl / SUB;
         const float ox = pn2_readlane_f32(s_fin.x[sl], 0), oy = pn2_readlane_f32(s_fin.y[sl], 0),
                     oz = pn2_readlane_f32(s_fin.z[sl], 0);
-        // two slots per packed instruction (v_pk_add / mul / fma_f32): the IEEE operations of pn2_sq3 in its order —
+        // two slots per float2 operation: the IEEE operations of pn2_sq3 in its order —
         // fma(dz, dz, fma(dx, dx, dy * dy)) — on both halves; an odd slot count leaves one scalar tail
         typedef float f2 __attribute__((ext_vector_type(2)));
         const f2 o2x = {ox, ox}, o2y = {oy, oy}, o2z = {oz, oz};

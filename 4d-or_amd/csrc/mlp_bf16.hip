@@ -1196,7 +1196,7 @@ __global__ __launch_bounds__(512, (FOLD || (RECOMP && KTK <= 2)) ? 4 : 2) void m
             const float4 xa = *(const float4 *)&sXr[m * 8], xb = *(const float4 *)&sXr[m * 8 + 4];
             const f2 v2 = {vr, vr};
             f2 *pp = reinterpret_cast<f2 *>(px[FOLD ? d : 0]);
-            pp[0] = __builtin_elementwise_fma(v2, f2{xa.x, xa.y}, pp[0]);   // v_pk_fma_f32
+            pp[0] = __builtin_elementwise_fma(v2, f2{xa.x, xa.y}, pp[0]);
             pp[1] = __builtin_elementwise_fma(v2, f2{xa.z, xa.w}, pp[1]);
             pp[2] = __builtin_elementwise_fma(v2, f2{xb.x, xb.y}, pp[2]);
             pp[3] = __builtin_elementwise_fma(v2, f2{xb.z, xb.w}, pp[3]);

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(512) void mlp_bwd_first_kernel(const FirstArgs a) {
                                                             (d_rb * 32 + 4 * lh + (r & 3) + 8 * (r >> 2)) * XW);
         const float4 xa = xr[0], xb = xr[1];                    // two broadcast ds_read_b128
         const f2 v2 = {v, v};
-        px[0] = __builtin_elementwise_fma(v2, f2{xa.x, xa.y}, px[0]);   // v_pk_fma_f32
+        px[0] = __builtin_elementwise_fma(v2, f2{xa.x, xa.y}, px[0]);
         px[1] = __builtin_elementwise_fma(v2, f2{xa.z, xa.w}, px[1]);
         px[2] = __builtin_elementwise_fma(v2, f2{xb.x, xb.y}, px[2]);
         px[3] = __builtin_elementwise_fma(v2, f2{xb.z, xb.w}, px[3]);
