@@ -927,6 +927,57 @@ int pn2_x3_pool_bwd(long long M, int N, int K, int ns, const float *Yp, const fl
                     const int *arg, const float *gPm, float *Gout, double *sums, float *dW, void *workspace,
                     size_t workspace_bytes, void *stream);
 
+/* --------------------------------------------------------------------- dense heads ---
+ * Element types of the entry points below. */
+#define PN2_DT_F32 0
+#define PN2_DT_BF16 1
+#define PN2_DT_F16 2
+
+/* Statistics of rows of logits (csrc/label_probs.hip).  logits (T, V) of `dtype`, row t at element t ld (any alignment of an
+ * element; ld may be smaller than V, 0 included: rows are only read); labels (T).
+ *   log_prob (T) f32: log softmax(row)[label]; 0 where label == ignore_index; NaN where it is outside [0, V)
+ *   entropy  (T) f32: -sum p log p in nats (-inf logits add 0)
+ *   top_log_prob / top_index (T, top): the `top` <= min(V, 64) best entries, descending, equal logits in ascending index order;
+ *       entries of -inf are no alternatives: such slots hold -inf and the index -1.  top = 0: both may be NULL
+ *   stats (T, 2) f32 for the gradient, or NULL
+ * A row of nothing but -inf: log_prob -inf, entropy 0, no alternatives, gradient 0.  A row with NaN or +inf: NaN, indices -1.
+ * The gradient: dlogits (T, V) dense, every element written, rounded once;  g_log_prob / g_entropy (T) f32, NULL = zero. */
+int pn2_label_logprobs(long long T, int V, long long ld, int dtype, const void *logits, const long long *labels,
+                       long long ignore_index, int top, float *log_prob, float *entropy, float *stats, float *top_log_prob,
+                       long long *top_index, void *stream);
+int pn2_label_logprobs_grad(long long T, int V, long long ld, int dtype, const void *logits, const long long *labels,
+                            long long ignore_index, const float *stats, const float *entropy, const float *g_log_prob,
+                            const float *g_entropy, void *dlogits, void *stream);
+
+/* Divergence of a teacher's k top logits from the student's softmax (csrc/label_probs.hip).  teacher_index (T, k),
+ * teacher_logits (T, k) of `teacher_dtype`;  with q = softmax(teacher / temperature) over the row's used slots and
+ * p = softmax(logits / temperature) over all V:   loss (T) f32 = temperature^2 sum_j q_j (log q_j - log p[index_j]).
+ * A slot with a negative index or the value -inf is unused; a row without a used slot has loss 0 and gradient 0 (its logits are
+ * not read).  An index >= V makes the row NaN.  An index may occur more than once.  stats (T, 4) f32 for the gradient, or NULL.
+ * The gradient: dlogits (T, V) dense = g_loss temperature (p - sum_j q_j [index_j = v]), every element written, rounded once. */
+int pn2_distill_topk(long long T, int V, long long ld, int dtype, const void *logits, int k, const long long *teacher_index,
+                     int teacher_dtype, const void *teacher_logits, float temperature, float *loss, float *stats, void *stream);
+int pn2_distill_topk_grad(long long T, int V, long long ld, int dtype, const void *logits, int k, const long long *teacher_index,
+                          int teacher_dtype, const void *teacher_logits, float temperature, const float *stats,
+                          const float *g_loss, void *dlogits, void *stream);
+
+/* A dense layer, y (M, N) = act(x W^T + bias) + residual, and its backward pass (csrc/linear_act.hip).  x (M, K) at row stride
+ * ldx, W (N, K) at row stride ldw, residual (M, N) at row stride ldr (or NULL), all of `dtype`, last axis contiguous, any
+ * alignment of an element; bias (N) of `dtype` or fp32 (or NULL); y, slope (M, N) dense.  act 0 none | 1 relu | 2 gelu (erf) |
+ * 3 gelu (tanh form) | 4 silu.  fp32 accumulation and epilogue, one rounding.  slope: act'(z), what the backward pass needs,
+ * fp32 for fp32 and fp16 for both 16-bit types (NULL: not wanted; never written for act 0).
+ * The gradient: dy (M, N) at row stride ldy; slope NULL stands for ones; dx (M, K), dw (N, K) dense, db (N) of db_dtype, each NULL
+ * = not wanted, every element written; sums in a fixed order.  want = 1 dx | 2 dw | 4 db.
+ * 1 <= N, K <= 4194240.  A workspace must not be shared by calls that may run at the same time. */
+size_t pn2_linear_act_workspace_bytes(long long M, int N, int K, int dtype);
+int pn2_linear_act(long long M, int N, int K, int dtype, const void *x, long long ldx, const void *w, long long ldw,
+                   const void *bias, int bias_dtype, int act, const void *residual, long long ldr, void *y, void *slope,
+                   void *workspace, size_t workspace_bytes, void *stream);
+size_t pn2_linear_act_grad_workspace_bytes(long long M, int N, int K, int dtype, int has_slope, int want);
+int pn2_linear_act_grad(long long M, int N, int K, int dtype, const void *dy, long long ldy, const void *slope, const void *x,
+                        long long ldx, const void *w, long long ldw, void *dx, void *dw, void *db, int db_dtype,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

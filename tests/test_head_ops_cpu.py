@@ -1,0 +1,89 @@
+"""Dense-head operators (pointnet2_ops.head_ops) without a GPU: every refusal comes before any launch, with its reason."""
+import ctypes
+
+import pytest
+import torch
+
+from pointnet2_ops import _ext, head_ops as ho
+
+
+def f(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+REFUSALS = [
+    ("CPU not supported", lambda: ho.linear_act(f(2, 3), f(4, 3))),
+    ("CPU not supported", lambda: ho.label_log_probs(f(2, 3), torch.zeros(2, dtype=torch.int64))),
+    ("CPU not supported", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), f(2, 1))),
+    # linear_act
+    ("weight must have shape", lambda: ho.linear_act(f(2, 3), f(4, 5))),
+    ("weight must have shape", lambda: ho.linear_act(f(2, 3), f(3))),
+    ("weight must have the type of x", lambda: ho.linear_act(f(2, 3), f(4, 3, dtype=torch.bfloat16))),
+    ("at least one row", lambda: ho.linear_act(f(2, 3), f(0, 3))),
+    ("at least one column", lambda: ho.linear_act(f(2, 0), f(4, 0))),
+    ("activation must be one of", lambda: ho.linear_act(f(2, 3), f(4, 3), activation="tanh")),
+    ("bias must be", lambda: ho.linear_act(f(2, 3), f(4, 3), f(3))),
+    ("bias must have the type", lambda: ho.linear_act(f(2, 3), f(4, 3), f(4, dtype=torch.float16))),
+    ("residual must broadcast", lambda: ho.linear_act(f(2, 3), f(4, 3), residual=f(2, 5))),
+    ("residual must have the type", lambda: ho.linear_act(f(2, 3), f(4, 3), residual=f(2, 4, dtype=torch.float16))),
+    ("float32, bfloat16 or float16", lambda: ho.linear_act(f(2, 3, dtype=torch.float64), f(4, 3, dtype=torch.float64))),
+    ("at least one axis", lambda: ho.linear_act(torch.tensor(1.0), f(4, 3))),
+    # label_log_probs
+    ("labels must be a long", lambda: ho.label_log_probs(f(2, 3), torch.zeros(2, dtype=torch.int32))),
+    ("labels must be a tensor of shape", lambda: ho.label_log_probs(f(2, 3), torch.zeros(3, dtype=torch.int64))),
+    ("top must lie in", lambda: ho.label_log_probs(f(2, 3), torch.zeros(2, dtype=torch.int64), top=4)),
+    ("top must lie in", lambda: ho.label_log_probs(f(2, 300), torch.zeros(2, dtype=torch.int64), top=65)),
+    ("top must lie in", lambda: ho.label_log_probs(f(2, 3), torch.zeros(2, dtype=torch.int64), top=-1)),
+    ("at least one column", lambda: ho.label_log_probs(f(2, 0), torch.zeros(2, dtype=torch.int64))),
+    # distill_top_k
+    ("teacher_index must be a long", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int32), f(2, 1))),
+    ("must have shape", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 2, dtype=torch.int64), f(2, 1))),
+    ("teacher_index must be a tensor of shape", lambda: ho.distill_top_k(f(2, 3), torch.zeros(3, 1, dtype=torch.int64), f(2, 1))),
+    ("k >= 1", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 0, dtype=torch.int64), f(2, 0))),
+    ("temperature", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), f(2, 1), temperature=0.0)),
+    ("temperature", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), f(2, 1), temperature=float("inf"))),
+    ("temperature", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), f(2, 1), temperature=float("nan"))),
+    ("must not require a gradient",
+     lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), f(2, 1).requires_grad_())),
+]
+
+
+@pytest.mark.parametrize("match,call", REFUSALS, ids=[f"{i}" for i in range(len(REFUSALS))])
+def test_refusals(match, call):
+    with pytest.raises(RuntimeError, match=match):
+        call()
+
+
+def test_entry_points_refuse_bad_arguments_before_any_launch():
+    """Every argument check of the C entry points returns its code on the host (the pointers are never followed)."""
+    lib = _ext._lib
+    some, big = ctypes.c_void_p(16), 1 << 40
+    EINVAL, ENULL, ENOSPC = -1, -2, -4
+
+    def linear(M=4, N=4, K=4, dt=0, x=some, w=some, b=None, bdt=0, act=0, y=some, ws=None, nb=0):
+        return lib.pn2_linear_act(M, N, K, dt, x, K, w, K, b, bdt, act, None, 0, y, None, ws, nb, None)
+    assert linear(M=-1) == linear(N=0) == linear(K=0) == linear(dt=3) == linear(dt=-1) == linear(act=5) == linear(act=-1) == EINVAL
+    assert linear(dt=1, b=some, bdt=2) == linear(M=big) == linear(N=(1 << 22)) == EINVAL
+    assert linear(x=None) == linear(w=None) == linear(y=None) == ENULL
+    assert linear(M=0, x=None) == 0
+    # a product whose contraction is split needs its workspace
+    assert lib.pn2_linear_act_workspace_bytes(64, 64, 4096, 0) > 0
+    assert linear(M=64, N=64, K=4096) == ENOSPC
+    assert linear(M=64, N=64, K=4096, nb=big) == ENULL
+
+    def grad(M=4, dy=some, x=some, w=some, dx=some, dw=some, db=None, bdt=0, nb=big, ws=some):
+        return lib.pn2_linear_act_grad(M, 4, 4, 0, dy, 4, None, x, 4, w, 4, dx, dw, db, bdt, ws, nb, None)
+    assert grad(M=0) == grad(db=some, bdt=1) == EINVAL
+    assert grad(dy=None) == grad(x=None) == grad(w=None) == ENULL
+    assert lib.pn2_linear_act_grad_workspace_bytes(4, 4, 4, 0, 1, 7) > 0
+
+    def labels(T=4, V=8, dt=0, x=some, y=some, top=0, lp=some, tl=None):
+        return lib.pn2_label_logprobs(T, V, V, dt, x, y, -100, top, lp, some, None, tl, tl, None)
+    assert labels(T=-1) == labels(V=0) == labels(dt=7) == labels(top=9) == labels(top=-1) == labels(V=100, top=65) == EINVAL
+    assert labels(x=None) == labels(y=None) == labels(lp=None) == labels(top=1) == ENULL
+    assert labels(T=0, x=None) == 0
+
+    def distill(k=2, t=1.0, tdt=0, x=some):
+        return lib.pn2_distill_topk(4, 8, 8, 0, x, k, some, tdt, some, t, some, None, None)
+    assert distill(k=0) == distill(t=0.0) == distill(t=-1.0) == distill(t=float("nan")) == distill(t=float("inf")) == EINVAL
+    assert distill(tdt=3) == EINVAL and distill(x=None) == ENULL
