@@ -20,6 +20,9 @@ typedef float la_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 la_f16x8 __attribute__((ext_vector_type(8)));
 
+#ifndef LA_CFG
+#define LA_CFG 2, 4, 8, 4
+#endif
 enum { ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU };
 
 // 16-byte fragments: 8 16-bit contraction indices per lane, or 4 fp32 ones (lane group g of 16 holds k = 4 g .. 4 g + 3; the
@@ -39,8 +42,9 @@ __device__ __forceinline__ la_f32x4 la_mma(HdF32, hd_u32x4 q, hd_u32x4 p, la_f32
   return c;
 }
 
-// act(z) and its slope
-template <int ACT>
+// act(z) and its slope.  FAST (16-bit results): erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7, half a step of fp32 where
+// it counts), which shares its exponential with the slope; erff costs twice the instructions.
+template <int ACT, bool FAST>
 __device__ __forceinline__ void la_act(float z, float &y, float &d) {
   if constexpr (ACT == ACT_NONE) {
     y = z;
@@ -53,9 +57,21 @@ __device__ __forceinline__ void la_act(float z, float &y, float &d) {
     y = z * s;
     d = __fmaf_rn(y, 1.f - s, s);
   } else if constexpr (ACT == ACT_GELU) {
-    const float cdf = 0.5f + 0.5f * erff(z * 0.7071067811865476f);
+    const float e = hd_exp2(-0.5f * kHdLog2e * z * z);
+    float cdf;
+    if constexpr (FAST) {
+      const float t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f * 0.7071067811865476f, fabsf(z), 1.f));
+      float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
+      q = __fmaf_rn(q, t, 1.421413741f);
+      q = __fmaf_rn(q, t, -0.284496736f);
+      q = __fmaf_rn(q, t, 0.254829592f);
+      q *= 0.5f * t * e;                               // (1 - erf(|z| / sqrt 2)) / 2
+      cdf = z < 0.f ? q : 1.f - q;
+    } else {
+      cdf = __fmaf_rn(0.5f, erff(z * 0.7071067811865476f), 0.5f);
+    }
     y = z * cdf;
-    d = __fmaf_rn(z * 0.3989422804014327f, hd_exp2(-0.5f * kHdLog2e * z * z), cdf);
+    d = __fmaf_rn(z * 0.3989422804014327f, e, cdf);
   } else {
     // (1 + tanh u) / 2 = 1 / (1 + e^(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3); beyond |z| = 30 the gate is 0 or 1
     const float w = fminf(fmaxf(z, -30.f), 30.f), w2 = w * w;
@@ -99,14 +115,15 @@ __device__ __forceinline__ float la_bias(const Epilogue &e, long long j) {
 template <class T>
 __device__ __forceinline__ void la_finish_any(const Epilogue &e, long long N, long long i, long long j, float z) {
   typedef typename T::elem elem;
+  constexpr bool kFast = sizeof(elem) == 2;
   z += la_bias<T>(e, j);
   float y, d;
   switch (e.act) {
-    case ACT_RELU: la_act<ACT_RELU>(z, y, d); break;
-    case ACT_GELU: la_act<ACT_GELU>(z, y, d); break;
-    case ACT_GELU_TANH: la_act<ACT_GELU_TANH>(z, y, d); break;
-    case ACT_SILU: la_act<ACT_SILU>(z, y, d); break;
-    default: la_act<ACT_NONE>(z, y, d);
+    case ACT_RELU: la_act<ACT_RELU, kFast>(z, y, d); break;
+    case ACT_GELU: la_act<ACT_GELU, kFast>(z, y, d); break;
+    case ACT_GELU_TANH: la_act<ACT_GELU_TANH, kFast>(z, y, d); break;
+    case ACT_SILU: la_act<ACT_SILU, kFast>(z, y, d); break;
+    default: la_act<ACT_NONE, kFast>(z, y, d);
   }
   if (e.res) y += T::load((const elem *)e.res + i * e.ldr + j);
   ((elem *)e.y)[i * N + j] = T::round(y);
@@ -209,6 +226,309 @@ __global__ __launch_bounds__(256) void la_any_kernel(Product a) {
       }
 }
 
+// ------------------------------------------------------------------------------------------------------ the tile kernel
+// A workgroup of WI x WJ waves owns a tile of (WI TI 16) x (WJ TJ 16) results; a wave holds TI x TJ accumulators.  Operand tiles of
+// 64 bytes of contraction (32 16-bit or 16 fp32 indices) travel global -> LDS directly (global_load_lds, 16 bytes per lane) into a
+// ring of kStages slots, three steps ahead; one barrier per step.  A step's Q fragments and, one by one, its P fragments are read
+// from LDS while the matrix instructions of the step before run: nothing waits on LDS between two barriers.
+//
+// LDS layout (16-byte pieces; XOR swizzles, applied to the GLOBAL address of a lane because the direct load writes lane-linear):
+//   K operand: rows of 64 bytes, piece c of row r at c ^ ((r >> 2) ^ (r >> 4)) & 3: the 16 rows of a fragment hit 16 different
+//     16-byte bank groups in both fragment orders used below;
+//   R operand: 32 (16) contraction rows of the tile's columns, piece c of row k at c ^ f(k); 16-bit fragments are read with the
+//     transposing ds_read_b64_tr_b16 (lane 4 b + a of 16 gives row b, columns 4 a .. 4 a + 3 and receives column lane, rows 0 .. 3),
+//     fp32 ones element by element.
+// Q's fragments are a permutation of its rows: fragment u, row r is j = (r >> 2) 16 + 4 u + (r & 3) of a group of 64, so that a lane
+// ends up with 16 consecutive columns of one result row (32 bytes per store, full lines per 4 lanes).
+constexpr int kStages = 4;
+
+template <int V> struct LaInt { static constexpr int value = V; };
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void la_each(F f) {
+  if constexpr (I < N) {
+    f(LaInt<I>{});
+    la_each<N, I + 1>(f);
+  }
+}
+
+__device__ __forceinline__ unsigned la_lds(const void *p) {
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const char *)p;
+}
+// 64 lanes x 16 bytes, global (uniform base + lane offset) -> LDS (uniform base + 16 lane)
+__device__ __forceinline__ void la_dma(unsigned lds, unsigned long long base, unsigned off) {
+  // (inline asm: the builtin is counted into lgkmcnt too, and every ds_read would wait for it; awaited by la_wait)
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(off), "s"(base) : "memory");
+}
+// all but the last N direct loads of this wave have landed, all but its last D LDS operations are done
+template <int N, int D>
+__device__ __forceinline__ void la_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)" ::"n"(N), "n"(D) : "memory");
+}
+
+__device__ __forceinline__ int la_swz_k(int r) { return ((r >> 2) ^ (r >> 4)) & 3; }
+template <bool PERM>
+__device__ __forceinline__ int la_swz_r(int k) {
+  return PERM ? (k & 1) | ((k & 2) << 2) : ((k & 3) << 1) | (k & 8);
+}
+
+template <class T, bool ROWS, bool PERM, int B, int NT>
+struct Operand {
+  typedef typename T::elem elem;
+  static constexpr int VE = T::kPerVec, KB = 4 * VE, ES = (int)sizeof(elem), PER = B * 4 / NT;   // pieces per thread and step
+  static constexpr int PW = B / VE;                                                              // R operand: pieces per row
+  unsigned off[PER];               // lane offsets of the direct loads
+  unsigned long long base;         // advances by a step
+  unsigned step;
+  __device__ __forceinline__ void init(const void *g, long long ld, long long r0, long long R, long long k0, int tid) {
+    const elem *p = (const elem *)g;
+    base = (unsigned long long)(ROWS ? p + k0 * ld + r0 : p + r0 * ld + k0);
+    step = ROWS ? (unsigned)(KB * ld * ES) : 64u;
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int at = n * NT + tid;
+      if constexpr (!ROWS) {
+        const int r = at >> 2, c = (at & 3) ^ la_swz_k(r);
+        const long long rr = r0 + r < R ? r : R - 1 - r0;          // rows out of range repeat the last one: never stored
+        off[n] = (unsigned)(rr * ld * ES + c * 16);
+      } else {
+        const int k = at / PW, c = (at % PW) ^ la_swz_r<PERM>(k);
+        const long long cc = r0 + (long long)(c + 1) * VE <= R ? c * VE : R - VE - r0;
+        off[n] = (unsigned)(k * ld * ES + cc * ES);
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(unsigned lds, int wave) {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) la_dma(lds + (n * NT + wave * 64) * 16, base, off[n]);
+    base += step;
+  }
+  // the last, partial step: pieces through registers, out of range = 0
+  __device__ __forceinline__ void tail(char *lds, const void *g, long long ld, long long r0, long long R, long long k0, long long k1,
+                                       int tid) {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int at = n * NT + tid;
+      long long r, k, left;
+      if constexpr (!ROWS) {
+        r = r0 + (at >> 2);
+        k = k0 + ((at & 3) ^ la_swz_k(at >> 2)) * VE;
+        left = r < R ? k1 - k : 0;
+      } else {
+        k = k0 + at / PW;
+        r = r0 + ((at % PW) ^ la_swz_r<PERM>(at / PW)) * VE;
+        left = k < k1 ? R - r : 0;
+      }
+      const elem *src = (const elem *)g + (ROWS ? k * ld + r : r * ld + k);
+      hd_u32x4 w = {0, 0, 0, 0};
+      if (left >= VE) {
+        w = hd_load16<T>(src);
+      } else {
+        elem v[VE];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[i] = i < left ? src[i] : T::round(0.f);
+        __builtin_memcpy(&w, v, 16);
+      }
+      *reinterpret_cast<hd_u32x4 *>(lds + at * 16) = w;
+    }
+  }
+  // fragment t of the wave whose rows start at w0 (a multiple of 64)
+  __device__ __forceinline__ static hd_u32x4 frag(const char *lds, int w0, int t, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!ROWS) {
+      const int row = w0 + (PERM ? (t >> 2) * 64 + (r >> 2) * 16 + (t & 3) * 4 + (r & 3) : t * 16 + r);
+      return *reinterpret_cast<const hd_u32x4 *>(lds + row * 64 + ((g ^ la_swz_k(row)) << 4));
+    } else if constexpr (ES == 2) {
+      const int a = r & 3, b = r >> 2;
+      const int col = w0 + (PERM ? (t >> 2) * 64 + a * 16 + (t & 3) * 4 : t * 16 + a * 4);
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      s4 h[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int k = g * 8 + n * 4 + b;
+        const char *at = lds + k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
+        h[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
+      }
+      return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int col = w0 + (PERM ? (t >> 2) * 64 + (r >> 2) * 16 + (t & 3) * 4 + (r & 3) : t * 16 + r);
+      hd_u32x4 w;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int k = g * 4 + n;
+        w[n] = *reinterpret_cast<const unsigned *>(lds + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
+      }
+      return w;
+    }
+  }
+};
+
+// 8 consecutive results of one row
+template <class T, int ACT>
+__device__ __forceinline__ void la_finish8(const Product &a, long long i, long long j, const float (&acc)[8]) {
+  typedef typename T::elem elem;
+  typedef typename SlopeOf<T>::type S;
+  const Epilogue &e = a.e;
+  if (i >= a.M || j >= a.N) return;
+  if (j + 8 > a.N) {
+    for (int n = 0; j + n < a.N; ++n) {
+      float z = acc[0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) z = n == q ? acc[q] : z;
+      if (a.splits > 1) a.partial[((long long)blockIdx.z * a.M + i) * a.N + j + n] = z;
+      else la_finish_any<T>(e, a.N, i, j + n, z);
+    }
+    return;
+  }
+  if (a.splits > 1) {
+    float *p = a.partial + ((long long)blockIdx.z * a.M + i) * a.N + j;
+    float lo[4] = {acc[0], acc[1], acc[2], acc[3]}, hi[4] = {acc[4], acc[5], acc[6], acc[7]};
+    hd_store16<HdF32>(p, HdF32::pack(lo));
+    hd_store16<HdF32>(p + 4, HdF32::pack(hi));
+    return;
+  }
+  float y[8], d[8], b[8], r[8];
+  auto load8 = [](auto type, const void *base, long long at, float (&f)[8]) {
+    typedef decltype(type) Q;
+    const typename Q::elem *p = (const typename Q::elem *)base + at;
+    if constexpr (Q::kPerVec == 8) {
+      Q::unpack(hd_load16<Q>(p), f);
+    } else {
+      float lo[4], hi[4];
+      Q::unpack(hd_load16<Q>(p), lo);
+      Q::unpack(hd_load16<Q>(p + 4), hi);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) { f[n] = lo[n]; f[4 + n] = hi[n]; }
+    }
+  };
+  auto store8 = [](auto type, void *base, long long at, const float (&f)[8]) {
+    typedef decltype(type) Q;
+    typename Q::elem *p = (typename Q::elem *)base + at;
+    if constexpr (Q::kPerVec == 8) {
+      hd_store16<Q>(p, Q::pack(f));
+    } else {
+      float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+      hd_store16<Q>(p, Q::pack(lo));
+      hd_store16<Q>(p + 4, Q::pack(hi));
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < 8; ++n) b[n] = 0.f;
+  if (e.bias) {
+    if (e.bias_f32) load8(HdF32{}, e.bias, j, b);
+    else load8(T{}, e.bias, j, b);
+  }
+  if (e.res) load8(T{}, e.res, i * e.ldr + j, r);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    la_act<ACT, sizeof(elem) == 2>(acc[n] + b[n], y[n], d[n]);
+    if (e.res) y[n] += r[n];
+  }
+  store8(T{}, e.y, i * a.N + j, y);
+  if constexpr (ACT != ACT_NONE) {
+    if (e.slope) store8(S{}, e.slope, i * a.N + j, d);
+  }
+}
+
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
+__global__ __launch_bounds__(64 * WI * WJ, WI * WJ / 4) void la_tile_kernel(Product a, int gi, int gj) {
+  constexpr int NT = 64 * WI * WJ, BI = WI * TI * 16, BJ = WJ * TJ * 16, KB = 4 * T::kPerVec, STAGE = (BI + BJ) * 64;
+  typedef Operand<T, PROWS, false, BI, NT> OP;
+  typedef Operand<T, QROWS, true, BJ, NT> OQ;
+  __shared__ __align__(1024) char ring[kStages * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // workgroups go round robin over the 8 XCDs: give each XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that the
+  // operand panels of a band are shared in its L2
+  int ti, tj;
+  {
+    const int n = gi * gj, id = blockIdx.x, per = n / 8, rem = n % 8, x = id % 8, q = id / 8;
+    const int at = x * per + (x < rem ? x : rem) + q;
+    const int band = at / (8 * gj), rows = gi - band * 8 < 8 ? gi - band * 8 : 8, in = at - band * 8 * gj;
+    ti = band * 8 + in % rows;
+    tj = in / rows;
+  }
+  const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
+  const long long k0 = (long long)blockIdx.z * a.kchunk, k1 = k0 + a.kchunk < a.K ? k0 + a.kchunk : a.K;
+  const int steps = (int)((k1 - k0) / KB), rest = (int)((k1 - k0) % KB);
+  const int wi = (wave % WI) * TI * 16, wj = (wave / WI) * TJ * 16;
+  constexpr int L = OP::PER + OQ::PER;                 // direct loads per wave and step
+  OP op;
+  OQ oq;
+  op.init(a.p, a.ldp, i0, a.M, k0, tid);
+  oq.init(a.q, a.ldq, j0, a.N, k0, tid);
+  const unsigned lds0 = la_lds(ring);
+  auto issue = [&](int s) __attribute__((always_inline)) {
+    const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (s % kStages) * STAGE);
+    op.issue(at, wave);
+    oq.issue(at + BI * 64, wave);
+  };
+  la_f32x4 acc[TI][TJ] = {};
+  hd_u32x4 p[TI], q[2][TJ];
+  const int ahead = steps < kStages - 1 ? steps : kStages - 1;
+  for (int s = 0; s < ahead; ++s) issue(s);
+  // (steps >= 1: the host sends shorter contractions elsewhere)
+  if (steps >= 3) la_wait<2 * L, 0>();
+  else if (steps == 2) la_wait<L, 0>();
+  else la_wait<0, 0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int u = 0; u < TJ; ++u) q[0][u] = OQ::frag(ring + BI * 64, wj, u, lane);
+#pragma unroll
+  for (int t = 0; t < TI; ++t) p[t] = OP::frag(ring, wi, t, lane);
+  // one step: (A) its successor has landed for every wave, (B) the slot of its predecessor is refilled (its reads are done: they
+  // lie before the last step's, of which there are at least D), (C) products and reads
+  constexpr int D = TI + TJ < 15 ? TI + TJ : 15;
+  auto step = [&](int s, auto cur_) __attribute__((always_inline)) {
+    constexpr int cur = decltype(cur_)::value;
+    if (s + 2 < steps) la_wait<L, D>();
+    else la_wait<0, D>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (s + 3 < steps) issue(s + 3);
+    const char *next = ring + ((s + 1) % kStages) * STAGE;
+    // (the step after the last reads a slot that holds older data: in bounds, never used)
+#pragma unroll
+    for (int u = 0; u < TJ; ++u) q[cur ^ 1][u] = OQ::frag(next + BI * 64, wj, u, lane);
+#pragma unroll
+    for (int t = 0; t < TI; ++t) {
+#pragma unroll
+      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[cur][u], p[t], acc[t][u]);
+      p[t] = OP::frag(next, wi, t, lane);
+    }
+  };
+  int s = 0;
+  for (; s + 1 < steps; s += 2) {
+    step(s, LaInt<0>{});
+    step(s + 1, LaInt<1>{});
+  }
+  if (s < steps) step(s, LaInt<0>{});
+  if (rest) {
+    __syncthreads();
+    op.tail(ring, a.p, a.ldp, i0, a.M, k0 + (long long)steps * KB, k1, tid);
+    oq.tail(ring + BI * 64, a.q, a.ldq, j0, a.N, k0 + (long long)steps * KB, k1, tid);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < TJ; ++u) q[0][u] = OQ::frag(ring + BI * 64, wj, u, lane);
+#pragma unroll
+    for (int t = 0; t < TI; ++t) {
+      p[t] = OP::frag(ring, wi, t, lane);
+#pragma unroll
+      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[t], acc[t][u]);
+    }
+  }
+  // (static indices by construction: as a loop, the long body is unrolled too late for the accumulators to stay in registers)
+  la_each<TI * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
+    constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
+    const long long i = i0 + wi + t * 16 + (lane & 15), j = j0 + wj + (u >> 2) * 64 + (lane >> 4) * 16 + (u & 3) * 4;
+    float z[8];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) { z[n] = acc[t][u][n]; z[4 + n] = acc[t][u + 1][n]; }
+    la_finish8<T, ACT>(a, i, j, z);
+  });
+}
+
 // the split contraction joined in a fixed order, then the epilogue
 template <class T>
 __global__ __launch_bounds__(256) void la_join_kernel(Product a) {
@@ -280,6 +600,38 @@ bool la_vec(const void *p, long long ld, int dtype) {
   return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0;
 }
 
+// The tile kernel's direct loads need 16-byte pieces: aligned bases and strides, and axes that are whole pieces.
+bool la_tiled(const Product &a, int dtype, bool prows, bool qrows) {
+  const long long ve = dtype == PN2_DT_F32 ? 4 : 8;
+  return la_vec(a.p, a.ldp, dtype) && la_vec(a.q, a.ldq, dtype) && a.ldp <= (1 << 22) && a.ldq <= (1 << 22) &&
+         (prows ? a.M : a.K) % ve == 0 && (qrows ? a.N : a.K) % ve == 0 && a.K >= 4 * ve && a.M >= 128 && a.N >= 128;
+}
+
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
+int la_tile_as(const Product &a, hipStream_t st) {
+  const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
+  const dim3 grid((unsigned)(gi * gj), 1, (unsigned)a.splits);
+  constexpr int NT = 64 * WI * WJ;
+  if constexpr (PROWS || QROWS) {
+    la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+  } else {
+    switch (a.splits > 1 ? ACT_NONE : a.e.act) {       // (a split contraction's epilogue is the join kernel's)
+      case ACT_RELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_RELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU_TANH: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU_TANH><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_SILU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_SILU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+    }
+  }
+  if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 256), 256, 0, st>>>(a);
+  return pn2_check_launch();
+}
+
+template <class T, bool PROWS, bool QROWS>
+int la_tile(const Product &a, hipStream_t st) {
+  return la_tile_as<T, PROWS, QROWS, LA_CFG>(a, st);
+}
+
 template <class T, bool PROWS, bool QROWS>
 int la_product(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) {
   la_plan(a, dtype);
@@ -287,6 +639,7 @@ int la_product(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) 
   if (ws_bytes < need) return PN2_ENOSPC;
   if (need && !ws) return PN2_ENULL;
   a.partial = (float *)ws;
+  if (la_tiled(a, dtype, PROWS, QROWS)) return la_tile<T, PROWS, QROWS>(a, st);
   a.vecp = la_vec(a.p, a.ldp, dtype);
   a.vecq = la_vec(a.q, a.ldq, dtype);
   const long long gx = la_div(a.M, 64), gy = la_div(a.N, 64);

@@ -92,7 +92,7 @@ def tiny(dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 17, 5), (3, 7, 9), (72, 512, 256), (1, 300, 1001), (130, 65, 33), (64, 64, 64), (257, 129, 2048), (5, 1, 700),
-          (1003, 77, 101), (16, 4096, 128), (33, 520, 4104), (300, 264, 72)]
+          (1003, 77, 101), (16, 4096, 128), (33, 520, 4104), (300, 264, 72), (256, 256, 32), (512, 776, 328), (640, 1304, 4104), (1032, 136, 1000), (2100, 520, 264)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
