@@ -21,7 +21,7 @@ typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 la_f16x8 __attribute__((ext_vector_type(8)));
 
 #ifndef LA_CFG
-#define LA_CFG 2, 4, 8, 4
+#define LA_CFG 2, 4, 8, 4, 4
 #endif
 enum { ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU };
 
@@ -229,19 +229,18 @@ __global__ __launch_bounds__(256) void la_any_kernel(Product a) {
 // ------------------------------------------------------------------------------------------------------ the tile kernel
 // A workgroup of WI x WJ waves owns a tile of (WI TI 16) x (WJ TJ 16) results; a wave holds TI x TJ accumulators.  Operand tiles of
 // 64 bytes of contraction (32 16-bit or 16 fp32 indices) travel global -> LDS directly (global_load_lds, 16 bytes per lane) into a
-// ring of kStages slots, three steps ahead; one barrier per step.  A step's Q fragments and, one by one, its P fragments are read
+// ring of NS slots, NS - 1 steps ahead; one barrier per step.  A step's Q fragments and, one by one, its P fragments are read
 // from LDS while the matrix instructions of the step before run: nothing waits on LDS between two barriers.
 //
 // LDS layout (16-byte pieces; XOR swizzles, applied to the GLOBAL address of a lane because the direct load writes lane-linear):
-//   K operand: rows of 64 bytes, piece c of row r at c ^ ((r >> 2) ^ (r >> 4)) & 3: the 16 rows of a fragment hit 16 different
-//     16-byte bank groups in both fragment orders used below;
+//   K operand: rows of 64 bytes, piece c of row r at c ^ s(x), x the fragment row's group of four, s = 0 3 2 1: a ds_read_b128 takes
+//     16 lanes per cycle, {0-3, 12-15, 20-23, 24-27} and so on, and those hit 16 different pieces of 256 bytes (with s = 0 1 2 3,
+//     free of conflicts for 16 consecutive lanes, half the LDS cycles were conflicts: 8.0 against 4.0 a read);
 //   R operand: 32 (16) contraction rows of the tile's columns, piece c of row k at c ^ f(k); 16-bit fragments are read with the
 //     transposing ds_read_b64_tr_b16 (lane 4 b + a of 16 gives row b, columns 4 a .. 4 a + 3 and receives column lane, rows 0 .. 3),
 //     fp32 ones element by element.
 // Q's fragments are a permutation of its rows: fragment u, row r is j = (r >> 2) 16 + 4 u + (r & 3) of a group of 64, so that a lane
 // ends up with 16 consecutive columns of one result row (32 bytes per store, full lines per 4 lanes).
-constexpr int kStages = 4;
-
 template <int V> struct LaInt { static constexpr int value = V; };
 template <int N, int I = 0, class F>
 __device__ __forceinline__ void la_each(F f) {
@@ -267,7 +266,11 @@ __device__ __forceinline__ void la_wait() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)" ::"n"(N), "n"(D) : "memory");
 }
 
-__device__ __forceinline__ int la_swz_k(int r) { return ((r >> 2) ^ (r >> 4)) & 3; }
+template <bool PERM>
+__device__ __forceinline__ int la_swz_k(int r) {
+  const int x = PERM ? r >> 4 : r >> 2;                // the fragment row's group of four
+  return (x ^ (x << 1)) & 3;
+}
 template <bool PERM>
 __device__ __forceinline__ int la_swz_r(int k) {
   return PERM ? (k & 1) | ((k & 2) << 2) : ((k & 3) << 1) | (k & 8);
@@ -277,6 +280,7 @@ template <class T, bool ROWS, bool PERM, int B, int NT>
 struct Operand {
   typedef typename T::elem elem;
   static constexpr int VE = T::kPerVec, KB = 4 * VE, ES = (int)sizeof(elem), PER = B * 4 / NT;   // pieces per thread and step
+  static constexpr int READS = ROWS ? (ES == 2 ? 2 : 4) : 1;                                     // LDS reads per fragment
   static constexpr int PW = B / VE;                                                              // R operand: pieces per row
   unsigned off[PER];               // lane offsets of the direct loads
   unsigned long long base;         // advances by a step
@@ -289,7 +293,7 @@ struct Operand {
     for (int n = 0; n < PER; ++n) {
       const int at = n * NT + tid;
       if constexpr (!ROWS) {
-        const int r = at >> 2, c = (at & 3) ^ la_swz_k(r);
+        const int r = at >> 2, c = (at & 3) ^ la_swz_k<PERM>(r);
         const long long rr = r0 + r < R ? r : R - 1 - r0;          // rows out of range repeat the last one: never stored
         off[n] = (unsigned)(rr * ld * ES + c * 16);
       } else {
@@ -299,11 +303,7 @@ struct Operand {
       }
     }
   }
-  __device__ __forceinline__ void issue(unsigned lds, int wave) {
-#pragma unroll
-    for (int n = 0; n < PER; ++n) la_dma(lds + (n * NT + wave * 64) * 16, base, off[n]);
-    base += step;
-  }
+  __device__ __forceinline__ void issue(int n, unsigned lds, int wave) { la_dma(lds + (n * NT + wave * 64) * 16, base, off[n]); }
   // the last, partial step: pieces through registers, out of range = 0
   __device__ __forceinline__ void tail(char *lds, const void *g, long long ld, long long r0, long long R, long long k0, long long k1,
                                        int tid) {
@@ -313,7 +313,7 @@ struct Operand {
       long long r, k, left;
       if constexpr (!ROWS) {
         r = r0 + (at >> 2);
-        k = k0 + ((at & 3) ^ la_swz_k(at >> 2)) * VE;
+        k = k0 + ((at & 3) ^ la_swz_k<PERM>(at >> 2)) * VE;
         left = r < R ? k1 - k : 0;
       } else {
         k = k0 + at / PW;
@@ -333,110 +333,114 @@ struct Operand {
       *reinterpret_cast<hd_u32x4 *>(lds + at * 16) = w;
     }
   }
-  // fragment t of the wave whose rows start at w0 (a multiple of 64)
-  __device__ __forceinline__ static hd_u32x4 frag(const char *lds, int w0, int t, int lane) {
+  // Fragment t of the wave whose rows start at w0 (a multiple of 64) = frag(slot + lane_base(w0), t): a lane's offsets differ between
+  // fragments by a constant, or by a constant exclusive-or.
+  __device__ __forceinline__ static unsigned lane_base(int w0, int lane) {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!ROWS) {
-      const int row = w0 + (PERM ? (t >> 2) * 64 + (r >> 2) * 16 + (t & 3) * 4 + (r & 3) : t * 16 + r);
-      return *reinterpret_cast<const hd_u32x4 *>(lds + row * 64 + ((g ^ la_swz_k(row)) << 4));
+      const int row = w0 + (PERM ? (r >> 2) * 16 + (r & 3) : r);           // (its swizzle does not depend on t)
+      return row * 64 + ((g ^ la_swz_k<PERM>(row)) << 4);
     } else if constexpr (ES == 2) {
-      const int a = r & 3, b = r >> 2;
-      const int col = w0 + (PERM ? (t >> 2) * 64 + a * 16 + (t & 3) * 4 : t * 16 + a * 4);
-      typedef short s4 __attribute__((ext_vector_type(4)));
-      s4 h[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int k = g * 8 + n * 4 + b;
-        const char *at = lds + k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
-        h[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
-      }
-      return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      const int a = r & 3, k = g * 8 + (r >> 2), col = w0 + a * (PERM ? 16 : 4);
+      return k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
     } else {
-      const int col = w0 + (PERM ? (t >> 2) * 64 + (r >> 2) * 16 + (t & 3) * 4 + (r & 3) : t * 16 + r);
+      return w0 + (PERM ? (r >> 2) * 16 + (r & 3) : r);                    // (the column; fp32 pays the address of every element)
+    }
+  }
+  __device__ __forceinline__ static hd_u32x4 frag(unsigned slot, unsigned base, int t, int lane) {
+    typedef __attribute__((address_space(3))) const hd_u32x4 *lds16;
+    if constexpr (!ROWS) {
+      return *(lds16)(slot + base + (PERM ? (t >> 2) * 4096 + (t & 3) * 256 : t * 1024));
+    } else if constexpr (ES == 2) {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4 *lds8;
+      // natural: 16 columns are 2 pieces;  permuted: 4 columns are half a piece
+      const unsigned at = (slot + base) ^ (PERM ? ((t >> 2) << 7) | (((t >> 1) & 1) << 4) : t << 5);
+      const unsigned half = PERM ? (t & 1) * 8 : 0;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(at + half));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(at + half + 4 * B * 2));       // four rows on: the same swizzle
+      return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int col = (int)base + (PERM ? (t >> 2) * 64 + (t & 3) * 4 : t * 16);
       hd_u32x4 w;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int k = g * 4 + n;
-        w[n] = *reinterpret_cast<const unsigned *>(lds + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
+        const int k = (lane >> 4) * 4 + n;
+        w[n] = *(__attribute__((address_space(3))) const unsigned *)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
       }
       return w;
     }
   }
 };
 
-// 8 consecutive results of one row
-template <class T, int ACT>
-__device__ __forceinline__ void la_finish8(const Product &a, long long i, long long j, const float (&acc)[8]) {
-  typedef typename T::elem elem;
-  typedef typename SlopeOf<T>::type S;
-  const Epilogue &e = a.e;
-  if (i >= a.M || j >= a.N) return;
-  if (j + 8 > a.N) {
-    for (int n = 0; j + n < a.N; ++n) {
-      float z = acc[0];
-#pragma unroll
-      for (int q = 1; q < 8; ++q) z = n == q ? acc[q] : z;
-      if (a.splits > 1) a.partial[((long long)blockIdx.z * a.M + i) * a.N + j + n] = z;
-      else la_finish_any<T>(e, a.N, i, j + n, z);
-    }
-    return;
-  }
-  if (a.splits > 1) {
-    float *p = a.partial + ((long long)blockIdx.z * a.M + i) * a.N + j;
-    float lo[4] = {acc[0], acc[1], acc[2], acc[3]}, hi[4] = {acc[4], acc[5], acc[6], acc[7]};
-    hd_store16<HdF32>(p, HdF32::pack(lo));
-    hd_store16<HdF32>(p + 4, HdF32::pack(hi));
-    return;
-  }
-  float y[8], d[8], b[8], r[8];
-  auto load8 = [](auto type, const void *base, long long at, float (&f)[8]) {
-    typedef decltype(type) Q;
-    const typename Q::elem *p = (const typename Q::elem *)base + at;
-    if constexpr (Q::kPerVec == 8) {
-      Q::unpack(hd_load16<Q>(p), f);
+// 8 consecutive elements, the first `left` of them in range (the others 0)
+template <class T>
+__device__ __forceinline__ void la_load8(const typename T::elem *p, long long left, float (&f)[8]) {
+  if (left >= 8) {
+    if constexpr (T::kPerVec == 8) {
+      T::unpack(hd_load16<T>(p), f);
     } else {
       float lo[4], hi[4];
-      Q::unpack(hd_load16<Q>(p), lo);
-      Q::unpack(hd_load16<Q>(p + 4), hi);
+      T::unpack(hd_load16<T>(p), lo);
+      T::unpack(hd_load16<T>(p + 4), hi);
 #pragma unroll
       for (int n = 0; n < 4; ++n) { f[n] = lo[n]; f[4 + n] = hi[n]; }
     }
-  };
-  auto store8 = [](auto type, void *base, long long at, const float (&f)[8]) {
-    typedef decltype(type) Q;
-    typename Q::elem *p = (typename Q::elem *)base + at;
-    if constexpr (Q::kPerVec == 8) {
-      hd_store16<Q>(p, Q::pack(f));
+  } else {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) f[n] = n < left ? T::load(p + n) : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void la_store8(typename T::elem *p, long long left, const float (&f)[8]) {
+  if (left >= 8) {
+    if constexpr (T::kPerVec == 8) {
+      hd_store16<T>(p, T::pack(f));
     } else {
       float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-      hd_store16<Q>(p, Q::pack(lo));
-      hd_store16<Q>(p + 4, Q::pack(hi));
+      hd_store16<T>(p, T::pack(lo));
+      hd_store16<T>(p + 4, T::pack(hi));
     }
-  };
+  } else {
 #pragma unroll
-  for (int n = 0; n < 8; ++n) b[n] = 0.f;
-  if (e.bias) {
-    if (e.bias_f32) load8(HdF32{}, e.bias, j, b);
-    else load8(T{}, e.bias, j, b);
-  }
-  if (e.res) load8(T{}, e.res, i * e.ldr + j, r);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    la_act<ACT, sizeof(elem) == 2>(acc[n] + b[n], y[n], d[n]);
-    if (e.res) y[n] += r[n];
-  }
-  store8(T{}, e.y, i * a.N + j, y);
-  if constexpr (ACT != ACT_NONE) {
-    if (e.slope) store8(S{}, e.slope, i * a.N + j, d);
+    for (int n = 0; n < 8; ++n)
+      if (n < left) p[n] = T::round(f[n]);
   }
 }
 
-template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
-__global__ __launch_bounds__(64 * WI * WJ, WI * WJ / 4) void la_tile_kernel(Product a, int gi, int gj) {
+// 8 consecutive results of one row: bias b and residual r are at hand (loads between the stores would wait for each other)
+template <class T, int ACT>
+__device__ __forceinline__ void la_finish8(const Product &a, long long i, long long j, const float *acc, const float *b,
+                                           const float (&r)[8]) {
+  typedef typename T::elem elem;
+  typedef typename SlopeOf<T>::type S;
+  const long long left = i < a.M ? a.N - j : 0;
+  if (left <= 0) return;
+  float y[8], d[8];
+  if (a.splits > 1) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) y[n] = acc[n];
+    la_store8<HdF32>(a.partial + ((long long)blockIdx.z * a.M + i) * a.N + j, left, y);
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    la_act<ACT, sizeof(elem) == 2>(acc[n] + b[n], y[n], d[n]);
+    y[n] += r[n];
+  }
+  la_store8<T>((elem *)a.e.y + i * a.N + j, left, y);
+  if constexpr (ACT != ACT_NONE) {
+    if (a.e.slope) la_store8<S>((typename S::elem *)a.e.slope + i * a.N + j, left, d);
+  }
+}
+
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS, int ACT>
+__global__ __launch_bounds__(64 * WI * WJ, TI * TJ > 32 ? 1 : 2) void la_tile_kernel(Product a, int gi, int gj) {
   constexpr int NT = 64 * WI * WJ, BI = WI * TI * 16, BJ = WJ * TJ * 16, KB = 4 * T::kPerVec, STAGE = (BI + BJ) * 64;
+  typedef typename T::elem elem;
   typedef Operand<T, PROWS, false, BI, NT> OP;
   typedef Operand<T, QROWS, true, BJ, NT> OQ;
-  __shared__ __align__(1024) char ring[kStages * STAGE];
+  __shared__ __align__(1024) char ring[NS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups go round robin over the 8 XCDs: give each XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that the
   // operand panels of a band are shared in its L2
@@ -458,74 +462,115 @@ __global__ __launch_bounds__(64 * WI * WJ, WI * WJ / 4) void la_tile_kernel(Prod
   op.init(a.p, a.ldp, i0, a.M, k0, tid);
   oq.init(a.q, a.ldq, j0, a.N, k0, tid);
   const unsigned lds0 = la_lds(ring);
-  auto issue = [&](int s) __attribute__((always_inline)) {
-    const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (s % kStages) * STAGE);
-    op.issue(at, wave);
-    oq.issue(at + BI * 64, wave);
-  };
-  la_f32x4 acc[TI][TJ] = {};
-  hd_u32x4 p[TI], q[2][TJ];
-  const int ahead = steps < kStages - 1 ? steps : kStages - 1;
-  for (int s = 0; s < ahead; ++s) issue(s);
-  // (steps >= 1: the host sends shorter contractions elsewhere)
-  if (steps >= 3) la_wait<2 * L, 0>();
-  else if (steps == 2) la_wait<L, 0>();
-  else la_wait<0, 0>();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-#pragma unroll
-  for (int u = 0; u < TJ; ++u) q[0][u] = OQ::frag(ring + BI * 64, wj, u, lane);
-#pragma unroll
-  for (int t = 0; t < TI; ++t) p[t] = OP::frag(ring, wi, t, lane);
-  // one step: (A) its successor has landed for every wave, (B) the slot of its predecessor is refilled (its reads are done: they
-  // lie before the last step's, of which there are at least D), (C) products and reads
-  constexpr int D = TI + TJ < 15 ? TI + TJ : 15;
-  auto step = [&](int s, auto cur_) __attribute__((always_inline)) {
-    constexpr int cur = decltype(cur_)::value;
-    if (s + 2 < steps) la_wait<L, D>();
-    else la_wait<0, D>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + 3 < steps) issue(s + 3);
-    const char *next = ring + ((s + 1) % kStages) * STAGE;
-    // (the step after the last reads a slot that holds older data: in bounds, never used)
-#pragma unroll
-    for (int u = 0; u < TJ; ++u) q[cur ^ 1][u] = OQ::frag(next + BI * 64, wj, u, lane);
-#pragma unroll
-    for (int t = 0; t < TI; ++t) {
-#pragma unroll
-      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[cur][u], p[t], acc[t][u]);
-      p[t] = OP::frag(next, wi, t, lane);
+  // direct load n of the next step; beyond the last step it repeats that one (in bounds, into a slot nobody reads any more), so that
+  // the loop has no branches and its waits are constants
+  int issued = 0;
+  auto issue = [&](int n) __attribute__((always_inline)) {
+    const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (issued % NS) * STAGE);
+    if (n < OP::PER) op.issue(n, at, wave);
+    else oq.issue(n - OP::PER, at + BI * 64, wave);
+    if (n == L - 1) {
+      ++issued;
+      op.base += issued < steps ? op.step : 0;
+      oq.base += issued < steps ? oq.step : 0;
     }
   };
-  int s = 0;
-  for (; s + 1 < steps; s += 2) {
-    step(s, LaInt<0>{});
-    step(s + 1, LaInt<1>{});
+  la_f32x4 acc[TI][TJ] = {};
+  hd_u32x4 p[2][TI], q[2][TJ];
+  constexpr int A = NS - 1;                            // steps in flight
+  // fragment n of a step, Q's first
+  const unsigned pb = OP::lane_base(wi, lane), qb = OQ::lane_base(wj, lane) + (QROWS && sizeof(elem) == 4 ? 0 : BI * 64);
+  auto read = [&](unsigned at, int n, int buf) __attribute__((always_inline)) {
+    if (n < TJ) q[buf][n] = OQ::frag(QROWS && sizeof(elem) == 4 ? at + BI * 64 : at, qb, n, lane);
+    else p[buf][n - TJ] = OP::frag(at, pb, n - TJ, lane);
+  };
+  // One step: (A) its successor has landed for every wave; (B) the slot of its predecessor is refilled: every wave's reads of it are
+  // done, they lie before the last step's, of which there are at least D; (C) products, one fragment of the successor read after
+  // each of the first ones, then the direct loads.  The order is pinned: left to itself the compiler sinks the reads, and the next
+  // step waits for them; loads before the products leave the matrix cores idle behind each barrier.
+  constexpr int D = TI + TJ < 15 ? TI + TJ : 15;
+  constexpr int GAP = TI * TJ * 3 / 4 / (TI + TJ), LGAP = TI * TJ * 3 / 4 / L;
+  static_assert(GAP > 0 && LGAP > 0, "room for the reads and the loads between the products");
+  auto step = [&](int s, auto cur_) __attribute__((always_inline)) {
+    constexpr int cur = decltype(cur_)::value;
+    la_wait<(A - 2) * L, D>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // (the step after the last one reads a slot of older data: in bounds, never used)
+    const unsigned next = lds0 + ((s + 1) % NS) * STAGE;
+    la_each<TI * TJ>([&](auto n_) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_)::value, t = n / TJ, u = n % TJ;
+      acc[t][u] = la_mma(T{}, q[cur][u], p[cur][t], acc[t][u]);
+      if constexpr (n % GAP == 0 && n / GAP < TI + TJ) read(next, n / GAP, cur ^ 1);
+      if constexpr (n % LGAP == LGAP / 2 && n / LGAP < L) issue(n / LGAP);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  if (steps > 0) {
+    for (int s = 0; s < A; ++s)
+#pragma unroll
+      for (int n = 0; n < L; ++n) issue(n);
+    la_wait<(A - 1) * L, 0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < TI + TJ; ++n) read(lds0, n, 0);
+    int s = 0;
+    for (; s + 1 < steps; s += 2) {
+      step(s, LaInt<0>{});
+      step(s + 1, LaInt<1>{});
+    }
+    if (s < steps) step(s, LaInt<0>{});
+    la_wait<0, 0>();                                   // no direct load is left when the workgroup gives its LDS back
   }
-  if (s < steps) step(s, LaInt<0>{});
   if (rest) {
     __syncthreads();
     op.tail(ring, a.p, a.ldp, i0, a.M, k0 + (long long)steps * KB, k1, tid);
     oq.tail(ring + BI * 64, a.q, a.ldq, j0, a.N, k0 + (long long)steps * KB, k1, tid);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < TJ; ++u) q[0][u] = OQ::frag(ring + BI * 64, wj, u, lane);
+    for (int n = 0; n < TI + TJ; ++n) read(lds0, n, 0);
 #pragma unroll
-    for (int t = 0; t < TI; ++t) {
-      p[t] = OP::frag(ring, wi, t, lane);
+    for (int t = 0; t < TI; ++t)
 #pragma unroll
-      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[t], acc[t][u]);
+      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[0][t], acc[t][u]);
+  }
+  // A lane's columns: 8 (TJ / 2) runs of ... (u >> 2) 64 + (lane >> 4) 16 + (u & 3) 4, u even.  The bias of all of them and the
+  // residual of GT rows at a time are read before the first store.
+  const long long jl = j0 + wj + (lane >> 4) * 16;
+  auto col = [&](int u) { return jl + (u >> 2) * 64 + (u & 3) * 4; };
+  float b[TJ / 2][8];
+  const bool whole = a.splits == 1;
+#pragma unroll
+  for (int u = 0; u < TJ; u += 2) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) b[u / 2][n] = 0.f;
+    if (whole && a.e.bias) {
+      if (a.e.bias_f32) la_load8<HdF32>((const float *)a.e.bias + col(u), a.N - col(u), b[u / 2]);
+      else la_load8<T>((const elem *)a.e.bias + col(u), a.N - col(u), b[u / 2]);
     }
   }
   // (static indices by construction: as a loop, the long body is unrolled too late for the accumulators to stay in registers)
-  la_each<TI * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
-    constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
-    const long long i = i0 + wi + t * 16 + (lane & 15), j = j0 + wj + (u >> 2) * 64 + (lane >> 4) * 16 + (u & 3) * 4;
-    float z[8];
+  constexpr int GT = 2;
+  la_each<TI / GT>([&](auto g_) __attribute__((always_inline)) {
+    constexpr int t0 = decltype(g_)::value * GT;
+    float r[GT][TJ / 2][8];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) { z[n] = acc[t][u][n]; z[4 + n] = acc[t][u + 1][n]; }
-    la_finish8<T, ACT>(a, i, j, z);
+    for (int t = 0; t < GT; ++t)
+#pragma unroll
+      for (int u = 0; u < TJ; u += 2) {
+        const long long i = i0 + wi + (t0 + t) * 16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) r[t][u / 2][n] = 0.f;
+        if (whole && a.e.res && i < a.M) la_load8<T>((const elem *)a.e.res + i * a.e.ldr + col(u), a.N - col(u), r[t][u / 2]);
+      }
+    la_each<GT * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
+      constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
+      float z[8];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) { z[n] = acc[t0 + t][u][n]; z[4 + n] = acc[t0 + t][u + 1][n]; }
+      la_finish8<T, ACT>(a, i0 + wi + (t0 + t) * 16 + (lane & 15), col(u), z, b[u / 2], r[t][u / 2]);
+    });
   });
 }
 
@@ -607,20 +652,20 @@ bool la_tiled(const Product &a, int dtype, bool prows, bool qrows) {
          (prows ? a.M : a.K) % ve == 0 && (qrows ? a.N : a.K) % ve == 0 && a.K >= 4 * ve && a.M >= 128 && a.N >= 128;
 }
 
-template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS>
 int la_tile_as(const Product &a, hipStream_t st) {
   const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
   const dim3 grid((unsigned)(gi * gj), 1, (unsigned)a.splits);
   constexpr int NT = 64 * WI * WJ;
   if constexpr (PROWS || QROWS) {
-    la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+    la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, NS, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
   } else {
     switch (a.splits > 1 ? ACT_NONE : a.e.act) {       // (a split contraction's epilogue is the join kernel's)
-      case ACT_RELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_RELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_GELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_GELU_TANH: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU_TANH><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_SILU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_SILU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+      case ACT_RELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_RELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_GELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU_TANH: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_GELU_TANH><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_SILU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_SILU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
     }
   }
   if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 256), 256, 0, st>>>(a);
