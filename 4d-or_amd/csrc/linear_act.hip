@@ -20,9 +20,6 @@ typedef float la_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 la_f16x8 __attribute__((ext_vector_type(8)));
 
-#ifndef LA_CFG
-#define LA_CFG 2, 4, 8, 4, 4
-#endif
 enum { ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU };
 
 // 16-byte fragments: 8 16-bit contraction indices per lane, or 4 fp32 ones (lane group g of 16 holds k = 4 g .. 4 g + 3; the
@@ -57,21 +54,23 @@ __device__ __forceinline__ void la_act(float z, float &y, float &d) {
     y = z * s;
     d = __fmaf_rn(y, 1.f - s, s);
   } else if constexpr (ACT == ACT_GELU) {
-    const float e = hd_exp2(-0.5f * kHdLog2e * z * z);
-    float cdf;
+    const float e = hd_exp2(-0.5f * kHdLog2e * (z * z));
     if constexpr (FAST) {
-      const float t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f * 0.7071067811865476f, fabsf(z), 1.f));
-      float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
-      q = __fmaf_rn(q, t, 1.421413741f);
-      q = __fmaf_rn(q, t, -0.284496736f);
-      q = __fmaf_rn(q, t, 0.254829592f);
-      q *= 0.5f * t * e;                               // (1 - erf(|z| / sqrt 2)) / 2
-      cdf = z < 0.f ? q : 1.f - q;
+      // tail = (1 - erf(|z| / sqrt 2)) / 2 = e w:  act = max(z, 0) - |z| tail,  slope = [z > 0] + sign(z) (|z| pdf - tail)
+      const float m = fminf(fabsf(z), 1e30f), t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f * 0.7071067811865476f, m, 1.f));
+      float w = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+      w = __fmaf_rn(w, t, 0.5f * 1.421413741f);
+      w = __fmaf_rn(w, t, 0.5f * -0.284496736f);
+      w = __fmaf_rn(w, t, 0.5f * 0.254829592f);
+      w *= t;
+      y = __fmaf_rn(-m, e * w, z <= 0.f ? 0.f : z);    // (NaN stays NaN)
+      const float h = e * __fmaf_rn(0.3989422804014327f, m, -w);
+      d = z > 0.f ? 1.f + h : -h;
     } else {
-      cdf = __fmaf_rn(0.5f, erff(z * 0.7071067811865476f), 0.5f);
+      const float cdf = __fmaf_rn(0.5f, erff(z * 0.7071067811865476f), 0.5f);
+      y = z * cdf;
+      d = __fmaf_rn(z * 0.3989422804014327f, e, cdf);
     }
-    y = z * cdf;
-    d = __fmaf_rn(z * 0.3989422804014327f, e, cdf);
   } else {
     // (1 + tanh u) / 2 = 1 / (1 + e^(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3); beyond |z| = 30 the gate is 0 or 1
     const float w = fminf(fmaxf(z, -30.f), 30.f), w2 = w * w;
@@ -99,7 +98,6 @@ struct Product {
   long long M, N, K;
   const void *p, *q;
   long long ldp, ldq;
-  int vecp, vecq;           // rows 16-byte aligned: vector loads
   int splits;
   long long kchunk;         // contraction indices per split (a multiple of the tile's)
   float *partial;           // splits > 1: (splits, M, N)
@@ -139,7 +137,7 @@ struct TileLoad {
   typedef typename T::elem elem;
   static constexpr int VE = T::kPerVec, KB = 4 * VE, LDT = 80 / (int)sizeof(elem);
   hd_u32x4 w;
-  __device__ __forceinline__ void fetch(const elem *g, long long ld, int vec, long long r0, long long R, long long k0, long long k1,
+  __device__ __forceinline__ void fetch(const elem *g, long long ld, long long r0, long long R, long long k0, long long k1,
                                         int tid) {
     long long r, k, n;
     const elem *src;
@@ -155,7 +153,7 @@ struct TileLoad {
       n = k < k1 ? R - r : 0;
       src = g + k * ld + r;
     }
-    if (vec && n >= VE) {
+    if (n >= VE) {
       w = hd_load16<T>(src);
     } else {
       elem v[VE];
@@ -190,15 +188,15 @@ __global__ __launch_bounds__(256) void la_any_kernel(Product a) {
   la_f32x4 acc[2][2] = {};
   TileLoad<T, PROWS> lp;
   TileLoad<T, QROWS> lq;
-  lp.fetch((const elem *)a.p, a.ldp, a.vecp, i0, a.M, k0, k1, tid);
-  lq.fetch((const elem *)a.q, a.ldq, a.vecq, j0, a.N, k0, k1, tid);
+  lp.fetch((const elem *)a.p, a.ldp, i0, a.M, k0, k1, tid);
+  lq.fetch((const elem *)a.q, a.ldq, j0, a.N, k0, k1, tid);
   for (long long k = k0; k < k1; k += KB) {
     lp.store(sp, tid);
     lq.store(sq, tid);
     __syncthreads();
     if (k + KB < k1) {
-      lp.fetch((const elem *)a.p, a.ldp, a.vecp, i0, a.M, k + KB, k1, tid);
-      lq.fetch((const elem *)a.q, a.ldq, a.vecq, j0, a.N, k + KB, k1, tid);
+      lp.fetch((const elem *)a.p, a.ldp, i0, a.M, k + KB, k1, tid);
+      lq.fetch((const elem *)a.q, a.ldq, j0, a.N, k + KB, k1, tid);
     }
     hd_u32x4 fp[2], fq[2];
     const int r = lane & 15, c = (lane >> 4) * T::kPerVec;
@@ -350,15 +348,15 @@ struct Operand {
   __device__ __forceinline__ static hd_u32x4 frag(unsigned slot, unsigned base, int t, int lane) {
     typedef __attribute__((address_space(3))) const hd_u32x4 *lds16;
     if constexpr (!ROWS) {
-      return *(lds16)(slot + base + (PERM ? (t >> 2) * 4096 + (t & 3) * 256 : t * 1024));
+      return *(lds16)(size_t)(slot + base + (PERM ? (t >> 2) * 4096 + (t & 3) * 256 : t * 1024));
     } else if constexpr (ES == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4 *lds8;
       // natural: 16 columns are 2 pieces;  permuted: 4 columns are half a piece
       const unsigned at = (slot + base) ^ (PERM ? ((t >> 2) << 7) | (((t >> 1) & 1) << 4) : t << 5);
       const unsigned half = PERM ? (t & 1) * 8 : 0;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(at + half));
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(at + half + 4 * B * 2));       // four rows on: the same swizzle
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half + 4 * B * 2));       // four rows on: the same swizzle
       return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       const int col = (int)base + (PERM ? (t >> 2) * 64 + (t & 3) * 4 : t * 16);
@@ -366,17 +364,17 @@ struct Operand {
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int k = (lane >> 4) * 4 + n;
-        w[n] = *(__attribute__((address_space(3))) const unsigned *)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
+        w[n] = *(__attribute__((address_space(3))) const unsigned *)(size_t)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
       }
       return w;
     }
   }
 };
 
-// 8 consecutive elements, the first `left` of them in range (the others 0)
-template <class T>
+// 8 consecutive elements; FULL: all of them in range, otherwise the first `left` (the others 0)
+template <class T, bool FULL>
 __device__ __forceinline__ void la_load8(const typename T::elem *p, long long left, float (&f)[8]) {
-  if (left >= 8) {
+  if (FULL || left >= 8) {
     if constexpr (T::kPerVec == 8) {
       T::unpack(hd_load16<T>(p), f);
     } else {
@@ -391,9 +389,9 @@ __device__ __forceinline__ void la_load8(const typename T::elem *p, long long le
     for (int n = 0; n < 8; ++n) f[n] = n < left ? T::load(p + n) : 0.f;
   }
 }
-template <class T>
+template <class T, bool FULL>
 __device__ __forceinline__ void la_store8(typename T::elem *p, long long left, const float (&f)[8]) {
-  if (left >= 8) {
+  if (FULL || left >= 8) {
     if constexpr (T::kPerVec == 8) {
       hd_store16<T>(p, T::pack(f));
     } else {
@@ -408,30 +406,68 @@ __device__ __forceinline__ void la_store8(typename T::elem *p, long long left, c
   }
 }
 
-// 8 consecutive results of one row: bias b and residual r are at hand (loads between the stores would wait for each other)
-template <class T, int ACT>
-__device__ __forceinline__ void la_finish8(const Product &a, long long i, long long j, const float *acc, const float *b,
-                                           const float (&r)[8]) {
+// The accumulators of a wave (its first row i, its lane's first column j) -> results.  A lane's columns are runs of 8 at
+// j + (u >> 2) 64 + (u & 3) 4, u even.  FULL: the tile lies inside the matrix (no guards).  The bias of all columns and the residual
+// of two rows at a time are read before the stores (loads between stores would wait for each other).
+template <class T, int ACT, bool FULL, bool RES, int TI, int TJ>
+__device__ __forceinline__ void la_epilogue(const Product &a, const la_f32x4 (&acc)[TI][TJ], long long i, long long j) {
   typedef typename T::elem elem;
   typedef typename SlopeOf<T>::type S;
-  const long long left = i < a.M ? a.N - j : 0;
-  if (left <= 0) return;
-  float y[8], d[8];
-  if (a.splits > 1) {
+  const Epilogue &e = a.e;
+  auto col = [&](int u) { return j + (u >> 2) * 64 + (u & 3) * 4; };
+  float b[TJ / 2][8];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) y[n] = acc[n];
-    la_store8<HdF32>(a.partial + ((long long)blockIdx.z * a.M + i) * a.N + j, left, y);
-    return;
-  }
+  for (int u = 0; u < TJ; u += 2) {
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    la_act<ACT, sizeof(elem) == 2>(acc[n] + b[n], y[n], d[n]);
-    y[n] += r[n];
+    for (int n = 0; n < 8; ++n) b[u / 2][n] = 0.f;
+    if (e.bias) {
+      if (e.bias_f32) la_load8<HdF32, FULL>((const float *)e.bias + col(u), a.N - col(u), b[u / 2]);
+      else la_load8<T, FULL>((const elem *)e.bias + col(u), a.N - col(u), b[u / 2]);
+    }
   }
-  la_store8<T>((elem *)a.e.y + i * a.N + j, left, y);
-  if constexpr (ACT != ACT_NONE) {
-    if (a.e.slope) la_store8<S>((typename S::elem *)a.e.slope + i * a.N + j, left, d);
-  }
+  // (static indices by construction: as a loop, the long body is unrolled too late for the accumulators to stay in registers)
+  la_each<TI / 2>([&](auto g_) __attribute__((always_inline)) {
+    constexpr int t0 = decltype(g_)::value * 2;
+    float r[2][TJ / 2][8];
+    if constexpr (RES) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < TJ; u += 2) {
+          const long long row = i + (t0 + t) * 16;
+          la_load8<T, FULL>((const elem *)e.res + row * e.ldr + col(u), FULL || row < a.M ? a.N - col(u) : 0, r[t][u / 2]);
+        }
+    }
+    la_each<TJ>([&](auto n_) __attribute__((always_inline)) {
+      constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
+      const long long row = i + (t0 + t) * 16, left = FULL || row < a.M ? a.N - col(u) : 0;
+      if (!FULL && left <= 0) return;
+      float y[8], d[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        la_act<ACT, sizeof(elem) == 2>(acc[t0 + t][u + n / 4][n % 4] + b[u / 2][n], y[n], d[n]);
+        if constexpr (RES) y[n] += r[t][u / 2][n];
+      }
+      la_store8<T, FULL>((elem *)e.y + row * a.N + col(u), left, y);
+      if constexpr (ACT != ACT_NONE) {
+        if (e.slope) la_store8<S, FULL>((typename S::elem *)e.slope + row * a.N + col(u), left, d);
+      }
+    });
+  });
+}
+
+// ... -> the partial sums of a split contraction
+template <int TI, int TJ>
+__device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&acc)[TI][TJ], long long i, long long j) {
+  la_each<TI * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
+    constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
+    const long long row = i + t * 16, c = j + (u >> 2) * 64 + (u & 3) * 4, left = row < a.M ? a.N - c : 0;
+    if (left <= 0) return;
+    float y[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) y[n] = acc[t][u + n / 4][n % 4];
+    la_store8<HdF32, false>(a.partial + ((long long)blockIdx.z * a.M + row) * a.N + c, left, y);
+  });
 }
 
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS, int ACT>
@@ -535,43 +571,15 @@ __global__ __launch_bounds__(64 * WI * WJ, TI * TJ > 32 ? 1 : 2) void la_tile_ke
 #pragma unroll
       for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[0][t], acc[t][u]);
   }
-  // A lane's columns: 8 (TJ / 2) runs of ... (u >> 2) 64 + (lane >> 4) 16 + (u & 3) 4, u even.  The bias of all of them and the
-  // residual of GT rows at a time are read before the first store.
-  const long long jl = j0 + wj + (lane >> 4) * 16;
-  auto col = [&](int u) { return jl + (u >> 2) * 64 + (u & 3) * 4; };
-  float b[TJ / 2][8];
-  const bool whole = a.splits == 1;
-#pragma unroll
-  for (int u = 0; u < TJ; u += 2) {
-#pragma unroll
-    for (int n = 0; n < 8; ++n) b[u / 2][n] = 0.f;
-    if (whole && a.e.bias) {
-      if (a.e.bias_f32) la_load8<HdF32>((const float *)a.e.bias + col(u), a.N - col(u), b[u / 2]);
-      else la_load8<T>((const elem *)a.e.bias + col(u), a.N - col(u), b[u / 2]);
-    }
+  const long long i = i0 + wi + (lane & 15), j = j0 + wj + (lane >> 4) * 16;
+  if (a.splits > 1) la_partial(a, acc, i, j);
+  else if (i0 + BI > a.M || j0 + BJ > a.N) {
+    if (a.e.res) la_epilogue<T, ACT, false, true>(a, acc, i, j);
+    else la_epilogue<T, ACT, false, false>(a, acc, i, j);
+  } else {
+    if (a.e.res) la_epilogue<T, ACT, true, true>(a, acc, i, j);
+    else la_epilogue<T, ACT, true, false>(a, acc, i, j);
   }
-  // (static indices by construction: as a loop, the long body is unrolled too late for the accumulators to stay in registers)
-  constexpr int GT = 2;
-  la_each<TI / GT>([&](auto g_) __attribute__((always_inline)) {
-    constexpr int t0 = decltype(g_)::value * GT;
-    float r[GT][TJ / 2][8];
-#pragma unroll
-    for (int t = 0; t < GT; ++t)
-#pragma unroll
-      for (int u = 0; u < TJ; u += 2) {
-        const long long i = i0 + wi + (t0 + t) * 16 + (lane & 15);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) r[t][u / 2][n] = 0.f;
-        if (whole && a.e.res && i < a.M) la_load8<T>((const elem *)a.e.res + i * a.e.ldr + col(u), a.N - col(u), r[t][u / 2]);
-      }
-    la_each<GT * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
-      constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
-      float z[8];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) { z[n] = acc[t0 + t][u][n]; z[4 + n] = acc[t0 + t][u + 1][n]; }
-      la_finish8<T, ACT>(a, i0 + wi + (t0 + t) * 16 + (lane & 15), col(u), z, b[u / 2], r[t][u / 2]);
-    });
-  });
 }
 
 // the split contraction joined in a fixed order, then the epilogue
@@ -584,34 +592,88 @@ __global__ __launch_bounds__(256) void la_join_kernel(Product a) {
   la_finish_any<T>(a.e, a.N, at / a.N, at % a.N, z);
 }
 
-// dz = dy slope (dz NULL: only the sums) and the column sums of a strip of rows -> part (strips, N) fp32
-template <class T>
-__global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, long long strip, const void *dy_, long long ldy,
+// dz = dy slope (SLOPE; otherwise dz is dy itself) and column sums: a workgroup takes 64 x VE columns and a strip of rows, its four
+// waves every fourth row; part (strips, N) fp32, or NULL.  Bound by its bytes (read dy and slope, write dz).
+template <class T, bool SLOPE>
+__global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, int strip, const void *dy_, long long ldy,
                                                     const void *slope_, void *dz_, float *part) {
   typedef typename T::elem elem;
   typedef typename SlopeOf<T>::type S;
-  const elem *dy = (const elem *)dy_;
-  const typename S::elem *slope = (const typename S::elem *)slope_;
-  elem *dz = (elem *)dz_;
-  const long long j = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (j >= N) return;
+  constexpr int VE = T::kPerVec, U = 4;
+  __shared__ float sum[3][64][VE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long j = ((long long)blockIdx.x * 64 + lane) * VE, left = N - j;
   const long long i0 = (long long)blockIdx.y * strip, i1 = i0 + strip < M ? i0 + strip : M;
-  float s = 0.f;
-  for (long long i = i0; i < i1; ++i) {
-    float v = T::load(dy + i * ldy + j);
-    if (slope) v *= S::load(slope + i * N + j);
-    if (dz) dz[i * N + j] = T::round(v);
-    s += v;
+  float s[VE];
+#pragma unroll
+  for (int n = 0; n < VE; ++n) s[n] = 0.f;
+  if (left >= VE) {
+    const elem *dy = (const elem *)dy_ + j;
+    const typename S::elem *slope = (const typename S::elem *)slope_ + j;
+    elem *dz = (elem *)dz_ + j;
+    for (long long i = i0 + wave; i < i1; i += 4 * U) {
+      hd_u32x4 wy[U], ws[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long row = i + 4 * u < i1 ? i + 4 * u : i;              // (a row past the strip repeats the first)
+        wy[u] = hd_load16<T>(dy + row * ldy);
+        if constexpr (SLOPE) ws[u] = hd_load16<S>(slope + row * N);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + 4 * u >= i1) break;
+        float f[VE];
+        T::unpack(wy[u], f);
+        if constexpr (SLOPE) {
+          float d[VE];
+          S::unpack(ws[u], d);
+#pragma unroll
+          for (int n = 0; n < VE; ++n) f[n] *= d[n];
+          hd_store16<T>(dz + (i + 4 * u) * N, T::pack(f));
+        }
+#pragma unroll
+        for (int n = 0; n < VE; ++n) s[n] += f[n];
+      }
+    }
+  } else if (left > 0) {
+    for (long long i = i0 + wave; i < i1; i += 4)
+#pragma unroll
+      for (int n = 0; n < VE; ++n) {
+        if (n >= left) continue;
+        float f = T::load((const elem *)dy_ + i * ldy + j + n);
+        if constexpr (SLOPE) {
+          f *= S::load((const typename S::elem *)slope_ + i * N + j + n);
+          ((elem *)dz_)[i * N + j + n] = T::round(f);
+        }
+        s[n] += f;
+      }
   }
-  if (part) part[(long long)blockIdx.y * N + j] = s;
+  if (!part) return;                                   // uniform
+  if (wave) {
+#pragma unroll
+    for (int n = 0; n < VE; ++n) sum[wave - 1][lane][n] = s[n];
+  }
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int n = 0; n < VE; ++n)
+      if (n < left) part[(long long)blockIdx.y * N + j + n] = (s[n] + sum[0][lane][n]) + (sum[1][lane][n] + sum[2][lane][n]);
+  }
 }
 
+// the strips' sums joined: 64 columns per workgroup, its four waves every fourth strip
 template <class T>
-__global__ __launch_bounds__(256) void la_db_kernel(long long N, long long strips, const float *part, void *db, int db_f32) {
-  const long long j = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (j >= N) return;
+__global__ __launch_bounds__(256) void la_db_kernel(long long N, int strips, const float *part, void *db, int db_f32) {
+  __shared__ float sum[3][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long j = (long long)blockIdx.x * 64 + lane;
   float s = 0.f;
-  for (long long i = 0; i < strips; ++i) s += part[i * N + j];
+  if (j < N)
+    for (int i = wave; i < strips; i += 4) s += part[(long long)i * N + j];
+  if (wave) sum[wave - 1][lane] = s;
+  __syncthreads();
+  if (wave || j >= N) return;
+  s = (s + sum[0][lane]) + (sum[1][lane] + sum[2][lane]);
   if (db_f32) ((float *)db)[j] = s;
   else ((typename T::elem *)db)[j] = T::round(s);
 }
@@ -621,35 +683,49 @@ constexpr long long kMaxDim = 1LL << 31;
 inline long long la_div(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t la_align(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// how often the contraction of a product is split: until two workgroups per CU run, at least four tiles of it each
-void la_plan(Product &a, int dtype) {
-  const long long kb = dtype == PN2_DT_F32 ? 16 : 32, tiles = la_div(a.M, 64) * la_div(a.N, 64), steps = la_div(a.K, kb);
-  long long s = 512 / tiles;
-  if (s > steps / 4) s = steps / 4;
-  if (s < 1) s = 1;
-  if (s > 64) s = 64;
-  const long long per = la_div(steps, s);
-  a.splits = (int)la_div(steps, per);
-  a.kchunk = per * kb;
-}
-
-size_t la_product_bytes(long long M, long long N, long long K, int dtype) {
-  Product a{};
-  a.M = M; a.N = N; a.K = K;
-  la_plan(a, dtype);
-  return a.splits > 1 ? la_align((size_t)a.splits * M * N * 4) : 0;
-}
+// Which kernel a product takes, by size, type and alignment, and how often its contraction is split.
+//   big   (256 x 256, 16-bit only): tiles for at least three quarters of the CUs.  8192^3: 1.35-1.46 PFLOP/s against 0.88 for mid
+//   mid   (128 x 128, two workgroups per CU)
+//   any   (64 x 64): one side below 96, or operands whose rows are no 16-byte pieces
+// A contraction is split until two workgroups per CU run, each at least four steps long.
+enum { KERNEL_ANY, KERNEL_MID, KERNEL_BIG };
 
 bool la_vec(const void *p, long long ld, int dtype) {
   const long long es = dtype == PN2_DT_F32 ? 4 : 2;
-  return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0;
+  return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && ld <= (1 << 22);
 }
 
-// The tile kernel's direct loads need 16-byte pieces: aligned bases and strides, and axes that are whole pieces.
-bool la_tiled(const Product &a, int dtype, bool prows, bool qrows) {
+int la_kernel_for(long long M, long long N, long long K, int dtype) {           // by size alone
+  if (M < 96 || N < 96 || K < (dtype == PN2_DT_F32 ? 16 : 32)) return KERNEL_ANY;
+  return dtype != PN2_DT_F32 && la_div(M, 256) * la_div(N, 256) >= 192 ? KERNEL_BIG : KERNEL_MID;
+}
+
+// the tile kernels' direct loads need 16-byte pieces: aligned bases and strides, and axes that are whole pieces
+bool la_pieces(const Product &a, int dtype, bool prows, bool qrows) {
   const long long ve = dtype == PN2_DT_F32 ? 4 : 8;
-  return la_vec(a.p, a.ldp, dtype) && la_vec(a.q, a.ldq, dtype) && a.ldp <= (1 << 22) && a.ldq <= (1 << 22) &&
-         (prows ? a.M : a.K) % ve == 0 && (qrows ? a.N : a.K) % ve == 0 && a.K >= 4 * ve && a.M >= 128 && a.N >= 128;
+  return la_vec(a.p, a.ldp, dtype) && la_vec(a.q, a.ldq, dtype) && (prows ? a.M : a.K) % ve == 0 && (qrows ? a.N : a.K) % ve == 0;
+}
+
+// -> contraction indices per split
+long long la_chunk(long long M, long long N, long long K, int dtype, int kernel) {
+  const long long kb = dtype == PN2_DT_F32 ? 16 : 32, steps = la_div(K, kb);
+  const long long edge = kernel == KERNEL_BIG ? 256 : kernel == KERNEL_MID ? 128 : 64;
+  long long s = (kernel == KERNEL_BIG ? 256 : 512) / (la_div(M, edge) * la_div(N, edge));
+  if (s > steps / 4) s = steps / 4;
+  if (s < 1) s = 1;
+  if (s > 64) s = 64;
+  return la_div(steps, s) * kb;
+}
+
+size_t la_partial_bytes(long long M, long long N, long long K, int dtype, int kernel) {
+  const long long splits = la_div(K, la_chunk(M, N, K, dtype, kernel));
+  return splits > 1 ? la_align((size_t)splits * M * N * 4) : 0;
+}
+
+// the most a product of this size can need, whatever its operands' alignment
+size_t la_product_bytes(long long M, long long N, long long K, int dtype) {
+  const size_t any = la_partial_bytes(M, N, K, dtype, KERNEL_ANY), tile = la_partial_bytes(M, N, K, dtype, la_kernel_for(M, N, K, dtype));
+  return any > tile ? any : tile;
 }
 
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS>
@@ -673,20 +749,18 @@ int la_tile_as(const Product &a, hipStream_t st) {
 }
 
 template <class T, bool PROWS, bool QROWS>
-int la_tile(const Product &a, hipStream_t st) {
-  return la_tile_as<T, PROWS, QROWS, LA_CFG>(a, st);
-}
-
-template <class T, bool PROWS, bool QROWS>
 int la_product(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) {
-  la_plan(a, dtype);
-  const size_t need = a.splits > 1 ? la_align((size_t)a.splits * a.M * a.N * 4) : 0;
+  const int kernel = la_pieces(a, dtype, PROWS, QROWS) ? la_kernel_for(a.M, a.N, a.K, dtype) : KERNEL_ANY;
+  a.kchunk = la_chunk(a.M, a.N, a.K, dtype, kernel);
+  a.splits = (int)la_div(a.K, a.kchunk);
+  const size_t need = la_partial_bytes(a.M, a.N, a.K, dtype, kernel);
   if (ws_bytes < need) return PN2_ENOSPC;
   if (need && !ws) return PN2_ENULL;
   a.partial = (float *)ws;
-  if (la_tiled(a, dtype, PROWS, QROWS)) return la_tile<T, PROWS, QROWS>(a, st);
-  a.vecp = la_vec(a.p, a.ldp, dtype);
-  a.vecq = la_vec(a.q, a.ldq, dtype);
+  if constexpr (sizeof(typename T::elem) == 2) {
+    if (kernel == KERNEL_BIG) return la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4, 4>(a, st);
+  }
+  if (kernel != KERNEL_ANY) return la_tile_as<T, PROWS, QROWS, 2, 2, 4, 4, 4>(a, st);
   const long long gx = la_div(a.M, 64), gy = la_div(a.N, 64);
   if (gy > 65535) return PN2_EINVAL;
   la_any_kernel<T, PROWS, QROWS><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)a.splits), 256, 0, st>>>(a);
@@ -698,10 +772,13 @@ inline bool la_bad(long long M, long long N, long long K, int dtype) {
   return M < 0 || N < 1 || K < 1 || M >= kMaxDim || N > 65535LL * 64 || K > 65535LL * 64 || dtype < PN2_DT_F32 || dtype > PN2_DT_F16;
 }
 
-constexpr long long kStripRows = 64;          // rows per partial column sum (at most 1024 strips)
-inline long long la_strip(long long M) {
-  const long long s = la_div(M, 1024);
-  return s > kStripRows ? s : kStripRows;
+// rows per partial column sum: enough workgroups for the chip, at least 16 rows each, at most 512 strips
+inline int la_strip(long long M, long long N, int dtype) {
+  const long long cols = la_div(N, dtype == PN2_DT_F32 ? 256 : 512);
+  long long strips = la_div(2048, cols);
+  if (strips > 512) strips = 512;
+  long long s = la_div(M, strips);
+  return (int)(s < 16 ? 16 : s);
 }
 
 template <class T>
@@ -714,7 +791,7 @@ GradSizes la_grad_sizes(long long M, long long N, long long K, int dtype, int ha
   GradSizes g{};
   const size_t es = dtype == PN2_DT_F32 ? 4 : 2;
   g.dz = has_slope ? la_align((size_t)M * N * es) : 0;
-  g.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M)) * N * 4) : 0;
+  g.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
   g.dx = (want & 1) ? la_product_bytes(M, K, N, dtype) : 0;
   g.dw = (want & 2) ? la_product_bytes(N, K, M, dtype) : 0;
   g.all = g.dz + g.part + (g.dx > g.dw ? g.dx : g.dw);      // the two products share their partial sums' space, one after the other
@@ -735,9 +812,11 @@ int la_backward(long long M, long long N, long long K, int dtype, const void *dy
   char *rest = at + g.dz + g.part;
   const size_t rest_bytes = ws_bytes - g.dz - g.part;
   if (slope || db) {
-    const long long strip = la_strip(M), strips = la_div(M, strip);
-    la_dz_kernel<T><<<dim3((unsigned)la_div(N, 256), (unsigned)strips), 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, part);
-    if (db) la_db_kernel<T><<<(unsigned)la_div(N, 256), 256, 0, st>>>(N, strips, part, db, db_f32);
+    const int strip = la_strip(M, N, dtype), strips = (int)la_div(M, strip);
+    const dim3 grid((unsigned)la_div(N, 64 * T::kPerVec), (unsigned)strips);
+    if (slope) la_dz_kernel<T, true><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, part);
+    else la_dz_kernel<T, false><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, nullptr, part);
+    if (db) la_db_kernel<T><<<(unsigned)la_div(N, 64), 256, 0, st>>>(N, strips, part, db, db_f32);
     const int rc = pn2_check_launch();
     if (rc != PN2_OK) return rc;
   }
