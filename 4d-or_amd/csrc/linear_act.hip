@@ -237,8 +237,8 @@ __global__ __launch_bounds__(256) void la_any_kernel(Product a) {
 //   R operand: 32 (16) contraction rows of the tile's columns, piece c of row k at c ^ f(k); 16-bit fragments are read with the
 //     transposing ds_read_b64_tr_b16 (lane 4 b + a of 16 gives row b, columns 4 a .. 4 a + 3 and receives column lane, rows 0 .. 3),
 //     fp32 ones element by element.
-// Q's fragments are a permutation of its rows: fragment u, row r is j = (r >> 2) 16 + 4 u + (r & 3) of a group of 64, so that a lane
-// ends up with 16 consecutive columns of one result row (32 bytes per store, full lines per 4 lanes).
+// Q's fragments are a permutation of its rows: fragment u, row r is j = (u >> 1) 32 + (r >> 2) 8 + (u & 1) 4 + (r & 3) of a group of
+// 64, so that two fragments give a lane 8 consecutive columns, and the four lanes of a row 32: 64 whole bytes per row and store.
 template <int V> struct LaInt { static constexpr int value = V; };
 template <int N, int I = 0, class F>
 __device__ __forceinline__ void la_each(F f) {
@@ -266,12 +266,12 @@ __device__ __forceinline__ void la_wait() {
 
 template <bool PERM>
 __device__ __forceinline__ int la_swz_k(int r) {
-  const int x = PERM ? r >> 4 : r >> 2;                // the fragment row's group of four
+  const int x = PERM ? r >> 3 : r >> 2;                // the fragment row's group of four
   return (x ^ (x << 1)) & 3;
 }
 template <bool PERM>
 __device__ __forceinline__ int la_swz_r(int k) {
-  return PERM ? (k & 1) | ((k & 2) << 2) : ((k & 3) << 1) | (k & 8);
+  return PERM ? (k & 3) << 2 : ((k & 3) << 1) | (k & 8);
 }
 
 template <class T, bool ROWS, bool PERM, int B, int NT>
@@ -336,30 +336,30 @@ struct Operand {
   __device__ __forceinline__ static unsigned lane_base(int w0, int lane) {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!ROWS) {
-      const int row = w0 + (PERM ? (r >> 2) * 16 + (r & 3) : r);           // (its swizzle does not depend on t)
+      const int row = w0 + (PERM ? (r >> 2) * 8 + (r & 3) : r);            // (its swizzle does not depend on t)
       return row * 64 + ((g ^ la_swz_k<PERM>(row)) << 4);
     } else if constexpr (ES == 2) {
-      const int a = r & 3, k = g * 8 + (r >> 2), col = w0 + a * (PERM ? 16 : 4);
+      const int a = r & 3, k = g * 8 + (r >> 2), col = w0 + a * (PERM ? 8 : 4);
       return k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
     } else {
-      return w0 + (PERM ? (r >> 2) * 16 + (r & 3) : r);                    // (the column; fp32 pays the address of every element)
+      return w0 + (PERM ? (r >> 2) * 8 + (r & 3) : r);                     // (the column; fp32 pays the address of every element)
     }
   }
   __device__ __forceinline__ static hd_u32x4 frag(unsigned slot, unsigned base, int t, int lane) {
     typedef __attribute__((address_space(3))) const hd_u32x4 *lds16;
     if constexpr (!ROWS) {
-      return *(lds16)(size_t)(slot + base + (PERM ? (t >> 2) * 4096 + (t & 3) * 256 : t * 1024));
+      return *(lds16)(size_t)(slot + base + (PERM ? (t >> 1) * 2048 + (t & 1) * 256 : t * 1024));
     } else if constexpr (ES == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4 *lds8;
-      // natural: 16 columns are 2 pieces;  permuted: 4 columns are half a piece
-      const unsigned at = (slot + base) ^ (PERM ? ((t >> 2) << 7) | (((t >> 1) & 1) << 4) : t << 5);
+      // natural: 16 columns are 2 pieces;  permuted: 32 columns are 4 pieces, 4 columns half a piece
+      const unsigned at = (slot + base) ^ (PERM ? (t >> 1) << 6 : t << 5);
       const unsigned half = PERM ? (t & 1) * 8 : 0;
       const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half));
       const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half + 4 * B * 2));       // four rows on: the same swizzle
       return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      const int col = (int)base + (PERM ? (t >> 2) * 64 + (t & 3) * 4 : t * 16);
+      const int col = (int)base + (PERM ? (t >> 1) * 32 + (t & 1) * 4 : t * 16);
       hd_u32x4 w;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -407,14 +407,14 @@ __device__ __forceinline__ void la_store8(typename T::elem *p, long long left, c
 }
 
 // The accumulators of a wave (its first row i, its lane's first column j) -> results.  A lane's columns are runs of 8 at
-// j + (u >> 2) 64 + (u & 3) 4, u even.  FULL: the tile lies inside the matrix (no guards).  The bias of all columns and the residual
+// j + 16 u, u even.  FULL: the tile lies inside the matrix (no guards).  The bias of all columns and the residual
 // of two rows at a time are read before the stores (loads between stores would wait for each other).
 template <class T, int ACT, bool FULL, bool RES, int TI, int TJ>
 __device__ __forceinline__ void la_epilogue(const Product &a, const la_f32x4 (&acc)[TI][TJ], long long i, long long j) {
   typedef typename T::elem elem;
   typedef typename SlopeOf<T>::type S;
   const Epilogue &e = a.e;
-  auto col = [&](int u) { return j + (u >> 2) * 64 + (u & 3) * 4; };
+  auto col = [&](int u) { return j + u * 16; };
   float b[TJ / 2][8];
 #pragma unroll
   for (int u = 0; u < TJ; u += 2) {
@@ -461,7 +461,7 @@ template <int TI, int TJ>
 __device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&acc)[TI][TJ], long long i, long long j) {
   la_each<TI * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
     constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
-    const long long row = i + t * 16, c = j + (u >> 2) * 64 + (u & 3) * 4, left = row < a.M ? a.N - c : 0;
+    const long long row = i + t * 16, c = j + u * 16, left = row < a.M ? a.N - c : 0;
     if (left <= 0) return;
     float y[8];
 #pragma unroll
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(64 * WI * WJ, TI * TJ > 32 ? 1 : 2) void la_tile_ke
 #pragma unroll
       for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[0][t], acc[t][u]);
   }
-  const long long i = i0 + wi + (lane & 15), j = j0 + wj + (lane >> 4) * 16;
+  const long long i = i0 + wi + (lane & 15), j = j0 + wj + (lane >> 4) * 8;
   if (a.splits > 1) la_partial(a, acc, i, j);
   else if (i0 + BI > a.M || j0 + BJ > a.N) {
     if (a.e.res) la_epilogue<T, ACT, false, true>(a, acc, i, j);
