@@ -226,15 +226,15 @@ __global__ __launch_bounds__(256) void la_any_kernel(Product a) {
 
 // ------------------------------------------------------------------------------------------------------ the tile kernel
 // A workgroup of WI x WJ waves owns a tile of (WI TI 16) x (WJ TJ 16) results; a wave holds TI x TJ accumulators.  Operand tiles of
-// 64 bytes of contraction (32 16-bit or 16 fp32 indices) travel global -> LDS directly (global_load_lds, 16 bytes per lane) into a
-// ring of NS slots, NS - 1 steps ahead; one barrier per step.  A step's Q fragments and, one by one, its P fragments are read
-// from LDS while the matrix instructions of the step before run: nothing waits on LDS between two barriers.
+// 128 bytes of contraction (64 16-bit or 32 fp32 indices: whole cache lines of a K operand, whose 64-byte halves cost the L1 twice
+// the requests) travel global -> LDS directly (global_load_lds, 16 bytes per lane) into one of two slots, a tile ahead.  A tile is
+// two steps; the fragments of a step are read from LDS while the matrix instructions of the step before run, so a wave never waits
+// for LDS, and there is one barrier per tile.
 //
 // LDS layout (16-byte pieces; XOR swizzles, applied to the GLOBAL address of a lane because the direct load writes lane-linear):
-//   K operand: rows of 64 bytes, piece c of row r at c ^ s(x), x the fragment row's group of four, s = 0 3 2 1: a ds_read_b128 takes
-//     16 lanes per cycle, {0-3, 12-15, 20-23, 24-27} and so on, and those hit 16 different pieces of 256 bytes (with s = 0 1 2 3,
-//     free of conflicts for 16 consecutive lanes, half the LDS cycles were conflicts: 8.0 against 4.0 a read);
-//   R operand: 32 (16) contraction rows of the tile's columns, piece c of row k at c ^ f(k); 16-bit fragments are read with the
+//   K operand: rows of 128 bytes, piece c of row r at c ^ f(r), f counting the fragment's row pairs: a ds_read_b128 takes 16 lanes
+//     per cycle, {0-3, 12-15, 20-23, 24-27} and so on, and those hit the 16 pieces of 256 bytes;
+//   R operand: contraction rows of the tile's columns, piece c of row k at c ^ f(k); 16-bit fragments are read with the
 //     transposing ds_read_b64_tr_b16 (lane 4 b + a of 16 gives row b, columns 4 a .. 4 a + 3 and receives column lane, rows 0 .. 3),
 //     fp32 ones element by element.
 // Q's fragments are a permutation of its rows: fragment u, row r is j = (u >> 1) 32 + (r >> 2) 8 + (u & 1) 4 + (r & 3) of a group of
@@ -258,16 +258,15 @@ __device__ __forceinline__ void la_dma(unsigned lds, unsigned long long base, un
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
-// all but the last N direct loads of this wave have landed, all but its last D LDS operations are done
-template <int N, int D>
+// all but the last N direct loads of this wave have landed, its LDS reads are done
+template <int N>
 __device__ __forceinline__ void la_wait() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)" ::"n"(N), "n"(D) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 template <bool PERM>
 __device__ __forceinline__ int la_swz_k(int r) {
-  const int x = PERM ? r >> 3 : r >> 2;                // the fragment row's group of four
-  return (x ^ (x << 1)) & 3;
+  return PERM ? ((r >> 1) & 1) | ((r >> 2) & 6) : (r >> 1) & 7;
 }
 template <bool PERM>
 __device__ __forceinline__ int la_swz_r(int k) {
@@ -277,21 +276,20 @@ __device__ __forceinline__ int la_swz_r(int k) {
 template <class T, bool ROWS, bool PERM, int B, int NT>
 struct Operand {
   typedef typename T::elem elem;
-  static constexpr int VE = T::kPerVec, KB = 4 * VE, ES = (int)sizeof(elem), PER = B * 4 / NT;   // pieces per thread and step
-  static constexpr int READS = ROWS ? (ES == 2 ? 2 : 4) : 1;                                     // LDS reads per fragment
+  static constexpr int VE = T::kPerVec, KB = 8 * VE, ES = (int)sizeof(elem), PER = B * 8 / NT;   // pieces per thread and tile
   static constexpr int PW = B / VE;                                                              // R operand: pieces per row
   unsigned off[PER];               // lane offsets of the direct loads
-  unsigned long long base;         // advances by a step
+  unsigned long long base;         // advances by a tile
   unsigned step;
   __device__ __forceinline__ void init(const void *g, long long ld, long long r0, long long R, long long k0, int tid) {
     const elem *p = (const elem *)g;
     base = (unsigned long long)(ROWS ? p + k0 * ld + r0 : p + r0 * ld + k0);
-    step = ROWS ? (unsigned)(KB * ld * ES) : 64u;
+    step = ROWS ? (unsigned)(KB * ld * ES) : 128u;
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       const int at = n * NT + tid;
       if constexpr (!ROWS) {
-        const int r = at >> 2, c = (at & 3) ^ la_swz_k<PERM>(r);
+        const int r = at >> 3, c = (at & 7) ^ la_swz_k<PERM>(r);
         const long long rr = r0 + r < R ? r : R - 1 - r0;          // rows out of range repeat the last one: never stored
         off[n] = (unsigned)(rr * ld * ES + c * 16);
       } else {
@@ -302,7 +300,7 @@ struct Operand {
     }
   }
   __device__ __forceinline__ void issue(int n, unsigned lds, int wave) { la_dma(lds + (n * NT + wave * 64) * 16, base, off[n]); }
-  // the last, partial step: pieces through registers, out of range = 0
+  // the last, partial tile: pieces through registers, out of range = 0
   __device__ __forceinline__ void tail(char *lds, const void *g, long long ld, long long r0, long long R, long long k0, long long k1,
                                        int tid) {
 #pragma unroll
@@ -310,8 +308,8 @@ struct Operand {
       const int at = n * NT + tid;
       long long r, k, left;
       if constexpr (!ROWS) {
-        r = r0 + (at >> 2);
-        k = k0 + ((at & 3) ^ la_swz_k<PERM>(at >> 2)) * VE;
+        r = r0 + (at >> 3);
+        k = k0 + ((at & 7) ^ la_swz_k<PERM>(at >> 3)) * VE;
         left = r < R ? k1 - k : 0;
       } else {
         k = k0 + at / PW;
@@ -331,13 +329,13 @@ struct Operand {
       *reinterpret_cast<hd_u32x4 *>(lds + at * 16) = w;
     }
   }
-  // Fragment t of the wave whose rows start at w0 (a multiple of 64) = frag(slot + lane_base(w0), t): a lane's offsets differ between
-  // fragments by a constant, or by a constant exclusive-or.
+  // Fragment t, step `half` of the tile, of the wave whose rows start at w0 (a multiple of 64) = frag(slot + lane_base(w0), t, half):
+  // a lane's offsets differ between fragments by a constant, or by a constant exclusive-or.
   __device__ __forceinline__ static unsigned lane_base(int w0, int lane) {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!ROWS) {
       const int row = w0 + (PERM ? (r >> 2) * 8 + (r & 3) : r);            // (its swizzle does not depend on t)
-      return row * 64 + ((g ^ la_swz_k<PERM>(row)) << 4);
+      return row * 128 + ((g ^ la_swz_k<PERM>(row)) << 4);
     } else if constexpr (ES == 2) {
       const int a = r & 3, k = g * 8 + (r >> 2), col = w0 + a * (PERM ? 8 : 4);
       return k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
@@ -345,25 +343,25 @@ struct Operand {
       return w0 + (PERM ? (r >> 2) * 8 + (r & 3) : r);                     // (the column; fp32 pays the address of every element)
     }
   }
+  template <int HALF>
   __device__ __forceinline__ static hd_u32x4 frag(unsigned slot, unsigned base, int t, int lane) {
     typedef __attribute__((address_space(3))) const hd_u32x4 *lds16;
     if constexpr (!ROWS) {
-      return *(lds16)(size_t)(slot + base + (PERM ? (t >> 1) * 2048 + (t & 1) * 256 : t * 1024));
+      return *(lds16)(size_t)(((slot + base) ^ (HALF << 6)) + (PERM ? (t >> 1) * 4096 + (t & 1) * 512 : t * 2048));
     } else if constexpr (ES == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4 *lds8;
       // natural: 16 columns are 2 pieces;  permuted: 32 columns are 4 pieces, 4 columns half a piece
-      const unsigned at = (slot + base) ^ (PERM ? (t >> 1) << 6 : t << 5);
-      const unsigned half = PERM ? (t & 1) * 8 : 0;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half));
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + half + 4 * B * 2));       // four rows on: the same swizzle
+      const unsigned at = ((slot + base) ^ (PERM ? (t >> 1) << 6 : t << 5)) + HALF * 32 * B * 2 + (PERM ? (t & 1) * 8 : 0);
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)at);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(size_t)(at + 4 * B * 2));      // four rows on: the same swizzle
       return __builtin_bit_cast(hd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       const int col = (int)base + (PERM ? (t >> 1) * 32 + (t & 1) * 4 : t * 16);
       hd_u32x4 w;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int k = (lane >> 4) * 4 + n;
+        const int k = HALF * 16 + (lane >> 4) * 4 + n;
         w[n] = *(__attribute__((address_space(3))) const unsigned *)(size_t)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
       }
       return w;
@@ -470,13 +468,12 @@ __device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&ac
   });
 }
 
-template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS, int ACT>
-__global__ __launch_bounds__(64 * WI * WJ, TI * TJ > 32 ? 1 : 2) void la_tile_kernel(Product a, int gi, int gj) {
-  constexpr int NT = 64 * WI * WJ, BI = WI * TI * 16, BJ = WJ * TJ * 16, KB = 4 * T::kPerVec, STAGE = (BI + BJ) * 64;
-  typedef typename T::elem elem;
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int gi, int gj) {
+  constexpr int NT = 64 * WI * WJ, BI = WI * TI * 16, BJ = WJ * TJ * 16, KB = 8 * T::kPerVec, SLOT = (BI + BJ) * 128;
   typedef Operand<T, PROWS, false, BI, NT> OP;
   typedef Operand<T, QROWS, true, BJ, NT> OQ;
-  __shared__ __align__(1024) char ring[NS * STAGE];
+  __shared__ __align__(1024) char ring[2 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups go round robin over the 8 XCDs: give each XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that the
   // operand panels of a band are shared in its L2
@@ -490,86 +487,89 @@ __global__ __launch_bounds__(64 * WI * WJ, TI * TJ > 32 ? 1 : 2) void la_tile_ke
   }
   const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
   const long long k0 = (long long)blockIdx.z * a.kchunk, k1 = k0 + a.kchunk < a.K ? k0 + a.kchunk : a.K;
-  const int steps = (int)((k1 - k0) / KB), rest = (int)((k1 - k0) % KB);
+  const int tiles = (int)((k1 - k0) / KB), rest = (int)((k1 - k0) % KB);
   const int wi = (wave % WI) * TI * 16, wj = (wave / WI) * TJ * 16;
-  constexpr int L = OP::PER + OQ::PER;                 // direct loads per wave and step
+  constexpr int L = OP::PER + OQ::PER;                 // direct loads per wave and tile
   OP op;
   OQ oq;
   op.init(a.p, a.ldp, i0, a.M, k0, tid);
   oq.init(a.q, a.ldq, j0, a.N, k0, tid);
   const unsigned lds0 = la_lds(ring);
-  // direct load n of the next step; beyond the last step it repeats that one (in bounds, into a slot nobody reads any more), so that
+  // direct load n of the next tile; beyond the last tile it repeats that one (in bounds, into a slot nobody reads any more), so that
   // the loop has no branches and its waits are constants
   int issued = 0;
   auto issue = [&](int n) __attribute__((always_inline)) {
-    const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (issued % NS) * STAGE);
+    const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (issued & 1) * SLOT);
     if (n < OP::PER) op.issue(n, at, wave);
-    else oq.issue(n - OP::PER, at + BI * 64, wave);
+    else oq.issue(n - OP::PER, at + BI * 128, wave);
     if (n == L - 1) {
       ++issued;
-      op.base += issued < steps ? op.step : 0;
-      oq.base += issued < steps ? oq.step : 0;
+      op.base += issued < tiles ? op.step : 0;
+      oq.base += issued < tiles ? oq.step : 0;
     }
   };
   la_f32x4 acc[TI][TJ] = {};
   hd_u32x4 p[2][TI], q[2][TJ];
-  constexpr int A = NS - 1;                            // steps in flight
-  // fragment n of a step, Q's first
-  const unsigned pb = OP::lane_base(wi, lane), qb = OQ::lane_base(wj, lane) + (QROWS && sizeof(elem) == 4 ? 0 : BI * 64);
-  auto read = [&](unsigned at, int n, int buf) __attribute__((always_inline)) {
-    if (n < TJ) q[buf][n] = OQ::frag(QROWS && sizeof(elem) == 4 ? at + BI * 64 : at, qb, n, lane);
-    else p[buf][n - TJ] = OP::frag(at, pb, n - TJ, lane);
+  const unsigned pb = OP::lane_base(wi, lane), qb = OQ::lane_base(wj, lane);
+  // fragment n of step HALF of the tile in `slot`, Q's first -> register set HALF
+  auto read = [&](unsigned slot, int n, auto half_) __attribute__((always_inline)) {
+    constexpr int half = decltype(half_)::value;
+    if (n < TJ) q[half][n] = OQ::template frag<half>(slot + BI * 128, qb, n, lane);
+    else p[half][n - TJ] = OP::template frag<half>(slot, pb, n - TJ, lane);
   };
-  // One step: (A) its successor has landed for every wave; (B) the slot of its predecessor is refilled: every wave's reads of it are
-  // done, they lie before the last step's, of which there are at least D; (C) products, one fragment of the successor read after
-  // each of the first ones, then the direct loads.  The order is pinned: left to itself the compiler sinks the reads, and the next
-  // step waits for them; loads before the products leave the matrix cores idle behind each barrier.
-  constexpr int D = TI + TJ < 15 ? TI + TJ : 15;
-  constexpr int GAP = TI * TJ * 3 / 4 / (TI + TJ), LGAP = TI * TJ * 3 / 4 / L;
+  // A step: the products of register set HALF, one read of the other set's fragments after every GAP of the first ones, LOAD: the
+  // direct loads in between, in its first half (they have little more than a step to land).  The order is pinned: left to itself the compiler sinks the reads, and the next step waits for them;
+  // loads before the products leave the matrix cores idle behind the barrier.
+  constexpr int GAP = TI * TJ * 3 / 4 / (TI + TJ), LGAP = TI * TJ / L / 2 > 0 ? TI * TJ / L / 2 : 1;
   static_assert(GAP > 0 && LGAP > 0, "room for the reads and the loads between the products");
-  auto step = [&](int s, auto cur_) __attribute__((always_inline)) {
-    constexpr int cur = decltype(cur_)::value;
-    la_wait<(A - 2) * L, D>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    // (the step after the last one reads a slot of older data: in bounds, never used)
-    const unsigned next = lds0 + ((s + 1) % NS) * STAGE;
+  auto step = [&](unsigned slot, auto half_, auto load_) __attribute__((always_inline)) {
+    constexpr int half = decltype(half_)::value;
     la_each<TI * TJ>([&](auto n_) __attribute__((always_inline)) {
       constexpr int n = decltype(n_)::value, t = n / TJ, u = n % TJ;
-      acc[t][u] = la_mma(T{}, q[cur][u], p[cur][t], acc[t][u]);
-      if constexpr (n % GAP == 0 && n / GAP < TI + TJ) read(next, n / GAP, cur ^ 1);
-      if constexpr (n % LGAP == LGAP / 2 && n / LGAP < L) issue(n / LGAP);
+      acc[t][u] = la_mma(T{}, q[half][u], p[half][t], acc[t][u]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n % GAP == 0 && n / GAP < TI + TJ) read(slot, n / GAP, LaInt<half ^ 1>{});
+      if constexpr (decltype(load_)::value && n % LGAP == LGAP / 2 && n / LGAP < L) issue(n / LGAP);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  if (steps > 0) {
-    for (int s = 0; s < A; ++s)
-#pragma unroll
-      for (int n = 0; n < L; ++n) issue(n);
-    la_wait<(A - 1) * L, 0>();
+  // every wave's direct loads have landed (all but the last N of each) and its LDS reads are done
+  auto meet = [&](auto n_) __attribute__((always_inline)) {
+    la_wait<decltype(n_)::value>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+  };
+  if (tiles > 0) {
 #pragma unroll
-    for (int n = 0; n < TI + TJ; ++n) read(lds0, n, 0);
-    int s = 0;
-    for (; s + 1 < steps; s += 2) {
-      step(s, LaInt<0>{});
-      step(s + 1, LaInt<1>{});
+    for (int n = 0; n < 2 * L; ++n) issue(n % L);
+    meet(LaInt<L>{});
+#pragma unroll
+    for (int n = 0; n < TI + TJ; ++n) read(lds0, n, LaInt<0>{});
+    for (int d = 0; d < tiles; ++d) {
+      step(lds0 + (d & 1) * SLOT, LaInt<0>{}, LaInt<0>{});
+      // the next tile has landed; this one's slot, whose last fragments were read in the step above, is refilled
+      meet(LaInt<0>{});
+      // (the last tile reads on in a slot of older data: in bounds, never used)
+      step(lds0 + ((d + 1) & 1) * SLOT, LaInt<1>{}, LaInt<1>{});
     }
-    if (s < steps) step(s, LaInt<0>{});
-    la_wait<0, 0>();                                   // no direct load is left when the workgroup gives its LDS back
+    la_wait<0>();                                      // no direct load is left when the workgroup gives its LDS back
   }
   if (rest) {
     __syncthreads();
-    op.tail(ring, a.p, a.ldp, i0, a.M, k0 + (long long)steps * KB, k1, tid);
-    oq.tail(ring + BI * 64, a.q, a.ldq, j0, a.N, k0 + (long long)steps * KB, k1, tid);
+    op.tail(ring, a.p, a.ldp, i0, a.M, k0 + (long long)tiles * KB, k1, tid);
+    oq.tail(ring + BI * 128, a.q, a.ldq, j0, a.N, k0 + (long long)tiles * KB, k1, tid);
     __syncthreads();
+    auto half = [&](auto half_) __attribute__((always_inline)) {
+      constexpr int h = decltype(half_)::value;
 #pragma unroll
-    for (int n = 0; n < TI + TJ; ++n) read(lds0, n, 0);
+      for (int n = 0; n < TI + TJ; ++n) read(lds0, n, LaInt<h>{});
 #pragma unroll
-    for (int t = 0; t < TI; ++t)
+      for (int t = 0; t < TI; ++t)
 #pragma unroll
-      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[0][u], p[0][t], acc[t][u]);
+        for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[h][u], p[h][t], acc[t][u]);
+    };
+    half(LaInt<0>{});
+    if (rest > KB / 2) half(LaInt<1>{});
   }
   const long long i = i0 + wi + (lane & 15), j = j0 + wj + (lane >> 4) * 8;
   if (a.splits > 1) la_partial(a, acc, i, j);
@@ -708,10 +708,10 @@ bool la_pieces(const Product &a, int dtype, bool prows, bool qrows) {
 
 // -> contraction indices per split
 long long la_chunk(long long M, long long N, long long K, int dtype, int kernel) {
-  const long long kb = dtype == PN2_DT_F32 ? 16 : 32, steps = la_div(K, kb);
+  const long long kb = dtype == PN2_DT_F32 ? 32 : 64, steps = la_div(K, kb);
   const long long edge = kernel == KERNEL_BIG ? 256 : kernel == KERNEL_MID ? 128 : 64;
   long long s = (kernel == KERNEL_BIG ? 256 : 512) / (la_div(M, edge) * la_div(N, edge));
-  if (s > steps / 4) s = steps / 4;
+  if (s > steps / 2) s = steps / 2;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
   return la_div(steps, s) * kb;
@@ -728,20 +728,20 @@ size_t la_product_bytes(long long M, long long N, long long K, int dtype) {
   return any > tile ? any : tile;
 }
 
-template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int NS>
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
 int la_tile_as(const Product &a, hipStream_t st) {
   const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
   const dim3 grid((unsigned)(gi * gj), 1, (unsigned)a.splits);
   constexpr int NT = 64 * WI * WJ;
   if constexpr (PROWS || QROWS) {
-    la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, NS, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+    la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
   } else {
     switch (a.splits > 1 ? ACT_NONE : a.e.act) {       // (a split contraction's epilogue is the join kernel's)
-      case ACT_RELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_RELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_GELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_GELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_GELU_TANH: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_GELU_TANH><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      case ACT_SILU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_SILU><<<grid, NT, 0, st>>>(a, gi, gj); break;
-      default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, NS, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
+      case ACT_RELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_RELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_GELU_TANH: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_GELU_TANH><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      case ACT_SILU: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_SILU><<<grid, NT, 0, st>>>(a, gi, gj); break;
+      default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
     }
   }
   if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 256), 256, 0, st>>>(a);
@@ -758,9 +758,9 @@ int la_product(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) 
   if (need && !ws) return PN2_ENULL;
   a.partial = (float *)ws;
   if constexpr (sizeof(typename T::elem) == 2) {
-    if (kernel == KERNEL_BIG) return la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4, 4>(a, st);
+    if (kernel == KERNEL_BIG) return la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4>(a, st);
   }
-  if (kernel != KERNEL_ANY) return la_tile_as<T, PROWS, QROWS, 2, 2, 4, 4, 4>(a, st);
+  if (kernel != KERNEL_ANY) return la_tile_as<T, PROWS, QROWS, 2, 2, 4, 4>(a, st);
   const long long gx = la_div(a.M, 64), gy = la_div(a.N, 64);
   if (gy > 65535) return PN2_EINVAL;
   la_any_kernel<T, PROWS, QROWS><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)a.splits), 256, 0, st>>>(a);
