@@ -98,6 +98,7 @@ struct Product {
   long long M, N, K;
   const void *p, *q;
   long long ldp, ldq;
+  long long rp, rq;         // rows of P and Q that may be read (an R operand's padded to whole 16-byte pieces)
   int splits;
   long long kchunk;         // contraction indices per split (a multiple of the tile's)
   float *partial;           // splits > 1: (splits, M, N)
@@ -127,101 +128,6 @@ __device__ __forceinline__ void la_finish_any(const Epilogue &e, long long N, lo
   ((elem *)e.y)[i * N + j] = T::round(y);
   typedef typename SlopeOf<T>::type S;
   if (e.slope) ((typename S::elem *)e.slope)[i * N + j] = S::round(d);
-}
-
-// A tile of 64 rows x 64 bytes of contraction (KB = 16 or 32 indices) goes through registers into LDS rows of 64 + 16 bytes.
-// K operand: thread -> (row tid / 4, 16-byte piece tid % 4).  R operand: thread -> (index tid / (64 / VE), piece), stored
-// transposed.  Rows and indices out of range are zero.
-template <class T, bool ROWS>
-struct TileLoad {
-  typedef typename T::elem elem;
-  static constexpr int VE = T::kPerVec, KB = 4 * VE, LDT = 80 / (int)sizeof(elem);
-  hd_u32x4 w;
-  __device__ __forceinline__ void fetch(const elem *g, long long ld, long long r0, long long R, long long k0, long long k1,
-                                        int tid) {
-    long long r, k, n;
-    const elem *src;
-    if constexpr (!ROWS) {
-      r = r0 + tid / 4;
-      k = k0 + (tid % 4) * VE;
-      n = r < R ? k1 - k : 0;
-      src = g + r * ld + k;
-    } else {
-      constexpr int PR = 64 / VE;
-      k = k0 + tid / PR;
-      r = r0 + (tid % PR) * VE;
-      n = k < k1 ? R - r : 0;
-      src = g + k * ld + r;
-    }
-    if (n >= VE) {
-      w = hd_load16<T>(src);
-    } else {
-      elem v[VE];
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[i] = i < n ? src[i] : T::round(0.f);
-      __builtin_memcpy(&w, v, 16);
-    }
-  }
-  __device__ __forceinline__ void store(elem *lds, int tid) const {
-    if constexpr (!ROWS) {
-      __builtin_memcpy((elem *)__builtin_assume_aligned(lds + (tid / 4) * LDT + (tid % 4) * VE, 16), &w, 16);
-    } else {
-      constexpr int PR = 64 / VE;
-      elem v[VE];
-      __builtin_memcpy(v, &w, 16);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) lds[((tid % PR) * VE + i) * LDT + tid / PR] = v[i];
-    }
-  }
-};
-
-// 64 x 64 tile, four waves of 32 x 32, any alignment and any size.
-template <class T, bool PROWS, bool QROWS>
-__global__ __launch_bounds__(256) void la_any_kernel(Product a) {
-  typedef typename T::elem elem;
-  constexpr int KB = 4 * T::kPerVec, LDT = 80 / (int)sizeof(elem);
-  __shared__ __align__(16) elem sp[64 * LDT], sq[64 * LDT];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long long i0 = (long long)blockIdx.x * 64, j0 = (long long)blockIdx.y * 64;
-  const long long k0 = (long long)blockIdx.z * a.kchunk, k1 = k0 + a.kchunk < a.K ? k0 + a.kchunk : a.K;
-  const int wi = (wave & 1) * 32, wj = (wave >> 1) * 32;
-  la_f32x4 acc[2][2] = {};
-  TileLoad<T, PROWS> lp;
-  TileLoad<T, QROWS> lq;
-  lp.fetch((const elem *)a.p, a.ldp, i0, a.M, k0, k1, tid);
-  lq.fetch((const elem *)a.q, a.ldq, j0, a.N, k0, k1, tid);
-  for (long long k = k0; k < k1; k += KB) {
-    lp.store(sp, tid);
-    lq.store(sq, tid);
-    __syncthreads();
-    if (k + KB < k1) {
-      lp.fetch((const elem *)a.p, a.ldp, i0, a.M, k + KB, k1, tid);
-      lq.fetch((const elem *)a.q, a.ldq, j0, a.N, k + KB, k1, tid);
-    }
-    hd_u32x4 fp[2], fq[2];
-    const int r = lane & 15, c = (lane >> 4) * T::kPerVec;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      __builtin_memcpy(&fp[t], __builtin_assume_aligned(sp + (wi + t * 16 + r) * LDT + c, 16), 16);
-      __builtin_memcpy(&fq[t], __builtin_assume_aligned(sq + (wj + t * 16 + r) * LDT + c, 16), 16);
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) acc[t][u] = la_mma(T{}, fq[u], fp[t], acc[t][u]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const long long i = i0 + wi + t * 16 + (lane & 15), j = j0 + wj + u * 16 + (lane >> 4) * 4 + n;
-        if (i >= a.M || j >= a.N) continue;
-        if (a.splits > 1) a.partial[((long long)blockIdx.z * a.M + i) * a.N + j] = acc[t][u][n];
-        else la_finish_any<T>(a.e, a.N, i, j, acc[t][u][n]);
-      }
 }
 
 // ------------------------------------------------------------------------------------------------------ the tile kernel
@@ -268,9 +174,12 @@ template <bool PERM>
 __device__ __forceinline__ int la_swz_k(int r) {
   return PERM ? ((r >> 1) & 1) | ((r >> 2) & 6) : (r >> 1) & 7;
 }
-template <bool PERM>
+// PW pieces per row.  A transposing read takes rows k & 3 at once; rows of 8 pieces (128 bytes) alternate between the halves of 256
+// bytes by themselves.
+template <bool PERM, int PW>
 __device__ __forceinline__ int la_swz_r(int k) {
-  return PERM ? (k & 3) << 2 : ((k & 3) << 1) | (k & 8);
+  if constexpr (PW == 8) return PERM ? (k & 2) << 1 : (k & 2) | ((k & 8) >> 1);
+  else return PERM ? (k & 3) << 2 : ((k & 3) << 1) | (k & 8);
 }
 
 template <class T, bool ROWS, bool PERM, int B, int NT>
@@ -293,7 +202,7 @@ struct Operand {
         const long long rr = r0 + r < R ? r : R - 1 - r0;          // rows out of range repeat the last one: never stored
         off[n] = (unsigned)(rr * ld * ES + c * 16);
       } else {
-        const int k = at / PW, c = (at % PW) ^ la_swz_r<PERM>(k);
+        const int k = at / PW, c = (at % PW) ^ la_swz_r<PERM, PW>(k);
         const long long cc = r0 + (long long)(c + 1) * VE <= R ? c * VE : R - VE - r0;
         off[n] = (unsigned)(k * ld * ES + cc * ES);
       }
@@ -313,7 +222,7 @@ struct Operand {
         left = r < R ? k1 - k : 0;
       } else {
         k = k0 + at / PW;
-        r = r0 + ((at % PW) ^ la_swz_r<PERM>(at / PW)) * VE;
+        r = r0 + ((at % PW) ^ la_swz_r<PERM, PW>(at / PW)) * VE;
         left = k < k1 ? R - r : 0;
       }
       const elem *src = (const elem *)g + (ROWS ? k * ld + r : r * ld + k);
@@ -329,7 +238,7 @@ struct Operand {
       *reinterpret_cast<hd_u32x4 *>(lds + at * 16) = w;
     }
   }
-  // Fragment t, step `half` of the tile, of the wave whose rows start at w0 (a multiple of 64) = frag(slot + lane_base(w0), t, half):
+  // Fragment t, step `half` of the tile, of the wave whose rows start at w0 (a multiple of 32) = frag(slot + lane_base(w0), t, half):
   // a lane's offsets differ between fragments by a constant, or by a constant exclusive-or.
   __device__ __forceinline__ static unsigned lane_base(int w0, int lane) {
     const int r = lane & 15, g = lane >> 4;
@@ -338,7 +247,7 @@ struct Operand {
       return row * 128 + ((g ^ la_swz_k<PERM>(row)) << 4);
     } else if constexpr (ES == 2) {
       const int a = r & 3, k = g * 8 + (r >> 2), col = w0 + a * (PERM ? 8 : 4);
-      return k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM>(k)) << 4) + ((col >> 2) & 1) * 8;
+      return k * (B * 2) + (((col >> 3) ^ la_swz_r<PERM, PW>(k)) << 4) + ((col >> 2) & 1) * 8;
     } else {
       return w0 + (PERM ? (r >> 2) * 8 + (r & 3) : r);                     // (the column; fp32 pays the address of every element)
     }
@@ -362,7 +271,7 @@ struct Operand {
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int k = HALF * 16 + (lane >> 4) * 4 + n;
-        w[n] = *(__attribute__((address_space(3))) const unsigned *)(size_t)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM>(k)) << 4) + (col & 3) * 4);
+        w[n] = *(__attribute__((address_space(3))) const unsigned *)(size_t)(slot + k * (B * 4) + (((col >> 2) ^ la_swz_r<PERM, PW>(k)) << 4) + (col & 3) * 4);
       }
       return w;
     }
@@ -492,8 +401,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
   constexpr int L = OP::PER + OQ::PER;                 // direct loads per wave and tile
   OP op;
   OQ oq;
-  op.init(a.p, a.ldp, i0, a.M, k0, tid);
-  oq.init(a.q, a.ldq, j0, a.N, k0, tid);
+  op.init(a.p, a.ldp, i0, a.rp, k0, tid);
+  oq.init(a.q, a.ldq, j0, a.rq, k0, tid);
   const unsigned lds0 = la_lds(ring);
   // direct load n of the next tile; beyond the last tile it repeats that one (in bounds, into a slot nobody reads any more), so that
   // the loop has no branches and its waits are constants
@@ -520,8 +429,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
   // A step: the products of register set HALF, one read of the other set's fragments after every GAP of the first ones, LOAD: the
   // direct loads in between, in its first half (they have little more than a step to land).  The order is pinned: left to itself the compiler sinks the reads, and the next step waits for them;
   // loads before the products leave the matrix cores idle behind the barrier.
-  constexpr int GAP = TI * TJ * 3 / 4 / (TI + TJ), LGAP = TI * TJ / L / 2 > 0 ? TI * TJ / L / 2 : 1;
-  static_assert(GAP > 0 && LGAP > 0, "room for the reads and the loads between the products");
+  constexpr int GAP = TI * TJ * 3 / 4 / (TI + TJ) > 0 ? TI * TJ * 3 / 4 / (TI + TJ) : 1, LGAP = TI * TJ / L / 2 > 0 ? TI * TJ / L / 2 : 1;
+  static_assert(TI + TJ <= TI * TJ && L <= TI * TJ, "room for the reads and the loads between the products");
   auto step = [&](unsigned slot, auto half_, auto load_) __attribute__((always_inline)) {
     constexpr int half = decltype(half_)::value;
     la_each<TI * TJ>([&](auto n_) __attribute__((always_inline)) {
@@ -556,8 +465,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
   }
   if (rest) {
     __syncthreads();
-    op.tail(ring, a.p, a.ldp, i0, a.M, k0 + (long long)tiles * KB, k1, tid);
-    oq.tail(ring + BI * 128, a.q, a.ldq, j0, a.N, k0 + (long long)tiles * KB, k1, tid);
+    op.tail(ring, a.p, a.ldp, i0, a.rp, k0 + (long long)tiles * KB, k1, tid);
+    oq.tail(ring + BI * 128, a.q, a.ldq, j0, a.rq, k0 + (long long)tiles * KB, k1, tid);
     __syncthreads();
     auto half = [&](auto half_) __attribute__((always_inline)) {
       constexpr int h = decltype(half_)::value;
@@ -582,21 +491,245 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
   }
 }
 
-// the split contraction joined in a fixed order, then the epilogue
+// the split contraction joined in a fixed order, then the epilogue: four consecutive results per thread
 template <class T>
 __global__ __launch_bounds__(256) void la_join_kernel(Product a) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= a.M * a.N) return;
-  float z = 0.f;
-  for (int s = 0; s < a.splits; ++s) z += a.partial[(long long)s * a.M * a.N + at];
-  la_finish_any<T>(a.e, a.N, at / a.N, at % a.N, z);
+  const long long n = a.M * a.N, at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+  if (at + 4 <= n) {
+    for (int s = 0; s < a.splits; ++s) {
+      float f[4];
+      HdF32::unpack(hd_load16<HdF32>(a.partial + s * n + at), f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) z[q] += f[q];
+    }
+  } else {
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (at + q < n) z[q] += a.partial[s * n + at + q];
+  }
+  long long i = at / a.N, j = at - i * a.N;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (at + q < n) la_finish_any<T>(a.e, a.N, i, j, z[q]);
+    if (++j == a.N) { j = 0; ++i; }
+  }
 }
 
-// dz = dy slope (SLOPE; otherwise dz is dy itself) and column sums: a workgroup takes 64 x VE columns and a strip of rows, its four
+// rows x cols at row stride ld -> rows at row stride `to` (a multiple of 16 bytes), the columns behind `cols` zero
+template <class T>
+__global__ __launch_bounds__(256) void la_pad_kernel(long long rows, long long cols, const void *src_, long long ld, void *dst_, long long to) {
+  typedef typename T::elem elem;
+  constexpr int VE = T::kPerVec;
+  const long long pieces = to / VE, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const long long r = at / pieces, c = (at - r * pieces) * VE;
+  const elem *src = (const elem *)src_ + r * ld + c;
+  float f[VE];
+  if (c + VE <= cols) {
+    hd_store16<T>((elem *)dst_ + r * to + c, hd_load16<T>(src));
+  } else {
+#pragma unroll
+    for (int n = 0; n < VE; ++n) f[n] = c + n < cols ? T::load(src + n) : 0.f;
+    hd_store16<T>((elem *)dst_ + r * to + c, T::pack(f));
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------- the small kernels
+// Few rows, or few results altogether: time is launches and round trips to memory, not products.  A workgroup owns (16 TI) x (16 TJ)
+// results and its W waves split the contraction, step by step in turn; fragments go from global memory straight into registers, U
+// steps in flight, with no LDS and no barrier before the one where the waves' sums are joined (in a fixed order) for the epilogue.
+// DZ: P is dz, formed from dy and the slope as it is read, so that the whole backward pass of such a layer is one launch.
+struct Small {
+  Product a;
+  const void *slope;        // DZ
+  long long lds;            // its row stride
+};
+
+// the fragment values of row r at contraction indices k .. k + VE - 1 (the first `left` of them in range, others 0), as floats
+template <class T, bool ROWS, bool FULL>
+__device__ __forceinline__ void la_direct(const void *base, long long ld, long long r, long long k, long long left, float (&f)[T::kPerVec]) {
+  const typename T::elem *p = (const typename T::elem *)base;
+  if constexpr (!ROWS) {
+    p += r * ld + k;
+    if (FULL || left >= T::kPerVec) T::unpack(hd_load16<T>(p), f);
+    else
+#pragma unroll
+      for (int n = 0; n < T::kPerVec; ++n) f[n] = n < left ? T::load(p + n) : 0.f;
+  } else {
+    p += k * ld + r;
+#pragma unroll
+    for (int n = 0; n < T::kPerVec; ++n) f[n] = FULL || n < left ? T::load(p + n * ld) : 0.f;
+  }
+}
+template <class T, bool ROWS, bool FULL, bool DZ>
+__device__ __forceinline__ hd_u32x4 la_direct_frag(const void *base, long long ld, const void *slope, long long lds, long long r,
+                                                   long long k, long long left, float &sum) {
+  if constexpr (!DZ && !ROWS) {
+    if (FULL || left >= T::kPerVec) return hd_load16<T>((const typename T::elem *)base + r * ld + k);
+  }
+  float f[T::kPerVec];
+  la_direct<T, ROWS, FULL>(base, ld, r, k, left, f);
+  if constexpr (DZ) {
+    if (slope) {
+      float d[T::kPerVec];
+      la_direct<typename SlopeOf<T>::type, ROWS, FULL>(slope, lds, r, k, left, d);
+#pragma unroll
+      for (int n = 0; n < T::kPerVec; ++n) f[n] *= d[n];
+    }
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int n = 0; n < T::kPerVec; ++n) sum += f[n];
+    }
+  }
+  return T::pack(f);
+}
+
+// db (DZ and ROWS only): the row sums of P are written there too (fp32 or T), by the workgroups of j0 = 0.  `lds`: 16 TI TJ W KB.
+template <class T, bool PROWS, bool QROWS, int TI, int TJ, int W, bool DZ>
+__device__ __forceinline__ void la_small_tile(const Small &s, long long i0, long long j0, void *db, int db_f32, float *lds) {
+  constexpr int VE = T::kPerVec, KB = 4 * VE, NF = TI + TJ, U = PROWS || QROWS || DZ || NF > 4 ? 2 : 4;
+  const Product &a = s.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+  long long pr[TI], qr[TJ];                            // rows out of range repeat the last one: never stored
+#pragma unroll
+  for (int t = 0; t < TI; ++t) pr[t] = i0 + t * 16 + r < a.M ? i0 + t * 16 + r : a.M - 1;
+#pragma unroll
+  for (int u = 0; u < TJ; ++u) qr[u] = j0 + u * 16 + r < a.N ? j0 + u * 16 + r : a.N - 1;
+  la_f32x4 acc[TI][TJ] = {};
+  float sum[TI];
+#pragma unroll
+  for (int t = 0; t < TI; ++t) sum[t] = 0.f;
+  const bool sums = DZ && PROWS && db && j0 == 0;
+  // Steps come in pairs (128 bytes of a K operand's rows: whole cache lines), wave w takes pairs w, w + W, ...; a group of U steps is
+  // loaded while the one before is multiplied.
+  constexpr int GK = U * W * KB;                       // contraction indices of a group, over all waves
+  const long long groups = a.K / GK;
+  constexpr int SETS = PROWS || QROWS ? 1 : 2;
+  hd_u32x4 p[SETS][U][TI], q[SETS][U][TJ];
+  auto load = [&](auto buf_, long long group) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_)::value;
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      const long long kk = group * GK + ((n / 2 * W + wave) * 2 + n % 2) * KB + g * VE;
+#pragma unroll
+      for (int t = 0; t < TI; ++t)
+        p[buf][n][t] = la_direct_frag<T, PROWS, true, DZ>(a.p, a.ldp, s.slope, s.lds, pr[t], kk, VE, sum[t]);
+#pragma unroll
+      for (int u = 0; u < TJ; ++u) q[buf][n][u] = la_direct_frag<T, QROWS, true, false>(a.q, a.ldq, nullptr, 0, qr[u], kk, VE, sum[0]);
+    }
+    __builtin_amdgcn_sched_barrier(0);                 // all of them are on their way before the products below
+  };
+  auto multiply = [&](auto buf_) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_)::value;
+#pragma unroll
+    for (int n = 0; n < U; ++n)
+#pragma unroll
+      for (int t = 0; t < TI; ++t)
+#pragma unroll
+        for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, q[buf][n][u], p[buf][n][t], acc[t][u]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (PROWS || QROWS) {                      // (an R operand's loads are single elements: one set of registers is enough)
+    for (long long m = 0; m < groups; ++m) {
+      load(LaInt<0>{}, m);
+      multiply(LaInt<0>{});
+    }
+  } else if (groups > 0) {
+    load(LaInt<0>{}, 0);
+    long long m = 0;
+    for (; m + 2 < groups; m += 2) {
+      load(LaInt<1>{}, m + 1);
+      multiply(LaInt<0>{});
+      load(LaInt<0>{}, m + 2);
+      multiply(LaInt<1>{});
+    }
+    if (m + 1 < groups) {
+      load(LaInt<1>{}, m + 1);
+      multiply(LaInt<0>{});
+      multiply(LaInt<1>{});
+    } else {
+      multiply(LaInt<0>{});
+    }
+  }
+  long long k = groups * GK + (long long)wave * KB;
+  for (; k < a.K; k += W * KB) {
+    const long long kk = k + g * VE, left = a.K - kk;
+    hd_u32x4 pt[TI], qt[TJ];
+#pragma unroll
+    for (int t = 0; t < TI; ++t)
+      pt[t] = la_direct_frag<T, PROWS, false, DZ>(a.p, a.ldp, s.slope, s.lds, pr[t], kk, left, sum[t]);
+#pragma unroll
+    for (int u = 0; u < TJ; ++u) qt[u] = la_direct_frag<T, QROWS, false, false>(a.q, a.ldq, nullptr, 0, qr[u], kk, left, sum[0]);
+#pragma unroll
+    for (int t = 0; t < TI; ++t)
+#pragma unroll
+      for (int u = 0; u < TJ; ++u) acc[t][u] = la_mma(T{}, qt[u], pt[t], acc[t][u]);
+  }
+#pragma unroll
+  for (int t = 0; t < TI; ++t)
+#pragma unroll
+    for (int u = 0; u < TJ; ++u) *reinterpret_cast<la_f32x4 *>(lds + ((wave * TI * TJ + t * TJ + u) * 64 + lane) * 4) = acc[t][u];
+  __syncthreads();
+  for (int e = tid; e < TI * TJ * 64; e += W * 64) {
+    la_f32x4 z = *reinterpret_cast<const la_f32x4 *>(lds + e * 4);
+#pragma unroll
+    for (int w = 1; w < W; ++w) z += *reinterpret_cast<const la_f32x4 *>(lds + (w * TI * TJ * 64 + e) * 4);
+    const int l = e & 63, tu = e >> 6;
+    const long long i = i0 + (tu / TJ) * 16 + (l & 15), j = j0 + (tu % TJ) * 16 + (l >> 4) * 4;
+    if (i >= a.M) continue;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (j + n < a.N) la_finish_any<T>(a.e, a.N, i, j + n, z[n]);
+  }
+  if (sums) {                                          // uniform over the workgroup
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TI; ++t) lds[(wave * TI + t) * 64 + lane] = sum[t];
+    __syncthreads();
+    for (int e = tid; e < TI * 16; e += W * 64) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) v += lds[(w * TI + e / 16) * 64 + h * 16 + e % 16];
+      const long long i = i0 + e;
+      if (i >= a.M) continue;
+      if (db_f32) ((float *)db)[i] = v;
+      else ((typename T::elem *)db)[i] = T::round(v);
+    }
+  }
+}
+
+template <class T, int TI, int TJ, int W>
+__global__ __launch_bounds__(64 * W) void la_small_kernel(Product a) {
+  __shared__ __align__(16) float lds[W * TI * TJ * 256];
+  const long long gi = (a.M + 16 * TI - 1) / (16 * TI);
+  la_small_tile<T, false, false, TI, TJ, W, false>(Small{a, nullptr, 0}, blockIdx.x % gi * (16 * TI), blockIdx.x / gi * (16 * TJ), nullptr, 0,
+                                                   lds);
+}
+
+// dx and dW (and db) in one launch: the first `ndx` workgroups take tiles of dx, the others of dW
+template <class T>
+__global__ __launch_bounds__(256) void la_small_grad_kernel(Small x, Small w, int ndx, void *db, int db_f32) {
+  __shared__ __align__(16) float lds[4 * 4 * 256];
+  const int id = blockIdx.x;
+  if (id < ndx) {
+    const int gi = (int)((x.a.M + 31) / 32);
+    la_small_tile<T, false, true, 2, 2, 4, true>(x, (long long)(id % gi) * 32, (long long)(id / gi) * 32, nullptr, 0, lds);
+  } else {
+    const int gi = (int)((w.a.M + 31) / 32), at = id - ndx;
+    la_small_tile<T, true, true, 2, 2, 4, true>(w, (long long)(at % gi) * 32, (long long)(at / gi) * 32, db, db_f32, lds);
+  }
+}
+
+// dz = dy slope (or dy, SLOPE false) at row stride ldz, or NULL, and column sums: a workgroup takes 64 x VE columns and a strip of rows, its four
 // waves every fourth row; part (strips, N) fp32, or NULL.  Bound by its bytes (read dy and slope, write dz).
 template <class T, bool SLOPE>
 __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, int strip, const void *dy_, long long ldy,
-                                                    const void *slope_, void *dz_, float *part) {
+                                                    const void *slope_, void *dz_, long long ldz, float *part) {
   typedef typename T::elem elem;
   typedef typename SlopeOf<T>::type S;
   constexpr int VE = T::kPerVec, U = 4;
@@ -629,8 +762,8 @@ __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, in
           S::unpack(ws[u], d);
 #pragma unroll
           for (int n = 0; n < VE; ++n) f[n] *= d[n];
-          hd_store16<T>(dz + (i + 4 * u) * N, T::pack(f));
         }
+        if (dz_) hd_store16<T>(dz + (i + 4 * u) * ldz, T::pack(f));
 #pragma unroll
         for (int n = 0; n < VE; ++n) s[n] += f[n];
       }
@@ -643,8 +776,8 @@ __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, in
         float f = T::load((const elem *)dy_ + i * ldy + j + n);
         if constexpr (SLOPE) {
           f *= S::load((const typename S::elem *)slope_ + i * N + j + n);
-          ((elem *)dz_)[i * N + j + n] = T::round(f);
         }
+        if (dz_) ((elem *)dz_)[i * ldz + j + n] = T::round(f);
         s[n] += f;
       }
   }
@@ -678,58 +811,95 @@ __global__ __launch_bounds__(256) void la_db_kernel(long long N, int strips, con
   else ((typename T::elem *)db)[j] = T::round(s);
 }
 
-constexpr long long kMaxDim = 1LL << 31;
+constexpr long long kMaxDim = 1LL << 31, kMaxStride = 1LL << 22;
 
 inline long long la_div(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t la_align(size_t n) { return (n + 255) & ~(size_t)255; }
+inline long long la_size(int dtype) { return dtype == PN2_DT_F32 ? 4 : 2; }
+inline long long la_whole(long long n, int dtype) { return la_div(n, 16 / la_size(dtype)) * (16 / la_size(dtype)); }   // in 16-byte pieces
 
-// Which kernel a product takes, by size, type and alignment, and how often its contraction is split.
-//   big   (256 x 256, 16-bit only): tiles for at least three quarters of the CUs.  8192^3: 1.35-1.46 PFLOP/s against 0.88 for mid
-//   mid   (128 x 128, two workgroups per CU)
-//   any   (64 x 64): one side below 96, or operands whose rows are no 16-byte pieces
-// A contraction is split until two workgroups per CU run, each at least four steps long.
-enum { KERNEL_ANY, KERNEL_MID, KERNEL_BIG };
+// Which kernel a product takes, and how often its contraction is split, by size and type.  Microseconds measured for bf16 unless
+// said otherwise, this choice against the next one:
+//   small   (no LDS, waves split the contraction) few rows, or few results: 1 x 4096 x 4096 8.2 against 16.8 for a split 64 x 64 tile;
+//           72 x 512 x 256 4.1 against 7.9;  fp32 also up to 512 x 512 (8.0 against 12.8 for 64 x 64; bf16 5.6 against 5.0)
+//   64 x 64       up to 512 tiles: 1024^3 7.2 against 8.1 (128 x 64) and 11.0 (128 x 128)
+//   128 x 64      2048^3 22.5 against 25.6 (64 x 64) and 24.5 (128 x 128);  fp32 128 against 127 and 134
+//   128 x 128     fp32 from 512 such tiles on: 4096 x 4096 x 512 dW 147 against 167
+//   256 x 256     16-bit, tiles for three quarters of the CUs: 8192^3 784 against 1248 (128 x 128)
+// Splits only where a workgroup would walk a long contraction while CUs idle (a join costs a launch and the partial sums' traffic):
+// 128 x 8192 x 8192 58 -> 35 with four; 1024^3 7.2 -> 12.5 with two.
+enum { SMALL_11, SMALL_21, SMALL_22, TILE_64, TILE_128_64, TILE_128, TILE_256 };
+struct Plan {
+  int kernel, splits;
+  long long kchunk;         // contraction indices per split
+};
 
-bool la_vec(const void *p, long long ld, int dtype) {
-  const long long es = dtype == PN2_DT_F32 ? 4 : 2;
-  return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0 && ld <= (1 << 22);
-}
-
-int la_kernel_for(long long M, long long N, long long K, int dtype) {           // by size alone
-  if (M < 96 || N < 96 || K < (dtype == PN2_DT_F32 ? 16 : 32)) return KERNEL_ANY;
-  return dtype != PN2_DT_F32 && la_div(M, 256) * la_div(N, 256) >= 192 ? KERNEL_BIG : KERNEL_MID;
-}
-
-// the tile kernels' direct loads need 16-byte pieces: aligned bases and strides, and axes that are whole pieces
-bool la_pieces(const Product &a, int dtype, bool prows, bool qrows) {
-  const long long ve = dtype == PN2_DT_F32 ? 4 : 8;
-  return la_vec(a.p, a.ldp, dtype) && la_vec(a.q, a.ldq, dtype) && (prows ? a.M : a.K) % ve == 0 && (qrows ? a.N : a.K) % ve == 0;
-}
-
-// -> contraction indices per split
-long long la_chunk(long long M, long long N, long long K, int dtype, int kernel) {
-  const long long kb = dtype == PN2_DT_F32 ? 32 : 64, steps = la_div(K, kb);
-  const long long edge = kernel == KERNEL_BIG ? 256 : kernel == KERNEL_MID ? 128 : 64;
-  long long s = (kernel == KERNEL_BIG ? 256 : 512) / (la_div(M, edge) * la_div(N, edge));
-  if (s > steps / 2) s = steps / 2;
+Plan la_plan(long long M, long long N, long long K, int dtype, bool small_ok) {
+  const bool f32 = dtype == PN2_DT_F32;
+  const long long n16 = la_div(M, 16) * la_div(N, 16);
+  Plan p{TILE_64, 1, K};
+  if (small_ok && K <= 16384) {
+    if (M <= 16) p.kernel = SMALL_11;
+    else if (M <= 32) p.kernel = SMALL_21;
+    else if (n16 <= 256) p.kernel = SMALL_11;
+    else if (n16 <= 512) p.kernel = SMALL_21;
+    else if (n16 <= (f32 ? 1024 : 512) || (N <= 32 && K <= 1024)) p.kernel = SMALL_22;
+    if (p.kernel != TILE_64) return p;
+  }
+  const long long t256 = la_div(M, 256) * la_div(N, 256), t128 = la_div(M, 128) * la_div(N, 128), t12864 = la_div(M, 128) * la_div(N, 64),
+                  t64 = la_div(M, 64) * la_div(N, 64);
+  long long tiles = t64;
+  if (!f32 && t256 >= 192) { p.kernel = TILE_256; tiles = t256; }
+  else if (f32 && t128 >= 512) { p.kernel = TILE_128; tiles = t128; }
+  else if (t64 > 512) { p.kernel = TILE_128_64; tiles = t12864; }
+  const long long kb = f32 ? 32 : 64, steps = la_div(K, kb);
+  long long s = (p.kernel == TILE_256 ? 256 : 512) / tiles;
+  if (s > steps / 32) s = steps / 32;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
-  return la_div(steps, s) * kb;
+  p.kchunk = la_div(steps, s) * kb;
+  p.splits = (int)la_div(K, p.kchunk);
+  return p;
+}
+size_t la_partial_bytes(const Plan &p, long long M, long long N) { return p.splits > 1 ? la_align((size_t)p.splits * M * N * 4) : 0; }
+
+// An operand as it is, or as a padded copy: the tile kernels' direct loads need rows of whole 16-byte pieces at 16-byte addresses.
+// rows x cols at row stride ld; an R operand's rows must also END with a piece.
+struct Matrix {
+  const void *p;
+  long long rows, cols, ld;
+  bool R;
+};
+bool la_direct_ok(const Matrix &o, int dtype) {
+  return ((uintptr_t)o.p & 15) == 0 && o.ld * la_size(dtype) % 16 == 0 && o.ld <= kMaxStride && (!o.R || la_whole(o.cols, dtype) == o.cols);
+}
+size_t la_copy_bytes(const Matrix &o, int dtype) {
+  return la_direct_ok(o, dtype) ? 0 : la_align((size_t)o.rows * la_whole(o.cols, dtype) * la_size(dtype));
 }
 
-size_t la_partial_bytes(long long M, long long N, long long K, int dtype, int kernel) {
-  const long long splits = la_div(K, la_chunk(M, N, K, dtype, kernel));
-  return splits > 1 ? la_align((size_t)splits * M * N * 4) : 0;
-}
+struct Space {              // the caller's workspace, handed out piece by piece
+  char *at;
+  void *take(size_t n) {
+    void *p = n ? at : nullptr;
+    at += n;
+    return p;
+  }
+};
 
-// the most a product of this size can need, whatever its operands' alignment
-size_t la_product_bytes(long long M, long long N, long long K, int dtype) {
-  const size_t any = la_partial_bytes(M, N, K, dtype, KERNEL_ANY), tile = la_partial_bytes(M, N, K, dtype, la_kernel_for(M, N, K, dtype));
-  return any > tile ? any : tile;
+template <class T>
+void la_pad(Matrix &o, int dtype, Space &ws, hipStream_t st) {
+  const size_t n = la_copy_bytes(o, dtype);
+  if (!n) return;
+  void *to = ws.take(n);
+  const long long ld = la_whole(o.cols, dtype);
+  la_pad_kernel<T><<<(unsigned)la_div(o.rows * (ld / T::kPerVec), 256), 256, 0, st>>>(o.rows, o.cols, o.p, o.ld, to, ld);
+  o.p = to;
+  o.ld = ld;
+  if (o.R) o.cols = ld;
 }
 
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
-int la_tile_as(const Product &a, hipStream_t st) {
+void la_tile_as(const Product &a, hipStream_t st) {
   const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
   const dim3 grid((unsigned)(gi * gj), 1, (unsigned)a.splits);
   constexpr int NT = 64 * WI * WJ;
@@ -744,32 +914,71 @@ int la_tile_as(const Product &a, hipStream_t st) {
       default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
     }
   }
-  if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 256), 256, 0, st>>>(a);
-  return pn2_check_launch();
+  if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 1024), 256, 0, st>>>(a);
 }
 
+template <class T, int TI, int TJ, int W>
+void la_small_as(const Product &a, hipStream_t st) {
+  la_small_kernel<T, TI, TJ, W><<<(unsigned)(la_div(a.M, 16 * TI) * la_div(a.N, 16 * TJ)), 64 * W, 0, st>>>(a);
+}
+
+// C = P Q^T by the plan; P and Q are fit for it (padded where a tile kernel reads them)
 template <class T, bool PROWS, bool QROWS>
-int la_product(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) {
-  const int kernel = la_pieces(a, dtype, PROWS, QROWS) ? la_kernel_for(a.M, a.N, a.K, dtype) : KERNEL_ANY;
-  a.kchunk = la_chunk(a.M, a.N, a.K, dtype, kernel);
-  a.splits = (int)la_div(a.K, a.kchunk);
-  const size_t need = la_partial_bytes(a.M, a.N, a.K, dtype, kernel);
-  if (ws_bytes < need) return PN2_ENOSPC;
-  if (need && !ws) return PN2_ENULL;
-  a.partial = (float *)ws;
-  if constexpr (sizeof(typename T::elem) == 2) {
-    if (kernel == KERNEL_BIG) return la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4>(a, st);
+int la_product(const Plan &plan, const Matrix &p, const Matrix &q, long long M, long long N, long long K, const Epilogue &e,
+               Space ws, hipStream_t st) {
+  Product a{};
+  a.M = M; a.N = N; a.K = K;
+  a.p = p.p; a.ldp = p.ld; a.rp = PROWS ? p.cols : p.rows;
+  a.q = q.p; a.ldq = q.ld; a.rq = QROWS ? q.cols : q.rows;
+  a.splits = plan.splits;
+  a.kchunk = plan.kchunk;
+  a.partial = (float *)ws.take(la_partial_bytes(plan, M, N));
+  a.e = e;
+  switch (plan.kernel) {
+    case TILE_256:
+      if constexpr (sizeof(typename T::elem) == 2) { la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4>(a, st); break; }
+      return PN2_EINVAL;                               // (never planned for fp32)
+    case TILE_128:
+      if constexpr (sizeof(typename T::elem) == 4) { la_tile_as<T, PROWS, QROWS, 2, 2, 4, 4>(a, st); break; }
+      return PN2_EINVAL;                               // (never planned for 16-bit types)
+    case TILE_128_64: la_tile_as<T, PROWS, QROWS, 2, 2, 4, 2>(a, st); break;
+    case TILE_64: la_tile_as<T, PROWS, QROWS, 2, 2, 2, 2>(a, st); break;
+    default:
+      if constexpr (!PROWS && !QROWS) {
+        if (plan.kernel == SMALL_11) la_small_as<T, 1, 1, 8>(a, st);
+        else if (plan.kernel == SMALL_21) la_small_as<T, 2, 1, 8>(a, st);
+        else la_small_as<T, 2, 2, 4>(a, st);
+      }
   }
-  if (kernel != KERNEL_ANY) return la_tile_as<T, PROWS, QROWS, 2, 2, 4, 4>(a, st);
-  const long long gx = la_div(a.M, 64), gy = la_div(a.N, 64);
-  if (gy > 65535) return PN2_EINVAL;
-  la_any_kernel<T, PROWS, QROWS><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)a.splits), 256, 0, st>>>(a);
-  if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 256), 256, 0, st>>>(a);
   return pn2_check_launch();
 }
 
 inline bool la_bad(long long M, long long N, long long K, int dtype) {
-  return M < 0 || N < 1 || K < 1 || M >= kMaxDim || N > 65535LL * 64 || K > 65535LL * 64 || dtype < PN2_DT_F32 || dtype > PN2_DT_F16;
+  return M < 0 || N < 1 || K < 1 || M >= kMaxDim || N > kMaxStride || K > kMaxStride || dtype < PN2_DT_F32 || dtype > PN2_DT_F16;
+}
+
+struct Forward {
+  Plan plan;
+  Matrix x, w;
+  size_t bytes;
+};
+Forward la_forward_plan(long long M, long long N, long long K, int dtype, const void *x, long long ldx, const void *w, long long ldw) {
+  Forward f;
+  f.plan = la_plan(M, N, K, dtype, true);
+  f.x = {x, M, K, ldx, false};
+  f.w = {w, N, K, ldw, false};
+  f.bytes = la_partial_bytes(f.plan, M, N);
+  if (f.plan.kernel >= TILE_64) f.bytes += la_copy_bytes(f.x, dtype) + la_copy_bytes(f.w, dtype);
+  return f;
+}
+template <class T>
+int la_forward(Forward f, long long M, long long N, long long K, int dtype, const Epilogue &e, void *ws, hipStream_t st) {
+  Space space{(char *)ws};
+  if (f.plan.kernel >= TILE_64) {
+    la_pad<T>(f.x, dtype, space, st);
+    la_pad<T>(f.w, dtype, space, st);
+  }
+  return la_product<T, false, false>(f.plan, f.x, f.w, M, N, K, e, space, st);
 }
 
 // rows per partial column sum: enough workgroups for the chip, at least 16 rows each, at most 512 strips
@@ -781,67 +990,88 @@ inline int la_strip(long long M, long long N, int dtype) {
   return (int)(s < 16 ? 16 : s);
 }
 
-template <class T>
-int la_forward(Product a, int dtype, void *ws, size_t ws_bytes, hipStream_t st) {
-  return la_product<T, false, false>(a, dtype, ws, ws_bytes, st);
+// The backward pass: one launch where everything is small (contractions of at most 2048 and 4096, 2^27 products: 512^3 10 us against 27
+// for the launches of the general path, whose launches a host thread also has to make), otherwise dz and db's strips, dx, dW.
+struct Backward {
+  bool small, own_dz;       // own_dz: dz is written (it is not dy itself)
+  Plan px, pw;
+  Matrix dz, dzr, w, x;   // dz as the K operand of dx and as the R operand of dW
+  size_t dz_bytes, part, copies, partial, bytes;
+};
+Backward la_backward_plan(long long M, long long N, long long K, int dtype, const void *dy, long long ldy, bool slope, const void *x,
+                          long long ldx, const void *w, long long ldw, int want) {
+  Backward b{};
+  b.small = (double)M * N * K <= (double)(1 << 27) && M <= 2048 && N <= 4096 && (want & 3) && !((want & 4) && !(want & 2));
+  if (b.small) return b;
+  const bool products = (want & 3) != 0;
+  b.dz = {dy, M, N, ldy, false};
+  b.dzr = {dy, M, N, ldy, true};
+  b.w = {w, N, K, ldw, true};
+  b.x = {x, M, K, ldx, true};
+  b.own_dz = products && (slope || !la_direct_ok(b.dz, dtype) || ((want & 2) && !la_direct_ok(b.dzr, dtype)));
+  b.dz_bytes = b.own_dz ? la_align((size_t)M * la_whole(N, dtype) * la_size(dtype)) : 0;
+  b.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
+  b.px = la_plan(M, K, N, dtype, false);
+  b.pw = la_plan(N, K, M, dtype, false);
+  // the two products use the rest one after the other
+  const size_t dx = (want & 1) ? la_copy_bytes(b.w, dtype) + la_partial_bytes(b.px, M, K) : 0;
+  const size_t dw = (want & 2) ? la_copy_bytes(b.x, dtype) + la_partial_bytes(b.pw, N, K) : 0;
+  b.bytes = b.dz_bytes + b.part + (dx > dw ? dx : dw);
+  return b;
 }
 
-struct GradSizes { size_t dz, part, dx, dw, all; };
-GradSizes la_grad_sizes(long long M, long long N, long long K, int dtype, int has_slope, int want) {
-  GradSizes g{};
-  const size_t es = dtype == PN2_DT_F32 ? 4 : 2;
-  g.dz = has_slope ? la_align((size_t)M * N * es) : 0;
-  g.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
-  g.dx = (want & 1) ? la_product_bytes(M, K, N, dtype) : 0;
-  g.dw = (want & 2) ? la_product_bytes(N, K, M, dtype) : 0;
-  g.all = g.dz + g.part + (g.dx > g.dw ? g.dx : g.dw);      // the two products share their partial sums' space, one after the other
-  return g;
-}
-
 template <class T>
-int la_backward(long long M, long long N, long long K, int dtype, const void *dy, long long ldy, const void *slope, const void *x,
-                long long ldx, const void *w, long long ldw, void *dx, void *dw, void *db, int db_f32, void *ws, size_t ws_bytes,
+int la_backward(Backward b, long long M, long long N, long long K, int dtype, const void *dy, long long ldy, const void *slope,
+                const void *x, long long ldx, const void *w, long long ldw, void *dx, void *dw, void *db, int db_f32, void *ws,
                 hipStream_t st) {
-  const int want = (dx ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0);
-  const GradSizes g = la_grad_sizes(M, N, K, dtype, slope != nullptr, want);
-  if (ws_bytes < g.all) return PN2_ENOSPC;
-  if (g.all && !ws) return PN2_ENULL;
-  char *at = (char *)ws;
-  void *dz = slope ? at : nullptr;
-  float *part = db ? (float *)(at + g.dz) : nullptr;
-  char *rest = at + g.dz + g.part;
-  const size_t rest_bytes = ws_bytes - g.dz - g.part;
-  if (slope || db) {
+  if (b.small) {
+    Small sx{}, sw{};
+    sx.a.M = M; sx.a.N = K; sx.a.K = N; sx.a.p = dy; sx.a.ldp = ldy; sx.a.q = w; sx.a.ldq = ldw; sx.a.e.y = dx; sx.slope = slope; sx.lds = N;
+    sw.a.M = N; sw.a.N = K; sw.a.K = M; sw.a.p = dy; sw.a.ldp = ldy; sw.a.q = x; sw.a.ldq = ldx; sw.a.e.y = dw; sw.slope = slope; sw.lds = N;
+    const long long ndx = dx ? la_div(M, 32) * la_div(K, 32) : 0, ndw = dw ? la_div(N, 32) * la_div(K, 32) : 0;
+    la_small_grad_kernel<T><<<(unsigned)(ndx + ndw), 256, 0, st>>>(sx, sw, (int)ndx, db, db_f32);
+    return pn2_check_launch();
+  }
+  Space space{(char *)ws};
+  void *dz = space.take(b.dz_bytes);
+  float *part = (float *)space.take(b.part);
+  const long long ldz = la_whole(N, dtype);
+  if (b.own_dz || db) {
     const int strip = la_strip(M, N, dtype), strips = (int)la_div(M, strip);
     const dim3 grid((unsigned)la_div(N, 64 * T::kPerVec), (unsigned)strips);
-    if (slope) la_dz_kernel<T, true><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, part);
-    else la_dz_kernel<T, false><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, nullptr, part);
+    if (slope) la_dz_kernel<T, true><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, ldz, part);
+    else la_dz_kernel<T, false><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, dz, ldz, part);
     if (db) la_db_kernel<T><<<(unsigned)la_div(N, 64), 256, 0, st>>>(N, strips, part, db, db_f32);
     const int rc = pn2_check_launch();
     if (rc != PN2_OK) return rc;
   }
-  const void *z = slope ? dz : dy;
-  const long long ldz = slope ? N : ldy;
+  if (b.own_dz) {
+    b.dz.p = b.dzr.p = dz;
+    b.dz.ld = b.dzr.ld = b.dzr.cols = ldz;
+  }
+  Epilogue e{};
   if (dx) {
-    Product a{};
-    a.M = M; a.N = K; a.K = N; a.p = z; a.ldp = ldz; a.q = w; a.ldq = ldw; a.e.y = dx;
-    const int rc = la_product<T, false, true>(a, dtype, rest, rest_bytes, st);
+    Space rest = space;
+    la_pad<T>(b.w, dtype, rest, st);
+    e.y = dx;
+    const int rc = la_product<T, false, true>(b.px, b.dz, b.w, M, K, N, e, rest, st);
     if (rc != PN2_OK) return rc;
   }
   if (dw) {
-    Product a{};
-    a.M = N; a.N = K; a.K = M; a.p = z; a.ldp = ldz; a.q = x; a.ldq = ldx; a.e.y = dw;
-    const int rc = la_product<T, true, true>(a, dtype, rest, rest_bytes, st);
-    if (rc != PN2_OK) return rc;
+    Space rest = space;
+    la_pad<T>(b.x, dtype, rest, st);
+    e.y = dw;
+    return la_product<T, true, true>(b.pw, b.dzr, b.x, N, K, M, e, rest, st);
   }
   return PN2_OK;
 }
 
 }  // namespace
 
-extern "C" size_t pn2_linear_act_workspace_bytes(long long M, int N, int K, int dtype) {
+extern "C" size_t pn2_linear_act_workspace_bytes(long long M, int N, int K, int dtype, const void *x, long long ldx, const void *w,
+                                                 long long ldw) {
   if (la_bad(M, N, K, dtype) || M == 0) return 0;
-  return la_product_bytes(M, N, K, dtype);
+  return la_forward_plan(M, N, K, dtype, x, ldx, w, ldw).bytes;
 }
 
 extern "C" int pn2_linear_act(long long M, int N, int K, int dtype, const void *x, long long ldx, const void *w, long long ldw,
@@ -852,19 +1082,22 @@ extern "C" int pn2_linear_act(long long M, int N, int K, int dtype, const void *
     return PN2_EINVAL;
   if (M == 0) return PN2_OK;
   if (!x || !w || !y) return PN2_ENULL;
-  Product a{};
-  a.M = M; a.N = N; a.K = K; a.p = x; a.ldp = ldx; a.q = w; a.ldq = ldw;
-  a.e.bias = bias; a.e.bias_f32 = bias_dtype == PN2_DT_F32; a.e.act = act; a.e.res = residual; a.e.ldr = ldr; a.e.y = y;
-  a.e.slope = act == ACT_NONE ? nullptr : slope;
+  const Forward f = la_forward_plan(M, N, K, dtype, x, ldx, w, ldw);
+  if (workspace_bytes < f.bytes) return PN2_ENOSPC;
+  if (f.bytes && !workspace) return PN2_ENULL;
+  Epilogue e{};
+  e.bias = bias; e.bias_f32 = bias_dtype == PN2_DT_F32; e.act = act; e.res = residual; e.ldr = ldr; e.y = y;
+  e.slope = act == ACT_NONE ? nullptr : slope;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == PN2_DT_F32) return la_forward<HdF32>(a, dtype, workspace, workspace_bytes, st);
-  if (dtype == PN2_DT_BF16) return la_forward<HdBF16>(a, dtype, workspace, workspace_bytes, st);
-  return la_forward<HdF16>(a, dtype, workspace, workspace_bytes, st);
+  if (dtype == PN2_DT_F32) return la_forward<HdF32>(f, M, N, K, dtype, e, workspace, st);
+  if (dtype == PN2_DT_BF16) return la_forward<HdBF16>(f, M, N, K, dtype, e, workspace, st);
+  return la_forward<HdF16>(f, M, N, K, dtype, e, workspace, st);
 }
 
-extern "C" size_t pn2_linear_act_grad_workspace_bytes(long long M, int N, int K, int dtype, int has_slope, int want) {
+extern "C" size_t pn2_linear_act_grad_workspace_bytes(long long M, int N, int K, int dtype, const void *dy, long long ldy, int has_slope,
+                                                      const void *x, long long ldx, const void *w, long long ldw, int want) {
   if (la_bad(M, N, K, dtype) || M == 0) return 0;
-  return la_grad_sizes(M, N, K, dtype, has_slope, want).all;
+  return la_backward_plan(M, N, K, dtype, dy, ldy, has_slope != 0, x, ldx, w, ldw, want).bytes;
 }
 
 extern "C" int pn2_linear_act_grad(long long M, int N, int K, int dtype, const void *dy, long long ldy, const void *slope,
@@ -873,9 +1106,14 @@ extern "C" int pn2_linear_act_grad(long long M, int N, int K, int dtype, const v
   if (la_bad(M, N, K, dtype) || M < 1 || ldy < 0 || ldx < 0 || ldw < 0 || (db && db_dtype != dtype && db_dtype != PN2_DT_F32))
     return PN2_EINVAL;
   if (!dy || (dx && !w) || (dw && !x)) return PN2_ENULL;
+  const int want = (dx ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0);
+  if (!want) return PN2_OK;
+  const Backward b = la_backward_plan(M, N, K, dtype, dy, ldy, slope != nullptr, x, ldx, w, ldw, want);
+  if (workspace_bytes < b.bytes) return PN2_ENOSPC;
+  if (b.bytes && !workspace) return PN2_ENULL;
   hipStream_t st = (hipStream_t)stream;
   const int f32 = db_dtype == PN2_DT_F32;
-  if (dtype == PN2_DT_F32) return la_backward<HdF32>(M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, workspace_bytes, st);
-  if (dtype == PN2_DT_BF16) return la_backward<HdBF16>(M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, workspace_bytes, st);
-  return la_backward<HdF16>(M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, workspace_bytes, st);
+  if (dtype == PN2_DT_F32) return la_backward<HdF32>(b, M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, st);
+  if (dtype == PN2_DT_BF16) return la_backward<HdBF16>(b, M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, st);
+  return la_backward<HdF16>(b, M, N, K, dtype, dy, ldy, slope, x, ldx, w, ldw, dx, dw, db, f32, workspace, st);
 }

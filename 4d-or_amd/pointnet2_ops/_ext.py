@@ -274,9 +274,10 @@ _lib.pn2_x3_gemm_supported.argtypes = [_c_int] * 5
 _lib.pn2_x3_gemm_supported.restype = _c_int
 _lib.pn2_x3_gemm_first_supported.argtypes = [_c_int] * 3
 _lib.pn2_x3_gemm_first_supported.restype = _c_int
-_lib.pn2_linear_act_workspace_bytes.argtypes = [ctypes.c_longlong] + [_c_int] * 3
+_lib.pn2_linear_act_workspace_bytes.argtypes = [ctypes.c_longlong] + [_c_int] * 3 + [_c_vp, ctypes.c_longlong] * 2
 _lib.pn2_linear_act_workspace_bytes.restype = _c_sz
-_lib.pn2_linear_act_grad_workspace_bytes.argtypes = [ctypes.c_longlong] + [_c_int] * 5
+_lib.pn2_linear_act_grad_workspace_bytes.argtypes = ([ctypes.c_longlong] + [_c_int] * 3 + [_c_vp, ctypes.c_longlong, _c_int] +
+                                                     [_c_vp, ctypes.c_longlong] * 2 + [_c_int])
 _lib.pn2_linear_act_grad_workspace_bytes.restype = _c_sz
 _lib.pn2_abi_version.restype = _c_int
 _lib.pn2_last_hip_error.restype = _c_int
@@ -2316,7 +2317,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None, want_slop
     slope = torch.empty(M, N, dtype=_slope_dtype(x.dtype), device=x.device) if want_slope and act else None
     if M == 0:
         return y, slope
-    nb = _lib.pn2_linear_act_workspace_bytes(M, N, K, dt)
+    nb = _lib.pn2_linear_act_workspace_bytes(M, N, K, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw)
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
     es = x.element_size()
     _call("pn2_linear_act", x, M, N, K, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), dt if bias is None else _DT[bias.dtype],
@@ -2354,7 +2355,8 @@ def linear_act_grad(dy, slope, x, weight, want_dx=True, want_dw=True, bias_dtype
     want = (1 if want_dx else 0) | (2 if want_dw else 0) | (4 if db is not None else 0)
     if M == 0 or want == 0:
         return dx, dw, db
-    nb = _lib.pn2_linear_act_grad_workspace_bytes(M, N, K, dt, int(slope is not None), want)
+    nb = _lib.pn2_linear_act_grad_workspace_bytes(M, N, K, dt, dy.data_ptr(), ldy, int(slope is not None), _ptr(x), ldx, _ptr(weight),
+                                                  ldw, want)
     ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
     es = dy.element_size()
     _call("pn2_linear_act_grad", dy, M, N, K, dt, dy.data_ptr(), ldy, _ptr(slope), _ptr(x), ldx, _ptr(weight), ldw, _ptr(dx),

@@ -968,12 +968,14 @@ int pn2_distill_topk_grad(long long T, int V, long long ld, int dtype, const voi
  * fp32 for fp32 and fp16 for both 16-bit types (NULL: not wanted; never written for act 0).
  * The gradient: dy (M, N) at row stride ldy; slope NULL stands for ones; dx (M, K), dw (N, K) dense, db (N) of db_dtype, each NULL
  * = not wanted, every element written; sums in a fixed order.  want = 1 dx | 2 dw | 4 db.
- * 1 <= N, K <= 4194240.  A workspace must not be shared by calls that may run at the same time. */
-size_t pn2_linear_act_workspace_bytes(long long M, int N, int K, int dtype);
+ * 1 <= N, K <= 4194304.  The workspace sizes take the operands (only their alignment is looked at).  A workspace must not be
+ * shared by calls that may run at the same time. */
+size_t pn2_linear_act_workspace_bytes(long long M, int N, int K, int dtype, const void *x, long long ldx, const void *w, long long ldw);
 int pn2_linear_act(long long M, int N, int K, int dtype, const void *x, long long ldx, const void *w, long long ldw,
                    const void *bias, int bias_dtype, int act, const void *residual, long long ldr, void *y, void *slope,
                    void *workspace, size_t workspace_bytes, void *stream);
-size_t pn2_linear_act_grad_workspace_bytes(long long M, int N, int K, int dtype, int has_slope, int want);
+size_t pn2_linear_act_grad_workspace_bytes(long long M, int N, int K, int dtype, const void *dy, long long ldy, int has_slope,
+                                           const void *x, long long ldx, const void *w, long long ldw, int want);
 int pn2_linear_act_grad(long long M, int N, int K, int dtype, const void *dy, long long ldy, const void *slope, const void *x,
                         long long ldx, const void *w, long long ldw, void *dx, void *dw, void *db, int db_dtype,
                         void *workspace, size_t workspace_bytes, void *stream);

@@ -63,19 +63,22 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     def linear(M=4, N=4, K=4, dt=0, x=some, w=some, b=None, bdt=0, act=0, y=some, ws=None, nb=0):
         return lib.pn2_linear_act(M, N, K, dt, x, K, w, K, b, bdt, act, None, 0, y, None, ws, nb, None)
     assert linear(M=-1) == linear(N=0) == linear(K=0) == linear(dt=3) == linear(dt=-1) == linear(act=5) == linear(act=-1) == EINVAL
-    assert linear(dt=1, b=some, bdt=2) == linear(M=big) == linear(N=(1 << 22)) == EINVAL
+    assert linear(dt=1, b=some, bdt=2) == linear(M=big) == linear(N=(1 << 22) + 1) == EINVAL
     assert linear(x=None) == linear(w=None) == linear(y=None) == ENULL
     assert linear(M=0, x=None) == 0
     # a product whose contraction is split needs its workspace
-    assert lib.pn2_linear_act_workspace_bytes(64, 64, 4096, 0) > 0
-    assert linear(M=64, N=64, K=4096) == ENOSPC
-    assert linear(M=64, N=64, K=4096, nb=big) == ENULL
+    assert lib.pn2_linear_act_workspace_bytes(64, 64, 32768, 0, some, 32768, some, 32768) > 0
+    assert linear(M=64, N=64, K=32768) == ENOSPC
+    assert linear(M=64, N=64, K=32768, nb=big) == ENULL
+    # ... and one whose operands have to be padded (a row stride of no whole 16 bytes)
+    assert lib.pn2_linear_act_workspace_bytes(2048, 2048, 512, 1, some, 512, some, 512) == 0
+    assert lib.pn2_linear_act_workspace_bytes(2048, 2048, 512, 1, some, 513, some, 512) >= 2048 * 512 * 2
 
     def grad(M=4, dy=some, x=some, w=some, dx=some, dw=some, db=None, bdt=0, nb=big, ws=some):
         return lib.pn2_linear_act_grad(M, 4, 4, 0, dy, 4, None, x, 4, w, 4, dx, dw, db, bdt, ws, nb, None)
     assert grad(M=0) == grad(db=some, bdt=1) == EINVAL
     assert grad(dy=None) == grad(x=None) == grad(w=None) == ENULL
-    assert lib.pn2_linear_act_grad_workspace_bytes(4, 4, 4, 0, 1, 7) > 0
+    assert lib.pn2_linear_act_grad_workspace_bytes(4096, 512, 512, 0, some, 512, 1, some, 512, some, 512, 7) >= 4096 * 512 * 4
 
     def labels(T=4, V=8, dt=0, x=some, y=some, top=0, lp=some, tl=None):
         return lib.pn2_label_logprobs(T, V, V, dt, x, y, -100, top, lp, some, None, tl, tl, None)
