@@ -16,14 +16,15 @@
 // overflow, are summed again with (x - m) c.
 //
 // Alternatives without a compare per element: every thread keeps the key (maximum, first vector that holds it) of its share
-// of the row; the k best elements of a row lie in the shares of the k threads with the best keys (an element of another
-// thread has k better keys above it), so only those shares are looked at again (from L2): k / BT of the row.
+// of the row.  64 groups of threads give 64 distinct keys; the k-th best of them is a lower bound of the k best elements (k groups
+// hold one at least as good), so only the shares of threads whose key reaches it are looked at again (from L2): for k = 20 about
+// 24 of 512.  Their elements at or above the bound are ranked by counting.
 #include "head_common.h"
 
 namespace {
 
-constexpr int kMaxTop = 64;              // one list entry per lane
-constexpr int kSmallV = 1024;            // up to here: one wave per row, the row in registers
+constexpr int kMaxTop = 64;              // one alternative per lane, one group of threads per alternative
+constexpr int kSmallV = 2048;            // up to here: one wave per row, the row in registers
 
 // order-preserving map float -> unsigned (-0 = +0; -inf -> kKeyNegInf; 0 = "nothing")
 constexpr unsigned kKeyNegInf = 0x007fffffu;
@@ -35,26 +36,17 @@ __device__ __forceinline__ float lp_unkey(unsigned k) {
   return __builtin_bit_cast(float, (int)k < 0 ? k & 0x7fffffffu : ~k);
 }
 
-// lane i <- lane i - 1 (lane 0 keeps its own)
-__device__ __forceinline__ unsigned lp_shift_up(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x138, 0xF, 0xF, false);   // wave_shr:1
-}
-
-// A descending list of 64 (key, index) pairs, one per lane; equal keys in ascending index order; key 0 = empty.
-struct TopList {
-  unsigned key;
-  int idx;
-  __device__ __forceinline__ void clear() { key = 0u; idx = 0x7fffffff; }
-  __device__ __forceinline__ bool above(unsigned k, int i) const { return key > k || (key == k && idx < i); }
-  __device__ __forceinline__ void insert(unsigned k, int i) {          // (k, i) wave-uniform
-    const int pos = __popcll(__ballot(above(k, i)));
-    const int lane = pn2_lane();
-    const unsigned pk = lp_shift_up(key);
-    const int pi = (int)lp_shift_up((unsigned)idx);
-    key = lane > pos ? pk : (lane == pos ? k : key);
-    idx = lane > pos ? pi : (lane == pos ? i : idx);
+// how many of the first n lanes' keys are larger than this lane's (equal keys: only 0, "nothing")
+__device__ __forceinline__ int lp_rank64(u64 key, int n) {
+  int rank = 0;
+  if (n >= 64) {
+#pragma unroll 8
+    for (int q = 0; q < 64; ++q) rank += pn2_readlane_u64(key, q) > key ? 1 : 0;
+  } else {
+    for (int q = 0; q < n; ++q) rank += pn2_readlane_u64(key, q) > key ? 1 : 0;
   }
-};
+  return rank;
+}
 
 struct RowSum {          // running statistics of (a part of) a row
   float m, M2, s, se;
@@ -134,16 +126,23 @@ __device__ __forceinline__ float lp_teacher(const FwdArgs &a, long long at) {
   return (float)((const _Float16 *)a.t_val)[at];
 }
 
-// One wave finishes a label row: stats are wave-uniform.
+// A row's label and its logit, read before the row itself (two dependent round trips to memory).
+struct Label {
+  long long y;
+  float x;
+};
 template <class T>
-__device__ __forceinline__ void lp_finish_label(const FwdArgs &a, long long row, const typename T::elem *x, const RowStat &r) {
+__device__ __forceinline__ Label lp_label(const FwdArgs &a, long long row, const typename T::elem *x) {
+  Label l;
+  l.y = a.labels[row];
+  l.x = l.y >= 0 && l.y < a.V ? T::load(x + l.y) : __builtin_nanf("");
+  return l;
+}
+// One wave finishes a label row: stats are wave-uniform.
+__device__ __forceinline__ void lp_finish_label(const FwdArgs &a, long long row, const Label &l, const RowStat &r) {
   if (pn2_lane() == 0) {
-    const long long y = a.labels[row];
     float lp = 0.f;
-    if (y != a.ignore) {
-      if (y < 0 || y >= a.V) lp = __builtin_nanf("");
-      else lp = lp_logp(T::load(x + y), r);
-    }
+    if (l.y != a.ignore) lp = l.y < 0 || l.y >= a.V ? l.x : lp_logp(l.x, r);
     a.log_prob[row] = lp;
     a.entropy[row] = r.entropy;
     if (a.stats) {
@@ -212,17 +211,20 @@ __device__ __forceinline__ void lp_finish_distill(const FwdArgs &a, long long ro
   }
 }
 
-__device__ __forceinline__ void lp_write_top(const FwdArgs &a, long long row, const TopList &l, const RowStat &r) {
-  const int lane = pn2_lane();
-  if (lane >= a.top) return;
-  const bool none = l.key <= kKeyNegInf || r.nan;
-  a.top_lp[row * a.top + lane] = r.nan ? __builtin_nanf("") : (none ? -kHdInf : lp_logp(lp_unkey(l.key), r));
-  a.top_idx[row * a.top + lane] = none ? -1 : l.idx;
-}
-
 enum { MODE_LABEL, MODE_DISTILL };
 
-// ------------------------------------------------------------------------------------------------ V <= 1024: a wave per row
+// one of the n candidates in LDS takes the place its rank gives it
+__device__ __forceinline__ void lp_place(const FwdArgs &a, long long row, const u64 *cand, int n, u64 mine, const RowStat &st) {
+  int rank = 0;
+#pragma unroll 8
+  for (int q = 0; q < n; ++q) rank += cand[q] > mine ? 1 : 0;
+  if (rank < a.top) {
+    a.top_lp[row * a.top + rank] = lp_logp(lp_unkey((unsigned)(mine >> 32)), st);
+    a.top_idx[row * a.top + rank] = (int)~(unsigned)mine;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ V <= 2048: a wave per row
 template <class T, int MODE, int EPL>
 __global__ __launch_bounds__(256) void lp_small_kernel(FwdArgs a) {
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -236,12 +238,18 @@ __global__ __launch_bounds__(256) void lp_small_kernel(FwdArgs a) {
       return;
     }
   }
+  Label label{};
+  if constexpr (MODE == MODE_LABEL) label = lp_label<T>(a, row, x);
   float v[EPL];
   float m = -kHdInf;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
+  for (int j = 0; j < EPL; ++j) {                      // (loads at clamped places: a branch each would make them wait for each other)
     const int i = lane + j * PN2_WAVE;
-    v[j] = i < a.V ? T::load(x + i) : -kHdInf;
+    v[j] = T::load(x + (i < a.V ? i : a.V - 1));
+  }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    v[j] = lane + j * PN2_WAVE < a.V ? v[j] : -kHdInf;
     m = fmaxf(m, v[j]);
   }
   // the maximum is known before the sum: exact differences, no limits needed
@@ -260,37 +268,54 @@ __global__ __launch_bounds__(256) void lp_small_kernel(FwdArgs a) {
   if constexpr (MODE == MODE_DISTILL) {
     lp_finish_distill<T>(a, row, x, f, true);
   } else {
-    lp_finish_label<T>(a, row, x, f);
+    lp_finish_label(a, row, label, f);
     if (a.top) {
-      TopList l;
-      l.clear();
-      for (int q = 0; q < a.top; ++q) {
-        unsigned bk = 0u, bi = 0u;
+      // the k-th best of the 64 lanes' best keys bounds the k best elements from below; those at or above it are ranked by counting
+      __shared__ u64 sh_cand[4][EPL * PN2_WAVE];
+      const int w = threadIdx.x >> 6;
+      u64 best = 0u;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          const unsigned k = lp_key(v[j]);
-          const bool better = k > bk;
-          bk = better ? k : bk;
-          bi = better ? ~(unsigned)(lane + j * PN2_WAVE) : bi;
-        }
-        unsigned mk, mi;
-        pn2_wave_argmax_u32x2(bk, bi, mk, mi);
-        if (mk <= kKeyNegInf) break;
-        const int at = (int)~mi;
-        if (lane == q) { l.key = mk; l.idx = at; }
-#pragma unroll
-        for (int j = 0; j < EPL; ++j)
-          if (at == lane + j * PN2_WAVE) v[j] = -kHdInf;
+      for (int j = 0; j < EPL; ++j) {
+        const unsigned k = lp_key(v[j]);
+        const u64 key = k <= kKeyNegInf ? 0u : ((u64)k << 32) | (unsigned)~(lane + j * PN2_WAVE);
+        best = key > best ? key : best;
       }
-      lp_write_top(a, row, l, f);
+      const int rank = lp_rank64(best, a.V);
+      if (lane < a.top) {                              // slots that no entry will take
+        a.top_lp[row * a.top + lane] = f.nan ? __builtin_nanf("") : -kHdInf;
+        a.top_idx[row * a.top + lane] = -1;
+      }
+      if (f.nan) return;
+      if constexpr (EPL == 1) {                        // the lanes' keys are the elements
+        if (best != 0u && rank < a.top) {
+          a.top_lp[row * a.top + rank] = lp_logp(v[0], f);
+          a.top_idx[row * a.top + rank] = lane;
+        }
+        return;
+      }
+      const u64 hit = __ballot(rank == a.top - 1 && best != 0u);
+      const u64 low = hit ? pn2_readlane_u64(best, __ffsll((unsigned long long)hit) - 1) : (u64)(kKeyNegInf + 1) << 32;
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        const unsigned k = lp_key(v[j]);
+        const u64 key = ((u64)k << 32) | (unsigned)~(lane + j * PN2_WAVE);
+        const u64 mask = __ballot(key >= low);
+        if (key >= low) sh_cand[w][n + pn2_prefix_popc(mask)] = key;
+        n += __popcll(mask);
+      }
+      __builtin_amdgcn_wave_barrier();                 // (LDS operations of a wave are in order)
+      for (int e = lane; e < n; e += PN2_WAVE) lp_place(a, row, sh_cand[w], n, sh_cand[w][e], f);
     }
   }
 }
 
-// --------------------------------------------------------------------------------------------- V > 1024: a workgroup per row
-template <class T, int MODE, bool TOP, int BT>
+// --------------------------------------------------------------------------------------------- V > 2048: a workgroup per row
+constexpr int kCand = 1024;              // elements kept in LDS for the final ranking
+
+template <class T, int MODE, bool TOP, int BT, int U>
 __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
-  constexpr int VE = T::kPerVec, U = 4, W = BT / PN2_WAVE;
+  constexpr int VE = T::kPerVec, W = BT / PN2_WAVE;
   constexpr bool ENT = MODE == MODE_LABEL;
   typedef typename T::elem elem;
   __shared__ float sh_m[W], sh_s[W], sh_se[W];
@@ -304,15 +329,49 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
       return;
     }
   }
+  Label label{};
+  if constexpr (MODE == MODE_LABEL) {
+    if (wave == W - 1) label = lp_label<T>(a, row, x);
+  }
   const float c = a.c, lim = lp_lim(c);
   r.M2 = lp_ref(r.m, c, lim);
-  const int nfull = a.V / VE, tail = a.V % VE;
+  const int nfull = a.V / VE, tail = a.V % VE, nvec = nfull + (tail != 0);
   int ord = 0x7fffffff;                                // first vector that holds the thread's maximum
-  int b = 0;
-  for (; b + BT * U <= nfull; b += BT * U) {
-    hd_u32x4 w[U];
+  // the row's last, partial vector, filled up with nothing (-inf)
+  auto last_vector = [&]() -> hd_u32x4 {
+    float g[VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = hd_load16<T>(x + (long long)(b + u * BT + tid) * VE);
+    for (int j = 0; j < VE; ++j) g[j] = j < tail ? T::load(x + (long long)nfull * VE + j) : -kHdInf;
+    return T::pack(g);
+  };
+  hd_u32x4 nothing;
+  {
+    float g[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) g[j] = -kHdInf;
+    nothing = T::pack(g);
+  }
+  // vector i of the row; behind the row's end: nothing.  (A load at a clamped place and a choice: no branch in front of the loads.)
+  auto whole = [&](int i) -> hd_u32x4 {
+    const hd_u32x4 w = hd_load16<T>(x + (long long)(i < nfull ? i : nfull - 1) * VE);
+    return i < nfull ? w : nothing;
+  };
+  auto fetch = [&](int i) -> hd_u32x4 {
+    hd_u32x4 w = whole(i);
+    if (tail && i == nfull) w = last_vector();
+    return w;
+  };
+  hd_u32x4 behind = nothing;
+  if (tail && tid == nfull % BT) behind = last_vector();
+  for (int b = 0; b < nfull; b += BT * U) {
+    hd_u32x4 w[U];
+    if (b + BT * U <= nfull) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = hd_load16<T>(x + (long long)(b + u * BT + tid) * VE);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = whole(b + u * BT + tid);
+    }
     float f[U * VE];
     float bm = -kHdInf;
     float best = r.m;
@@ -330,21 +389,16 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
     }
     lp_add<ENT>(r, f, bm, c, lim);
   }
-  for (int i = b + tid; i < nfull + (tail != 0); i += BT) {
-    float g[VE];
-    if (i < nfull) {
-      T::unpack(hd_load16<T>(x + (long long)i * VE), g);
-    } else {
+  if (tail) {
+    float f[VE];
+    T::unpack(behind, f);
+    float vm = f[0];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) g[j] = j < tail ? T::load(x + (long long)i * VE + j) : -kHdInf;
-    }
-    float vm = g[0];
-#pragma unroll
-    for (int j = 1; j < VE; ++j) vm = fmaxf(vm, g[j]);
+    for (int i = 1; i < VE; ++i) vm = fmaxf(vm, f[i]);
     if constexpr (TOP) {
-      if (vm > r.m) ord = i;
+      if (vm > r.m) ord = nfull;
     }
-    lp_add<ENT>(r, g, vm, c, lim);
+    lp_add<ENT>(r, f, vm, c, lim);
   }
   const float own = r.m;
   // the row's sums, in a fixed order
@@ -388,100 +442,97 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
     if (wave == 0) lp_finish_distill<T>(a, row, x, st, true);
     return;
   }
-  if (wave == W - 1) lp_finish_label<T>(a, row, x, st);
+  if (wave == W - 1) lp_finish_label(a, row, label, st);
   if constexpr (TOP) {
-    __shared__ unsigned sh_key[BT];
-    __shared__ int sh_ord[BT];
-    __shared__ int sh_win[kMaxTop];
-    __shared__ int sh_nwin;
-    __shared__ unsigned sh_lkey[W][kMaxTop];
-    __shared__ int sh_lidx[W][kMaxTop];
-    const unsigned okey = own == -kHdInf ? 0u : lp_key(own);
-    sh_key[tid] = okey;
-    sh_ord[tid] = ord;
-    __syncthreads();
-    if (wave == 0) {
-      // the `top` best of the threads' keys: W keys per lane, one wave-wide arg-max per winner
-      constexpr int R = W;
-      unsigned key[R], inv[R];
-#pragma unroll
-      for (int q = 0; q < R; ++q) {
-        key[q] = sh_key[q * PN2_WAVE + lane];
-        inv[q] = ~(unsigned)sh_ord[q * PN2_WAVE + lane];
-      }
-      int n = 0;
-      for (; n < a.top; ++n) {
-        unsigned bk = 0u, bi = 0u;
-        int bq = 0;
-#pragma unroll
-        for (int q = 0; q < R; ++q) {
-          const bool better = key[q] > bk || (key[q] == bk && inv[q] > bi);
-          bk = better ? key[q] : bk;
-          bi = better ? inv[q] : bi;
-          bq = better ? q : bq;
-        }
-        unsigned mk, mi;
-        const u64 who = pn2_wave_argmax_u32x2(bk, bi, mk, mi);
-        if (mk == 0u) break;
-        if (lane == __ffsll((unsigned long long)who) - 1) {
-          sh_win[n] = bq * PN2_WAVE + lane;
-#pragma unroll
-          for (int q = 0; q < R; ++q)
-            if (q == bq) key[q] = 0u;
-        }
-      }
-      if (lane == 0) sh_nwin = n;
+    __shared__ u64 sh_group[64], sh_low;
+    __shared__ int sh_win[BT], sh_count[2];            // winners, candidates
+    __shared__ u64 sh_cand[kCand + 1], sh_best[W];
+    // keys as one number: value above, vector (or element) below, earlier ones larger
+    const u64 mine = own == -kHdInf ? 0u : ((u64)lp_key(own) << 32) | (unsigned)~ord;
+    // the best key of each of 64 groups of neighbouring threads; the k-th best of them bounds the k best elements from below
+    u64 g = mine;
+    {
+      u64 o = pn2_dpp_u64<PN2_DPP_QUAD_XOR1>(g);
+      g = o > g ? o : g;
+      o = pn2_dpp_u64<PN2_DPP_QUAD_XOR2>(g);
+      g = o > g ? o : g;
+      if constexpr (BT >= 512) { o = pn2_dpp_u64<PN2_DPP_ROW_HALF_MIRROR>(g); g = o > g ? o : g; }
+      if constexpr (BT >= 1024) { o = pn2_dpp_u64<PN2_DPP_ROW_MIRROR>(g); g = o > g ? o : g; }
+    }
+    if (tid % (BT / 64) == 0) sh_group[tid / (BT / 64)] = g;
+    if (tid < 2) sh_count[tid] = 0;
+    if (tid < a.top) {                                 // slots that no entry will take
+      a.top_lp[row * a.top + tid] = st.nan ? __builtin_nanf("") : -kHdInf;
+      a.top_idx[row * a.top + tid] = -1;
     }
     __syncthreads();
-    const int nwin = sh_nwin;
-    // the k-th key bounds the elements from below (fewer winners than `top`: everything counts)
-    const int last = nwin == a.top ? sh_win[nwin - 1] : -1;
-    const unsigned low_key = last >= 0 ? sh_key[last] : kKeyNegInf + 1;
-    const int low_ord = last >= 0 ? sh_ord[last] : 0x7fffffff;
-    TopList l;
-    l.clear();
-    const int nvec = nfull + (tail != 0);
+    if (st.nan) return;                                // uniform over the workgroup
+    if (wave == 0) {
+      const u64 k = sh_group[lane];
+      const int rank = lp_rank64(k, 64);               // (keys of non-empty groups differ: their vectors do)
+      const u64 hit = __ballot(rank == a.top - 1 && k != 0u);
+      const u64 low = hit ? pn2_readlane_u64(k, __ffsll((unsigned long long)hit) - 1) : (u64)(kKeyNegInf + 1) << 32;
+      if (lane == 0) sh_low = low;
+    }
+    __syncthreads();
+    const u64 low = sh_low;
+    if (mine >= low && mine != 0u) sh_win[atomicAdd(&sh_count[0], 1)] = tid;     // (any order: the ranking below is total)
+    __syncthreads();
+    const int nwin = sh_count[0];
+    // (one share at a time: a single row's time is this code's trip through the instruction cache, 15.1 us against 16.5 us unrolled)
     for (int w = wave; w < nwin; w += W) {
-      const int t = sh_win[w];
-      for (int s0 = t; s0 < nvec; s0 += BT * PN2_WAVE) {           // the share of thread t, a vector per lane
-        const int i = s0 + lane * BT;
-        float g[VE];
-        if (i < nfull) {
-          T::unpack(hd_load16<T>(x + (long long)i * VE), g);
-        } else {
-#pragma unroll
-          for (int j = 0; j < VE; ++j) g[j] = i == nfull && j < tail ? T::load(x + (long long)i * VE + j) : -kHdInf;
-        }
+      for (int i = sh_win[w] + lane * BT; __builtin_amdgcn_readfirstlane(i) < nvec; i += BT * PN2_WAVE) {   // its vectors, one per lane
+        float f[VE];
+        T::unpack(fetch(i), f);
+        unsigned k[VE], hits = 0u;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          const unsigned k = lp_key(g[j]);
-          bool cand = k > low_key || (k == low_key && i <= low_ord);
-          cand = cand && i < nvec && k > kKeyNegInf && g[j] == g[j];
-          u64 todo = __ballot(cand);
-          while (todo) {
-            const int src = __ffsll((unsigned long long)todo) - 1;
-            todo &= todo - 1;
-            l.insert((unsigned)__builtin_amdgcn_readlane((int)k, src), __builtin_amdgcn_readlane(i, src) * VE + j);
+          k[j] = lp_key(f[j]);
+          // (what lies behind the row's end reads as -inf, below any bound)
+          if ((((u64)k[j] << 32) | (unsigned)~i) >= low) hits |= 1u << j;
+        }
+        if (hits) {
+          const int at = atomicAdd(&sh_count[1], __popc(hits));
+#pragma unroll
+          for (int j = 0; j < VE; ++j) {               // (what is no candidate, or one too many, goes to a slot that nobody reads)
+            const int to = at + __popc(hits & ((1u << j) - 1u));
+            sh_cand[((hits >> j) & 1u) && to < kCand ? to : kCand] = ((u64)k[j] << 32) | (unsigned)~(i * VE + j);
           }
         }
       }
     }
-    sh_lkey[wave][lane] = l.key;
-    sh_lidx[wave][lane] = l.idx;
     __syncthreads();
-    if (wave == 0) {
-      for (int w = 1; w < W; ++w) {
-        const unsigned k = sh_lkey[w][lane];
-        const int i = sh_lidx[w][lane];
-        // (a list is sorted: its used entries are the first ones)
-        u64 todo = __ballot(k != 0u);
-        while (todo) {
-          const int src = __ffsll((unsigned long long)todo) - 1;
-          todo &= todo - 1;
-          l.insert((unsigned)__builtin_amdgcn_readlane((int)k, src), __builtin_amdgcn_readlane(i, src));
+    const int n = sh_count[1];
+    if (n <= kCand) {
+      for (int e = tid; e < n; e += BT) lp_place(a, row, sh_cand, n, sh_cand[e], st);
+      return;
+    }
+    // rows with very many equal entries at the bound: one pass over the row per alternative, each the best below the last
+    u64 last = ~(u64)0;
+    for (int q = 0; q < a.top; ++q) {
+      u64 best = 0u;
+      for (int i = tid; i < nvec; i += BT) {
+        float f[VE];
+        T::unpack(fetch(i), f);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const unsigned k = lp_key(f[j]);
+          const u64 key = ((u64)k << 32) | (unsigned)~(i * VE + j);
+          if (k > kKeyNegInf && key < last && key > best) best = key;
         }
       }
-      lp_write_top(a, row, l, st);
+      best = pn2_wave_max_u64(best);
+      if (lane == 0) sh_best[wave] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) best = sh_best[w] > best ? sh_best[w] : best;
+      __syncthreads();
+      if (best == 0u) break;                           // uniform over the workgroup
+      if (tid == 0) {
+        a.top_lp[row * a.top + q] = lp_logp(lp_unkey((unsigned)(best >> 32)), st);
+        a.top_idx[row * a.top + q] = (int)~(unsigned)best;
+      }
+      last = best;
     }
   }
 }
@@ -508,6 +559,8 @@ __device__ __forceinline__ float lp_teacher(const BwdArgs &a, long long at) {
   return (float)((const _Float16 *)a.t_val)[at];
 }
 
+constexpr int kTeacher = 256;            // a teacher's indices kept in LDS; further ones are read again
+
 // GROUP threads own a segment of one row.  Bound by its bytes (V read, V written); ~6 vector instructions per element.
 template <class T, int MODE, int GROUP>
 __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
@@ -515,9 +568,10 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
   typedef typename T::elem elem;
   const int tid = threadIdx.x % GROUP;
   const long long unit = GROUP == 256 ? (long long)blockIdx.x : (long long)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
-  const long long row = unit / a.nseg;
-  if (row >= a.T) return;                              // (GROUP < 256 only: no barrier below is left behind)
-  const int seg = (int)(unit - row * a.nseg);
+  const long long nth = unit / a.nseg;
+  if (nth >= a.T) return;                              // (GROUP < 256 only: no barrier below is left behind)
+  const long long row = a.T - 1 - nth;                 // the rows the forward pass read last may still be in the cache
+  const int seg = (int)(unit - nth * a.nseg);
   const elem *x = (const elem *)a.logits + row * a.ld;
   elem *dx = (elem *)a.dlogits + row * (long long)a.V;
   const int nfull = a.V / VE, tail = a.V % VE, nvec = nfull + (tail != 0);
@@ -597,22 +651,50 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
   }
   if constexpr (MODE == MODE_DISTILL) {
     // the teacher's entries of this segment again, whole: an index that occurs more than once takes the sum of its q
-    if constexpr (GROUP == 256) __syncthreads();       // after the stores above (one wave: program order)
+    __shared__ int sh_i[256 / GROUP][kTeacher];
+    const int own = GROUP == 256 ? 0 : threadIdx.x / GROUP;
     const float tm = a.stats[4 * row + 2], tls2 = a.stats[4 * row + 3];
     const long long at = row * a.k, e0 = (long long)v0 * VE, e1 = (long long)v1 * VE < a.V ? (long long)v1 * VE : a.V;
-    for (int j = tid; j < a.k; j += GROUP) {
+    const int kept = a.k < kTeacher ? a.k : kTeacher;
+    for (int j = tid; j < kept; j += GROUP) {
       const long long i = a.t_idx[at + j];
-      if (i < e0 || i >= e1) continue;
-      bool first = true;
-      for (int n = 0; n < j && first; ++n) first = a.t_idx[at + n] != i;
-      if (!first) continue;
+      sh_i[own][j] = i >= e0 && i < e1 ? (int)i : -1;
+    }
+    // (also after the stores above; one wave: program order)
+    if constexpr (GROUP == 256) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+    auto index = [&](int j) -> int {
+      if (j < kTeacher) return sh_i[own][j];
+      const long long i = a.t_idx[at + j];
+      return i >= e0 && i < e1 ? (int)i : -1;
+    };
+    for (int j = tid; j < a.k; j += GROUP) {
+      const int i = index(j);
+      if (i < 0) continue;
       float q = 0.f;
-      for (int n = j; n < a.k; ++n)
-        if (a.t_idx[at + n] == i) q += hd_exp2((lp_teacher(a, at + n) - tm) * c - tls2);
+      bool first = true;
+      for (int n = 0; n < a.k; ++n) {
+        if (index(n) != i) continue;
+        if (n < j) { first = false; break; }
+        q += hd_exp2((lp_teacher(a, at + n) - tm) * c - tls2);
+      }
+      if (!first) continue;
       const float p = hd_exp2(__fmaf_rn(T::load(x + i) - m, c, -ls2));
       dx[i] = T::round((p - q) * A);
     }
   }
+}
+
+template <class T, int MODE, bool TOP>
+void lp_row_launch(const FwdArgs &a, hipStream_t st) {
+  // Fewer rows than CUs: one big workgroup per row with its loads on their way at once (1 x 131072 bf16 with 20 alternatives 15 us, 25
+  // with 512 threads).  Otherwise several workgroups per CU, smaller ones for short rows, whose time is the selection's round trips
+  // (8192 x 16384 bf16 with 20 alternatives: 95 us with 256 threads, 122 with 512; 8192 x 131072: 0.43 ms with 512).
+  const unsigned grid = (unsigned)a.T;
+  const int nvec = (a.V + T::kPerVec - 1) / T::kPerVec;
+  if (nvec > 1024 && a.T <= 256) lp_row_kernel<T, MODE, TOP, 1024, 8><<<grid, 1024, 0, st>>>(a);
+  else if (nvec <= 4096) lp_row_kernel<T, MODE, TOP, 256, 4><<<grid, 256, 0, st>>>(a);
+  else lp_row_kernel<T, MODE, TOP, 512, 4><<<grid, 512, 0, st>>>(a);
 }
 
 template <class T, int MODE>
@@ -621,12 +703,12 @@ int lp_forward(const FwdArgs &a, hipStream_t st) {
     const unsigned grid = (unsigned)((a.T + 3) / 4);
     if (a.V <= 64) lp_small_kernel<T, MODE, 1><<<grid, 256, 0, st>>>(a);
     else if (a.V <= 256) lp_small_kernel<T, MODE, 4><<<grid, 256, 0, st>>>(a);
-    else lp_small_kernel<T, MODE, 16><<<grid, 256, 0, st>>>(a);
+    else if (a.V <= 1024) lp_small_kernel<T, MODE, 16><<<grid, 256, 0, st>>>(a);
+    else lp_small_kernel<T, MODE, 32><<<grid, 256, 0, st>>>(a);
     return pn2_check_launch();
   }
-  const unsigned grid = (unsigned)a.T;
-  if (MODE == MODE_LABEL && a.top) lp_row_kernel<T, MODE, true, 512><<<grid, 512, 0, st>>>(a);
-  else lp_row_kernel<T, MODE, false, 512><<<grid, 512, 0, st>>>(a);
+  if (MODE == MODE_LABEL && a.top) lp_row_launch<T, MODE, true>(a, st);
+  else lp_row_launch<T, MODE, false>(a, st);
   return pn2_check_launch();
 }
 
