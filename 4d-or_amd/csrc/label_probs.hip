@@ -618,6 +618,20 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
     }
     return;                                            // uniform over the group
   }
+  // distill: the teacher's entries of this segment, read while the row is on its way
+  struct Teacher { int i; float q; };                  // i < 0: unused, or in another segment
+  __shared__ Teacher sh_t[MODE == MODE_DISTILL ? 256 / GROUP : 1][MODE == MODE_DISTILL ? kTeacher : 1];
+  const int own = GROUP == 256 ? 0 : threadIdx.x / GROUP, kept = a.k < kTeacher ? a.k : kTeacher;
+  const float tm = MODE == MODE_DISTILL ? a.stats[4 * row + 2] : 0.f, tls2 = MODE == MODE_DISTILL ? a.stats[4 * row + 3] : 0.f;
+  const long long e0 = (long long)v0 * VE, e1 = (long long)v1 * VE < a.V ? (long long)v1 * VE : a.V;
+  auto entry = [&](int j) -> Teacher {
+    const long long i = a.t_idx[row * a.k + j];
+    if (i < e0 || i >= e1) return Teacher{-1, 0.f};
+    return Teacher{(int)i, hd_exp2((lp_teacher(a, row * a.k + j) - tm) * c - tls2)};
+  };
+  if constexpr (MODE == MODE_DISTILL) {
+    for (int j = tid; j < kept; j += GROUP) sh_t[own][j] = entry(j);
+  }
   const int yv = y >= 0 ? (int)(y / VE) : -1, yj = y >= 0 ? (int)(y % VE) : 0;
   auto one = [&](int i, hd_u32x4 w) {
     float f[VE];
@@ -650,37 +664,29 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
     }
   }
   if constexpr (MODE == MODE_DISTILL) {
-    // the teacher's entries of this segment again, whole: an index that occurs more than once takes the sum of its q
-    __shared__ int sh_i[256 / GROUP][kTeacher];
-    const int own = GROUP == 256 ? 0 : threadIdx.x / GROUP;
-    const float tm = a.stats[4 * row + 2], tls2 = a.stats[4 * row + 3];
-    const long long at = row * a.k, e0 = (long long)v0 * VE, e1 = (long long)v1 * VE < a.V ? (long long)v1 * VE : a.V;
-    const int kept = a.k < kTeacher ? a.k : kTeacher;
-    for (int j = tid; j < kept; j += GROUP) {
-      const long long i = a.t_idx[at + j];
-      sh_i[own][j] = i >= e0 && i < e1 ? (int)i : -1;
-    }
+    // the teacher's entries of this segment again, whole: an index that occurs more than once takes the sum of its q.
     // (also after the stores above; one wave: program order)
     if constexpr (GROUP == 256) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
-    auto index = [&](int j) -> int {
-      if (j < kTeacher) return sh_i[own][j];
-      const long long i = a.t_idx[at + j];
-      return i >= e0 && i < e1 ? (int)i : -1;
-    };
     for (int j = tid; j < a.k; j += GROUP) {
-      const int i = index(j);
-      if (i < 0) continue;
+      const Teacher me = j < kTeacher ? sh_t[own][j] : entry(j);
+      if (me.i < 0) continue;
       float q = 0.f;
-      bool first = true;
-      for (int n = 0; n < a.k; ++n) {
-        if (index(n) != i) continue;
-        if (n < j) { first = false; break; }
-        q += hd_exp2((lp_teacher(a, at + n) - tm) * c - tls2);
+      int before = 0;
+#pragma unroll 8
+      for (int n = 0; n < kept; ++n) {
+        const Teacher o = sh_t[own][n];
+        q += o.i == me.i ? o.q : 0.f;
+        before |= o.i == me.i && n < j ? 1 : 0;
       }
-      if (!first) continue;
-      const float p = hd_exp2(__fmaf_rn(T::load(x + i) - m, c, -ls2));
-      dx[i] = T::round((p - q) * A);
+      for (int n = kept; n < a.k; ++n) {
+        const Teacher o = entry(n);
+        q += o.i == me.i ? o.q : 0.f;
+        before |= o.i == me.i && n < j ? 1 : 0;
+      }
+      if (before) continue;
+      const float p = hd_exp2(__fmaf_rn(T::load(x + me.i) - m, c, -ls2));
+      dx[me.i] = T::round((p - q) * A);
     }
   }
 }
