@@ -519,21 +519,28 @@ __global__ __launch_bounds__(256) void la_join_kernel(Product a) {
 }
 
 // rows x cols at row stride ld -> rows at row stride `to` (a multiple of 16 bytes), the columns behind `cols` zero
+struct Copy {
+  long long rows, cols, ld, to;
+  const void *src;
+  void *dst;
+};
+// both operands of a product in one launch: the first `first` workgroups copy a, the others b
 template <class T>
-__global__ __launch_bounds__(256) void la_pad_kernel(long long rows, long long cols, const void *src_, long long ld, void *dst_, long long to) {
+__global__ __launch_bounds__(256) void la_pad_kernel(Copy a, Copy b, unsigned first) {
   typedef typename T::elem elem;
   constexpr int VE = T::kPerVec;
-  const long long pieces = to / VE, at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= rows * pieces) return;
+  const Copy &o = blockIdx.x < first ? a : b;
+  const long long pieces = o.to / VE, at = (long long)(blockIdx.x < first ? blockIdx.x : blockIdx.x - first) * 256 + threadIdx.x;
+  if (at >= o.rows * pieces) return;
   const long long r = at / pieces, c = (at - r * pieces) * VE;
-  const elem *src = (const elem *)src_ + r * ld + c;
+  const elem *src = (const elem *)o.src + r * o.ld + c;
   float f[VE];
-  if (c + VE <= cols) {
-    hd_store16<T>((elem *)dst_ + r * to + c, hd_load16<T>(src));
+  if (c + VE <= o.cols) {
+    hd_store16<T>((elem *)o.dst + r * o.to + c, hd_load16<T>(src));
   } else {
 #pragma unroll
-    for (int n = 0; n < VE; ++n) f[n] = c + n < cols ? T::load(src + n) : 0.f;
-    hd_store16<T>((elem *)dst_ + r * to + c, T::pack(f));
+    for (int n = 0; n < VE; ++n) f[n] = c + n < o.cols ? T::load(src + n) : 0.f;
+    hd_store16<T>((elem *)o.dst + r * o.to + c, T::pack(f));
   }
 }
 
@@ -886,16 +893,23 @@ struct Space {              // the caller's workspace, handed out piece by piece
   }
 };
 
+// those of a and b that need it become padded copies (b may be NULL)
 template <class T>
-void la_pad(Matrix &o, int dtype, Space &ws, hipStream_t st) {
-  const size_t n = la_copy_bytes(o, dtype);
-  if (!n) return;
-  void *to = ws.take(n);
-  const long long ld = la_whole(o.cols, dtype);
-  la_pad_kernel<T><<<(unsigned)la_div(o.rows * (ld / T::kPerVec), 256), 256, 0, st>>>(o.rows, o.cols, o.p, o.ld, to, ld);
-  o.p = to;
-  o.ld = ld;
-  if (o.R) o.cols = ld;
+void la_pad(Matrix *a, Matrix *b, int dtype, Space &ws, hipStream_t st) {
+  Copy job[2] = {};
+  unsigned blocks[2] = {0, 0};
+  for (int n = 0; n < 2; ++n) {
+    Matrix *o = n ? b : a;
+    const size_t bytes = o ? la_copy_bytes(*o, dtype) : 0;
+    if (!bytes) continue;
+    const long long to = la_whole(o->cols, dtype);
+    job[n] = {o->rows, o->cols, o->ld, to, o->p, ws.take(bytes)};
+    blocks[n] = (unsigned)la_div(o->rows * (to / T::kPerVec), 256);
+    o->p = job[n].dst;
+    o->ld = to;
+    if (o->R) o->cols = to;
+  }
+  if (blocks[0] + blocks[1]) la_pad_kernel<T><<<blocks[0] + blocks[1], 256, 0, st>>>(job[0], job[1], blocks[0]);
 }
 
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
@@ -975,8 +989,7 @@ template <class T>
 int la_forward(Forward f, long long M, long long N, long long K, int dtype, const Epilogue &e, void *ws, hipStream_t st) {
   Space space{(char *)ws};
   if (f.plan.kernel >= TILE_64) {
-    la_pad<T>(f.x, dtype, space, st);
-    la_pad<T>(f.w, dtype, space, st);
+    la_pad<T>(&f.x, &f.w, dtype, space, st);
   }
   return la_product<T, false, false>(f.plan, f.x, f.w, M, N, K, e, space, st);
 }
@@ -996,7 +1009,7 @@ struct Backward {
   bool small, own_dz;       // own_dz: dz is written (it is not dy itself)
   Plan px, pw;
   Matrix dz, dzr, w, x;   // dz as the K operand of dx and as the R operand of dW
-  size_t dz_bytes, part, copies, partial, bytes;
+  size_t dz_bytes, part, bytes;
 };
 Backward la_backward_plan(long long M, long long N, long long K, int dtype, const void *dy, long long ldy, bool slope, const void *x,
                           long long ldx, const void *w, long long ldw, int want) {
@@ -1013,10 +1026,10 @@ Backward la_backward_plan(long long M, long long N, long long K, int dtype, cons
   b.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
   b.px = la_plan(M, K, N, dtype, false);
   b.pw = la_plan(N, K, M, dtype, false);
+  const size_t copies = ((want & 1) ? la_copy_bytes(b.w, dtype) : 0) + ((want & 2) ? la_copy_bytes(b.x, dtype) : 0);
   // the two products use the rest one after the other
-  const size_t dx = (want & 1) ? la_copy_bytes(b.w, dtype) + la_partial_bytes(b.px, M, K) : 0;
-  const size_t dw = (want & 2) ? la_copy_bytes(b.x, dtype) + la_partial_bytes(b.pw, N, K) : 0;
-  b.bytes = b.dz_bytes + b.part + (dx > dw ? dx : dw);
+  const size_t dx = (want & 1) ? la_partial_bytes(b.px, M, K) : 0, dw = (want & 2) ? la_partial_bytes(b.pw, N, K) : 0;
+  b.bytes = b.dz_bytes + b.part + copies + (dx > dw ? dx : dw);
   return b;
 }
 
@@ -1049,19 +1062,16 @@ int la_backward(Backward b, long long M, long long N, long long K, int dtype, co
     b.dz.p = b.dzr.p = dz;
     b.dz.ld = b.dzr.ld = b.dzr.cols = ldz;
   }
+  la_pad<T>(dx ? &b.w : nullptr, dw ? &b.x : nullptr, dtype, space, st);
   Epilogue e{};
   if (dx) {
-    Space rest = space;
-    la_pad<T>(b.w, dtype, rest, st);
     e.y = dx;
-    const int rc = la_product<T, false, true>(b.px, b.dz, b.w, M, K, N, e, rest, st);
+    const int rc = la_product<T, false, true>(b.px, b.dz, b.w, M, K, N, e, space, st);
     if (rc != PN2_OK) return rc;
   }
   if (dw) {
-    Space rest = space;
-    la_pad<T>(b.x, dtype, rest, st);
     e.y = dw;
-    return la_product<T, true, true>(b.pw, b.dzr, b.x, N, K, M, e, rest, st);
+    return la_product<T, true, true>(b.pw, b.dzr, b.x, N, K, M, e, space, st);
   }
   return PN2_OK;
 }
