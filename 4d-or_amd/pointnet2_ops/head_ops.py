@@ -25,6 +25,15 @@ ACTIVATIONS = tuple(_ext.ACTIVATIONS)
 LabelLogProbs = collections.namedtuple("LabelLogProbs", "log_prob entropy top_log_prob top_index")
 
 
+def _once(backward):
+    """once_differentiable, without its price where no graph of the backward pass is being built."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _matrix(t, name):
     """(..., C) -> (rows, C) with a contiguous last axis; a copy only where the strides allow no view."""
     if not isinstance(t, torch.Tensor) or t.dim() < 1:
@@ -44,7 +53,7 @@ class _LinearAct(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         need_dx, need_dw, need_db, need_dr, _ = ctx.needs_input_grad
         dx = dw = db = None
@@ -92,7 +101,7 @@ class _LabelLogProbs(Function):
         return lp, ent, tlp, tix
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g_lp, g_ent, _tlp, _tix):
         if g_lp is None and g_ent is None:
             return None, None, None, None
@@ -138,7 +147,7 @@ class _DistillTopK(Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         logits, index, values, stats = ctx.saved_tensors
         return _ext.distill_topk_grad(logits, index, values, ctx.temperature, stats, g.contiguous()), None, None, None

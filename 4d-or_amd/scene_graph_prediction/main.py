@@ -172,6 +172,9 @@ def main(argv=None):
     ap.add_argument("--objects", type=int, default=9)
     ap.add_argument("--weights", type=str, default=None, help="state_dict (.pth) of the reference model")
     ap.add_argument("--out", type=str, default="scan_relations_synthetic.json")
+    ap.add_argument("--alternatives", type=int, default=0,
+                    help="infer: also write the K best predicates of every edge with their log probabilities and the edge's entropy, "
+                         "to <out>.alternatives.json (GPU)")
     ap.add_argument("--cache-dir", type=str, default=None,
                     help="evaluate: folder of the reference's prepared samples ({scan_id}.npz, or_dataset.py:94-120), e.g. "
                          "datasets/4D-OR/scene_graph_cache_no_gt")
@@ -230,11 +233,17 @@ def main(argv=None):
             total = sum(float(model.validation_step(to_device(s, device), i)) for i, s in enumerate(scans))
         print(json.dumps({k: v for k, v in model.evaluate_predictions(total, "val").items() if k != "per_take"}))
         return
-    results = {}
+    results, alternatives = {}, {}
     with torch.no_grad():
         for i, scan in enumerate(scans):
-            scan_id, rels = model.predict_step(to_device(scan, device), i)
+            batch = to_device(scan, device)
+            scan_id, rels = model.predict_step(batch, i)
             results[scan_id] = rels
+            if args.alternatives > 0:
+                alternatives[scan_id] = model.predict_alternatives(batch, args.alternatives)[1]
+    if args.alternatives > 0:
+        with open(args.out + ".alternatives.json", "w") as f:
+            json.dump(alternatives, f)
     with open(args.out, "w") as f:                            # same wire format as main.py:111-115
         json.dump(results, f)
     print(f"wrote {args.out}: {sum(len(v) for v in results.values())} triples for {len(results)} scans")

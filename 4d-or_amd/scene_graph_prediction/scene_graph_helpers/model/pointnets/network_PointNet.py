@@ -4,6 +4,8 @@ rocBLAS through torch — SURVEY.md §8 A14).  Mirrors ``PointNetCls``
 (:227-271): 256 -> 512 -> 256 (dropout 0.3 before the optional BN) -> k,
 log-softmax; the relation head late-fuses the image embedding and the
 subject/object one-hot before ``fc3``."""
+import os
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -45,11 +47,22 @@ def scan_batch_norm(bn: nn.BatchNorm1d, x, ptr):
 
 
 class _Head(BaseNetwork):
+    #: heads without BatchNorm on the GPU: Linear + bias + ReLU of the trunk as one kernel each, forward and (layers of this size) the
+    #: whole backward pass (pointnet2_ops/head_ops.py linear_act) instead of torch's library product and elementwise kernels.  Same
+    #: fp32 mathematics, another order of sums.  Off by default: results stay bit for bit what they were.
+    fused_linear = os.environ.get("PN2_FUSED_HEADS", "0") == "1"
+
     def _make_trunk(self, in_size, batch_norm, drop_out):
         self.fc1 = nn.Linear(in_size, 512)
         self.fc2 = nn.Linear(512, 256)
 
     def _trunk(self, x, use_bn, scan_ptr=None):
+        if self.fused_linear and x.is_cuda and not use_bn:
+            from pointnet2_ops.head_ops import linear_act
+            x = linear_act(x, self.fc1.weight, self.fc1.bias, "relu")
+            if not (self.use_drop_out and self.training):          # dropout sits between fc2 and its ReLU
+                return linear_act(x, self.fc2.weight, self.fc2.bias, "relu")
+            return self.relu(self.dropout(linear_act(x, self.fc2.weight, self.fc2.bias)))
         x = self.fc1(x)
         if use_bn:
             x = scan_batch_norm(self.bn1, x, scan_ptr)

@@ -229,7 +229,28 @@ class SGPNModelWrapper(nn.Module):
         else:
             loss_obj = F.nll_loss(obj_pred, batch["gt_class"], weight=w_obj)
             loss_rel = F.nll_loss(rel_pred, batch["gt_rels"], weight=w_rel)
-        return self.mconfig["lambda_o"] * loss_obj + loss_rel
+        total = self.mconfig["lambda_o"] * loss_obj + loss_rel
+        teacher = batch.get("teacher_rels")
+        if teacher is not None:                                     # another model's best predicates (teacher_relations below)
+            from pointnet2_ops.head_ops import distill_top_k
+            t = float(self.mconfig.get("distill_temperature", 1.0))
+            total = total + float(self.mconfig.get("lambda_distill", 1.0)) * distill_top_k(rel_pred, teacher[0], teacher[1], t).mean()
+        return total
+
+    @torch.no_grad()
+    def relation_alternatives(self, rel_pred, top, labels=None):
+        """The `top` best predicates of every edge with their log probabilities, the entropy of the edge's distribution and the log
+        probability of `labels` (default: the best predicate) -> pointnet2_ops.head_ops.LabelLogProbs, on the device."""
+        from pointnet2_ops.head_ops import label_log_probs
+        rel_pred = rel_pred.detach()
+        return label_log_probs(rel_pred, rel_pred.argmax(1) if labels is None else labels, top=min(int(top), rel_pred.size(1)))
+
+    @torch.no_grad()
+    def teacher_relations(self, batch, top=5):
+        """(index (edges, top), log probability (edges, top)) of this model's best predicates: what a student's batch carries as
+        "teacher_rels" — e.g. a model with images (no_gt_image) teaching one without (no_gt)."""
+        r = self.relation_alternatives(self(batch)[1], top)
+        return r.top_index, r.top_log_prob
 
     def _step(self, batch, split):
         obj_pred, rel_pred, *_ = self(batch, return_meta_data=True)
@@ -242,6 +263,18 @@ class SGPNModelWrapper(nn.Module):
 
     def validation_step(self, batch, batch_idx=0):
         return self._step(batch, "val")
+
+    def predict_alternatives(self, batch, top=3):
+        """-> (scan_id, [(subject_name, object_name, entropy, [(predicate, log probability), ...]), ...]) for EVERY edge of one scan,
+        best predicate first: the answer of predict_step with what else the model held possible."""
+        if batch.get("scenes") is not None:
+            raise ValueError("predict_alternatives takes one scan at a time")
+        r = self.relation_alternatives(self(batch)[1], top)
+        edges = batch["edge_indices"].transpose(0, 1).cpu().tolist()
+        objs, out = batch["objs_json"], []
+        for (start, end), h, names, lps in zip(edges, r.entropy.cpu().tolist(), r.top_index.cpu().tolist(), r.top_log_prob.cpu().tolist()):
+            out.append((objs[start + 1], objs[end + 1], h, [(self.relationNames[n], lp) for n, lp in zip(names, lps) if n >= 0]))
+        return batch["scan_id"], out
 
     def predict_step(self, batch, batch_idx=0, dataloader_idx=0):
         """-> (scan_id, [(subject_name, predicate, object_name), ...]); 'none' edges dropped."""

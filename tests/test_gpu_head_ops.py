@@ -612,3 +612,65 @@ def test_rows_past_two_to_the_32_elements():
     check(r.log_prob[rows.cuda()], *want["log_prob"])
     assert torch.equal(r.top_index[rows.cuda()].cpu(), want["top_index"])
     assert float((r.entropy[1:1000] - math.log(V)).abs().max()) < 1e-5
+
+
+# ------------------------------------------------------------------------------------------------- the model's own paths
+@pytest.mark.parametrize("train", [False, True])
+def test_fused_heads_equal_the_library_heads(train, monkeypatch):
+    """Both classification heads with the trunk's layers as linear_act: outputs and gradients of the library route within fp32
+    rounding of a 512-term product per layer (three layers, gradients relative to their largest entry)."""
+    from scene_graph_prediction.scene_graph_helpers.model.pointnets import network_PointNet as npn
+    torch.manual_seed(0)
+    obj = npn.PointNetCls(12, in_size=256, batch_norm=False, drop_out=True).cuda().train(train)
+    rel = npn.PointNetRelCls(15, in_size=256, batch_norm=False, drop_out=True, n_object_types=6).cuda().train(train)
+    x, e, hot = torch.randn(9, 256).cuda(), torch.randn(72, 256).cuda(), torch.zeros(72, 12).cuda()
+    hot[torch.arange(72), torch.arange(72) % 12] = 1
+
+    def run(fused):
+        monkeypatch.setattr(npn._Head, "fused_linear", fused)
+        torch.manual_seed(5)                                        # the same dropout masks
+        xs, es = x.clone().requires_grad_(), e.clone().requires_grad_()
+        a, b = obj(xs), rel(es, relation_objects_one_hot=hot)
+        params = [*obj.parameters(), *rel.parameters()]
+        return [a, b], torch.autograd.grad(a[:, 3].sum() + b[:, 5].sum(), [xs, es, *params])
+    out, grads = run(False)
+    out2, grads2 = run(True)
+    for a, b in zip(out, out2):
+        torch.testing.assert_close(a, b, atol=3 * 512 * U * float(a.abs().max()), rtol=0)
+    for a, b in zip(grads, grads2):
+        torch.testing.assert_close(a, b, atol=3 * 512 * U * float(a.abs().max()), rtol=0)
+
+
+def test_model_alternatives_and_learning_from_a_teacher(tmp_path):
+    import json
+    from scene_graph_prediction import main as runner
+    out = tmp_path / "rels.json"
+    runner.main(["--mode", "infer", "--scans", "1", "--objects", "4", "--out", str(out), "--alternatives", "3"])
+    rels = json.load(open(out))
+    more = json.load(open(str(out) + ".alternatives.json"))
+    assert rels.keys() == more.keys()
+    (scan, edges), = more.items()
+    assert len(edges) == 12
+    best = {(a, b): alt for a, b, _, alt in edges}
+    for a, b, entropy, alt in edges:
+        assert len(alt) == 3 and 0 <= entropy <= math.log(15) + 1e-5
+        assert all(p >= q for (_, p), (_, q) in zip(alt, alt[1:])) and sum(math.exp(p) for _, p in alt) <= 1 + 1e-5
+    for sub, pred, ob in rels[scan]:
+        assert best[(sub, ob)][0][0] == pred                        # the best alternative is predict_step's answer
+    # a student's loss with a teacher's alternatives in its batch
+    config = runner.config_loader("no_gt.json")
+    torch.manual_seed(1)
+    model = runner.SGPNModelWrapper(config, 12, 15, torch.ones(12), torch.ones(15), runner.RELATION_NAMES).cuda()
+    gen = torch.Generator().manual_seed(2)
+    rel_pred = torch.log_softmax(rnd(gen, 20, 15), 1).requires_grad_()
+    obj_pred = torch.log_softmax(rnd(gen, 5, 12), 1)
+    teacher = model.relation_alternatives(rnd(gen, 20, 15, scale=2.0), 5)
+    batch = dict(gt_class=torch.zeros(5, dtype=torch.int64).cuda(), gt_rels=torch.zeros(20, dtype=torch.int64).cuda())
+    plain = model.loss(obj_pred, rel_pred, batch)
+    taught = model.loss(obj_pred, rel_pred, dict(batch, teacher_rels=(teacher.top_index, teacher.top_log_prob)))
+    q = torch.softmax(teacher.top_log_prob.double(), 1)
+    want = (q * (q.log() - torch.log_softmax(rel_pred.double(), 1).gather(1, teacher.top_index))).sum(1).mean()
+    assert abs(float(taught - plain) - float(want)) <= 64 * U * (abs(float(want)) + abs(float(taught)))
+    g, = torch.autograd.grad(taught - plain, rel_pred)
+    wg, = torch.autograd.grad(want, rel_pred)
+    torch.testing.assert_close(g.double(), wg.double(), atol=64 * U, rtol=64 * U)
