@@ -8,7 +8,8 @@
 // matrix cores (v_mfma_f32_16x16x32 for 16-bit types, v_mfma_f32_16x16x4_f32 for fp32); bias, activation, slope and residual are
 // fp32 in the epilogue; each output is rounded once.  The SLOPE is what is stored, not z: rounding d costs every dz a relative
 // half-step, rounding z would cost an absolute one where d crosses zero.  Slopes lie in [-0.2, 1.2], so 16-bit types store them
-// as fp16 (2^-11; bf16 would be 2^-8 for the same bytes); dz is rounded to the operands' type for the matrix cores.
+// in 16-bit fixed point, steps of 2^-14: off by at most 2^-15 (fp16 would be off by up to 2^-11 near 1, bf16 by 2^-8), 0 and 1
+// exact, NaN as -2.  dz is rounded to the operands' type for the matrix cores.
 //
 // The matrix instruction takes Q as its row operand and P as its column operand, so a lane of the result holds one row i of C
 // and four consecutive columns j: bias, residual and stores are contiguous per lane.
@@ -88,10 +89,42 @@ struct Epilogue {
   const void *res;          // (M, N) at stride ldr, or NULL
   long long ldr;
   void *y;                  // (M, N) dense
-  void *slope;              // (M, N) dense, fp32 for fp32 and fp16 for 16-bit types, or NULL
+  void *slope;              // (M, N) dense, fp32 for fp32 and fixed point for 16-bit types, or NULL
 };
 
-template <class T> struct SlopeOf { typedef HdF16 type; };
+struct Fixed {              // 16-bit fixed point, see above
+  typedef short elem;
+  static constexpr int kPerVec = 8;
+  static __device__ __forceinline__ float value(int i) { return i == -32768 ? __builtin_nanf("") : (float)i * 0x1p-14f; }
+  static __device__ __forceinline__ float load(const elem *p) { return value(*p); }
+  static __device__ __forceinline__ elem round(float v) { return v == v ? (elem)rintf(v * 0x1p14f) : (elem)-32768; }
+  static __device__ __forceinline__ void unpack(hd_u32x4 w, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = (int)w[i];
+      f[2 * i] = value((short)u);
+      f[2 * i + 1] = value(u >> 16);
+    }
+  }
+  static __device__ __forceinline__ hd_u32x4 pack(const float (&f)[8]) {
+    hd_u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // two of them in one instruction: round(32767 v)
+      typedef short s2 __attribute__((ext_vector_type(2)));
+      const s2 h = __builtin_bit_cast(s2, __builtin_amdgcn_cvt_pknorm_i16(f[2 * i] * (16384.f / 32767.f), f[2 * i + 1] * (16384.f / 32767.f)));
+      w[i] = __builtin_bit_cast(unsigned, h);
+    }
+    const float any = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    if (!(any == any)) {                               // rare
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (unsigned short)round(f[2 * i]) | (unsigned)(unsigned short)round(f[2 * i + 1]) << 16;
+    }
+    return w;
+  }
+};
+
+template <class T> struct SlopeOf { typedef Fixed type; };
 template <> struct SlopeOf<HdF32> { typedef HdF32 type; };
 
 struct Product {

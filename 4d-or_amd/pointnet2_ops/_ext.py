@@ -21,6 +21,7 @@ fails this module raises.  torch is used for device memory and streams only.
 import collections
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 
@@ -2273,26 +2274,47 @@ def _rows(t, name, cols=None, dtype=None, like="the logits"):
     """Check a matrix of floating rows -> (dtype code, row stride): last axis contiguous, any row stride."""
     if not isinstance(t, torch.Tensor):
         _fail(f"{name} must be a torch.Tensor")
-    if t.dtype not in _DT:
+    code = _DT.get(t.dtype)
+    if code is None:
         _fail(f"{name} must be a float32, bfloat16 or float16 tensor")
     if dtype is not None and t.dtype != dtype:
         _fail(f"{name} must have the type of {like} ({dtype})")
-    if t.dim() != 2 or (cols is not None and t.size(1) != cols):
+    shape = t.shape
+    if len(shape) != 2 or (cols is not None and shape[1] != cols):
         _fail(f"{name} must have shape (rows, {'columns' if cols is None else cols})")
-    if t.size(1) < 1:
+    if shape[1] < 1:
         _fail(f"{name} must have at least one column")
-    if t.size(1) > 1 and t.size(0) > 0 and t.stride(1) != 1:
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1 and shape[0] > 0:
         _fail(f"{name} must have a contiguous last axis")
-    return _DT[t.dtype], t.stride(0) if t.size(0) > 1 else t.size(1)
+    return code, stride[0] if shape[0] > 1 else shape[1]
+
+
+def _on_one_device(lead, *others):
+    """_same_device for tensors that are, the slow form where they are not."""
+    device = lead[0].device
+    if device.type != "cuda" or any(t is not None and t.device != device for t, _ in others):
+        _same_device(lead, *others)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(M, N, K, dt, x, ldx, w, ldw):
+    """(addresses modulo 16: only the operands' alignment counts)"""
+    return _lib.pn2_linear_act_workspace_bytes(M, N, K, dt, x, ldx, w, ldw)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_grad_workspace(M, N, K, dt, dy, ldy, slope, x, ldx, w, ldw, want):
+    return _lib.pn2_linear_act_grad_workspace_bytes(M, N, K, dt, dy, ldy, slope, x, ldx, w, ldw, want)
 
 
 def _slope_dtype(dtype):
-    return torch.float32 if dtype == torch.float32 else torch.float16
+    return torch.float32 if dtype == torch.float32 else torch.int16
 
 
 def linear_act(x, weight, bias=None, activation="none", residual=None, want_slope=False):
     """act(x weight^T + bias) + residual: x (M,K), weight (N,K), bias (N) of x's type or fp32, residual (M,N) -> y (M,N) of x's
-    type and, if wanted, the slope act'(z) for linear_act_grad (fp32, or fp16 for 16-bit types; None for activation "none").  fp32 accumulation, one rounding."""
+    type and, if wanted, the slope act'(z) for linear_act_grad (fp32, or int16 in steps of 2^-14 for 16-bit types; None for activation "none").  fp32 accumulation, one rounding."""
     dt, ldx = _rows(x, "x")
     M, K = x.shape
     _, ldw = _rows(weight, "weight", K, x.dtype, "x")
@@ -2312,15 +2334,16 @@ def linear_act(x, weight, bias=None, activation="none", residual=None, want_slop
         _, ldr = _rows(residual, "residual", N, x.dtype, "x")
         if residual.size(0) != M:
             _fail(f"residual must have shape ({M}, {N})")
-    _same_device((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"))
+    _on_one_device((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"))
     y = torch.empty(M, N, dtype=x.dtype, device=x.device)
     slope = torch.empty(M, N, dtype=_slope_dtype(x.dtype), device=x.device) if want_slope and act else None
     if M == 0:
         return y, slope
-    nb = _lib.pn2_linear_act_workspace_bytes(M, N, K, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw)
+    px, pw = x.data_ptr(), weight.data_ptr()
+    nb = _linear_workspace(M, N, K, dt, px & 15, ldx, pw & 15, ldw)
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
     es = x.element_size()
-    _call("pn2_linear_act", x, M, N, K, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), dt if bias is None else _DT[bias.dtype],
+    _call("pn2_linear_act", x, M, N, K, dt, px, ldx, pw, ldw, _ptr(bias), dt if bias is None else _DT[bias.dtype],
           act, _ptr(residual), ldr, y.data_ptr(), _ptr(slope), _ptr(ws), nb,
           alg_bytes=es * (M * K + N * K + M * N * (1 + (residual is not None) + (slope is not None))), alg_flops=2 * M * N * K)
     return y, slope
@@ -2346,7 +2369,7 @@ def linear_act_grad(dy, slope, x, weight, want_dx=True, want_dw=True, bias_dtype
         _fail("slope must be the tensor linear_act returned")
     if bias_dtype is not None and bias_dtype not in (dy.dtype, torch.float32):
         _fail(f"bias must have the type of x ({dy.dtype}) or float32")
-    _same_device((dy, "dy"), (slope, "slope"), (x, "x"), (weight, "weight"))
+    _on_one_device((dy, "dy"), (slope, "slope"), (x, "x"), (weight, "weight"))
     want_dx, want_dw = bool(want_dx), bool(want_dw)
     new = torch.zeros if M == 0 else torch.empty
     dx = new(M, K, dtype=dy.dtype, device=dy.device) if want_dx else None
@@ -2355,11 +2378,11 @@ def linear_act_grad(dy, slope, x, weight, want_dx=True, want_dw=True, bias_dtype
     want = (1 if want_dx else 0) | (2 if want_dw else 0) | (4 if db is not None else 0)
     if M == 0 or want == 0:
         return dx, dw, db
-    nb = _lib.pn2_linear_act_grad_workspace_bytes(M, N, K, dt, dy.data_ptr(), ldy, int(slope is not None), _ptr(x), ldx, _ptr(weight),
-                                                  ldw, want)
+    pdy, px, pw = dy.data_ptr(), _ptr(x) or 0, _ptr(weight) or 0
+    nb = _linear_grad_workspace(M, N, K, dt, pdy & 15, ldy, int(slope is not None), px & 15, ldx, pw & 15, ldw, want)
     ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
     es = dy.element_size()
-    _call("pn2_linear_act_grad", dy, M, N, K, dt, dy.data_ptr(), ldy, _ptr(slope), _ptr(x), ldx, _ptr(weight), ldw, _ptr(dx),
+    _call("pn2_linear_act_grad", dy, M, N, K, dt, pdy, ldy, _ptr(slope), px, ldx, pw, ldw, _ptr(dx),
           _ptr(dw), _ptr(db), dt if db is None else _DT[bias_dtype], _ptr(ws), nb,
           alg_bytes=es * (M * N * (1 + (slope is not None)) + M * K * (want_dx + want_dw) + N * K * (want_dx + want_dw)),
           alg_flops=2 * M * N * K * (want_dx + want_dw))
@@ -2381,7 +2404,7 @@ def label_logprobs(logits, labels, top=0, ignore_index=-100, want_stats=False):
     top = int(top)
     if top < 0 or top > min(V, MAX_TOP):
         _fail(f"top must lie in 0 .. min(columns, {MAX_TOP})")
-    _same_device((logits, "logits"), (labels, "labels"))
+    _on_one_device((logits, "logits"), (labels, "labels"))
     f32 = dict(dtype=torch.float32, device=logits.device)
     lp, ent = torch.empty(T, **f32), torch.empty(T, **f32)
     tlp = torch.empty(T, top, **f32) if top else None
@@ -2406,7 +2429,7 @@ def label_logprobs_grad(logits, labels, stats, entropy, g_log_prob, g_entropy, i
                 _fail(f"{name} must have shape ({T},)")
     if stats.shape != (T, 2) or entropy.shape != (T,):
         _fail("stats and entropy must be the tensors label_logprobs returned")
-    _same_device((logits, "logits"), (labels, "labels"), (stats, "stats"), (entropy, "entropy"), (g_log_prob, "g_log_prob"),
+    _on_one_device((logits, "logits"), (labels, "labels"), (stats, "stats"), (entropy, "entropy"), (g_log_prob, "g_log_prob"),
                  (g_entropy, "g_entropy"))
     out = torch.empty(T, V, dtype=logits.dtype, device=logits.device)
     if T:
@@ -2436,7 +2459,7 @@ def distill_topk(logits, teacher_index, teacher_logits, temperature=1.0, want_st
     dt, ld = _rows(logits, "logits")
     t = _check_teacher(logits, teacher_index, teacher_logits, temperature)
     T, V = logits.shape
-    _same_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"))
+    _on_one_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"))
     loss = torch.empty(T, dtype=torch.float32, device=logits.device)
     stats = torch.empty(T, 4, dtype=torch.float32, device=logits.device) if want_stats else None
     if T:
@@ -2454,7 +2477,7 @@ def distill_topk_grad(logits, teacher_index, teacher_logits, temperature, stats,
     _f32(stats, "stats"); _f32(g_loss, "g_loss")
     if stats.shape != (T, 4) or g_loss.shape != (T,):
         _fail("stats must be the tensor distill_topk returned, g_loss one gradient per row")
-    _same_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"), (stats, "stats"),
+    _on_one_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"), (stats, "stats"),
                  (g_loss, "g_loss"))
     out = torch.empty(T, V, dtype=logits.dtype, device=logits.device)
     if T:

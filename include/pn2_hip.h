@@ -965,7 +965,7 @@ int pn2_distill_topk_grad(long long T, int V, long long ld, int dtype, const voi
  * ldx, W (N, K) at row stride ldw, residual (M, N) at row stride ldr (or NULL), all of `dtype`, last axis contiguous, any
  * alignment of an element; bias (N) of `dtype` or fp32 (or NULL); y, slope (M, N) dense.  act 0 none | 1 relu | 2 gelu (erf) |
  * 3 gelu (tanh form) | 4 silu.  fp32 accumulation and epilogue, one rounding.  slope: act'(z), what the backward pass needs,
- * fp32 for fp32 and fp16 for both 16-bit types (NULL: not wanted; never written for act 0).
+ * fp32 for fp32 and int16 in steps of 2^-14 for both 16-bit types (NULL: not wanted; never written for act 0).
  * The gradient: dy (M, N) at row stride ldy; slope NULL stands for ones; dx (M, K), dw (N, K) dense, db (N) of db_dtype, each NULL
  * = not wanted, every element written; sums in a fixed order.  want = 1 dx | 2 dw | 4 db.
  * 1 <= N, K <= 4194304.  The workspace sizes take the operands (only their alignment is looked at).  A workspace must not be
