@@ -860,14 +860,15 @@ inline long long la_whole(long long n, int dtype) { return la_div(n, 16 / la_siz
 
 // Which kernel a product takes, and how often its contraction is split, by size and type.  Microseconds measured for bf16 unless
 // said otherwise, this choice against the next one:
-//   small   (no LDS, waves split the contraction) few rows, or few results: 1 x 4096 x 4096 8.2 against 16.8 for a split 64 x 64 tile;
-//           72 x 512 x 256 4.1 against 7.9;  fp32 also up to 512 x 512 (8.0 against 12.8 for 64 x 64; bf16 5.6 against 5.0)
+//   small   (no LDS, waves split the contraction) few rows, or few results: 1 x 4096 x 4096 8.2 against 16.8 for a split 64 x 64 tile,
+//           72 x 512 x 256 4.1 against 7.9;  but 8 x 32768 x 2048 33 against 22, 32 x 8192 x 8192 46 against 27.  fp32, whose weights
+//           cost twice: up to 16 rows always (16 x 8192 x 8192 61 against 74), and up to 512 x 512 (8.0 against 12.8)
 //   64 x 64       up to 512 tiles: 1024^3 7.2 against 8.1 (128 x 64) and 11.0 (128 x 128)
 //   128 x 64      2048^3 22.5 against 25.6 (64 x 64) and 24.5 (128 x 128);  fp32 128 against 127 and 134
 //   128 x 128     fp32 from 512 such tiles on: 4096 x 4096 x 512 dW 147 against 167
 //   256 x 256     16-bit, tiles for three quarters of the CUs: 8192^3 784 against 1248 (128 x 128)
 // Splits only where a workgroup would walk a long contraction while CUs idle (a join costs a launch and the partial sums' traffic):
-// 128 x 8192 x 8192 58 -> 35 with four; 1024^3 7.2 -> 12.5 with two.
+// 128 x 8192 x 8192 58 -> 35 with four, 64 x 4096 x 4096 21 -> 15 with four instead of two; 1024^3 7.2 -> 12.5 with two.
 enum { SMALL_11, SMALL_21, SMALL_22, TILE_64, TILE_128_64, TILE_128, TILE_256 };
 struct Plan {
   int kernel, splits;
@@ -879,11 +880,9 @@ Plan la_plan(long long M, long long N, long long K, int dtype, bool small_ok) {
   const long long n16 = la_div(M, 16) * la_div(N, 16);
   Plan p{TILE_64, 1, K};
   if (small_ok && K <= 16384) {
-    if (M <= 16) p.kernel = SMALL_11;
-    else if (M <= 32) p.kernel = SMALL_21;
-    else if (n16 <= 256) p.kernel = SMALL_11;
-    else if (n16 <= 512) p.kernel = SMALL_21;
-    else if (n16 <= (f32 ? 1024 : 512) || (N <= 32 && K <= 1024)) p.kernel = SMALL_22;
+    if (M <= (f32 ? 16 : 4) || n16 <= 256) p.kernel = SMALL_11;
+    else if (n16 <= 512 && (f32 || K <= 4096)) p.kernel = SMALL_21;
+    else if ((f32 && n16 <= 1024) || (N <= 32 && K <= 1024)) p.kernel = SMALL_22;
     if (p.kernel != TILE_64) return p;
   }
   const long long t256 = la_div(M, 256) * la_div(N, 256), t128 = la_div(M, 128) * la_div(N, 128), t12864 = la_div(M, 128) * la_div(N, 64),
@@ -894,7 +893,8 @@ Plan la_plan(long long M, long long N, long long K, int dtype, bool small_ok) {
   else if (t64 > 512) { p.kernel = TILE_128_64; tiles = t12864; }
   const long long kb = f32 ? 32 : 64, steps = la_div(K, kb);
   long long s = (p.kernel == TILE_256 ? 256 : 512) / tiles;
-  if (s > steps / 32) s = steps / 32;
+  const long long least = f32 ? 32 : 16;               // tiles of 128 bytes a workgroup walks at least
+  if (s > steps / least) s = steps / least;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
   p.kchunk = la_div(steps, s) * kb;
