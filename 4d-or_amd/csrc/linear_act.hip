@@ -378,19 +378,29 @@ __device__ __forceinline__ void la_epilogue(const Product &a, const la_f32x4 (&a
           la_load8<T, FULL>((const elem *)e.res + row * e.ldr + col(u), FULL || row < a.M ? a.N - col(u) : 0, r[t][u / 2]);
         }
     }
-    la_each<TJ>([&](auto n_) __attribute__((always_inline)) {
-      constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
-      const long long row = i + (t0 + t) * 16, left = FULL || row < a.M ? a.N - col(u) : 0;
-      if (!FULL && left <= 0) return;
-      float y[8], d[8];
+    la_each<2>([&](auto t_) __attribute__((always_inline)) {
+      constexpr int t = decltype(t_)::value;
+      const long long row = i + (t0 + t) * 16;
+      if (!FULL && row >= a.M) return;
+      float y[TJ / 2][8], d[TJ / 2][8];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        la_act<ACT, sizeof(elem) == 2>(acc[t0 + t][u + n / 4][n % 4] + b[u / 2][n], y[n], d[n]);
-        if constexpr (RES) y[n] += r[t][u / 2][n];
-      }
-      la_store8<T, FULL>((elem *)e.y + row * a.N + col(u), left, y);
+      for (int u = 0; u < TJ; u += 2)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          la_act<ACT, sizeof(elem) == 2>(acc[t0 + t][u + n / 4][n % 4] + b[u / 2][n], y[u / 2][n], d[u / 2][n]);
+          if constexpr (RES) y[u / 2][n] += r[t][u / 2][n];
+        }
+      // (the halves of a cache line of y one right after the other, then the slope's: between them a line can leave the cache half
+      // written, and the tile's results are more than the cache)
+#pragma unroll
+      for (int u = 0; u < TJ; u += 2)
+        if (FULL || a.N > col(u)) la_store8<T, FULL>((elem *)e.y + row * a.N + col(u), a.N - col(u), y[u / 2]);
       if constexpr (ACT != ACT_NONE) {
-        if (e.slope) la_store8<S, FULL>((typename S::elem *)e.slope + row * a.N + col(u), left, d);
+        if (e.slope) {
+#pragma unroll
+          for (int u = 0; u < TJ; u += 2)
+            if (FULL || a.N > col(u)) la_store8<S, FULL>((typename S::elem *)e.slope + row * a.N + col(u), a.N - col(u), d[u / 2]);
+        }
       }
     });
   });

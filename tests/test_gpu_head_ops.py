@@ -93,7 +93,10 @@ def tiny(dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 17, 5), (3, 7, 9), (72, 512, 256), (1, 300, 1001), (130, 65, 33), (64, 64, 64), (257, 129, 2048), (5, 1, 700),
-          (1003, 77, 101), (16, 4096, 128), (33, 520, 4104), (300, 264, 72), (256, 256, 32), (512, 776, 328), (640, 1304, 4104), (1032, 136, 1000), (2100, 520, 264)]
+          (1003, 77, 101), (16, 4096, 128), (33, 520, 4104), (300, 264, 72), (256, 256, 32), (512, 776, 328), (640, 1304, 4104), (1032, 136, 1000), (2100, 520, 264),
+          # one of every kernel and rule: few columns, 128 x 64 and 128 x 128 (fp32) / 256 x 256 (16-bit) tiles, padded copies, split sums
+          (128, 1000, 300), (5000, 20, 100), (2100, 1032, 264), (8200, 1030, 40), (4100, 2900, 72), (1003, 777, 1001), (640, 1301, 4099),
+          (20000, 40, 33), (7, 3000, 20000)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -540,7 +543,7 @@ def test_a_head_trained_from_a_teacher(dtype):
     want = want + 4 * (q * (q.log() - l2.gather(1, teacher[0]))).sum(1).mean()
     wg = torch.autograd.grad(want, ref)
     tol = 5 * max(half(dtype), 64 * U)
-    assert abs(float(loss - want)) <= tol * float(want.abs())
+    assert abs(float((loss - want).detach())) <= tol * float(want.detach().abs())
     for g, e in zip(grads, wg):
         assert g.dtype == dtype
         rms = float(e.pow(2).mean().sqrt())
@@ -577,6 +580,40 @@ def test_captured_step_replays_with_new_inputs():
         for a, b in zip(got, step()):
             # (mean() of the loss is torch's; everything else is bit-identical between eager and replay)
             assert torch.equal(a, b) if a.dtype != torch.float32 else torch.allclose(a, b, rtol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1003, 777, 1001), (300, 200, 9000), (4096, 96, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_captured_layer_with_copies_and_split_sums(shape, dtype):
+    """Workspaces inside a graph: padded copies, dz, strips of db, partial sums; two graphs of the same layer replayed in turn."""
+    M, N, K = shape
+    gen = torch.Generator().manual_seed(M)
+    x, w, dy = rnd(gen, M, K, dtype=dtype), rnd(gen, N, K, scale=K ** -0.5, dtype=dtype), rnd(gen, M, N, dtype=dtype)
+    b = rnd(gen, N, dtype=dtype)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = ho.linear_act(*leaves, "gelu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for n in range(4):
+        x.copy_(rnd(torch.Generator().manual_seed(50 + n), M, K, dtype=dtype))
+        dy.copy_(rnd(torch.Generator().manual_seed(60 + n), M, N, dtype=dtype))
+        g, out = graphs[n % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, e) for a, e in zip(got, step()))
 
 
 def test_two_streams_at_once_and_record_of_inputs():
