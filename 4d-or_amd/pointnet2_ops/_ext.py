@@ -21,7 +21,6 @@ fails this module raises.  torch is used for device memory and streams only.
 import collections
 import contextlib
 import ctypes
-import functools
 import os
 import threading
 
@@ -411,9 +410,11 @@ _FN = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _call(name, ref, *args, alg_bytes=0, alg_flops=0, tag=None, label=None):
-    """Enqueue `name` on the current stream of `ref`'s device (`label`: row name in the kernel timer, default `name`)."""
-    fn = _FN.get(name)
+def _call(name, ref, *args, alg_bytes=0, alg_flops=0, tag=None, label=None, fn=None):
+    """Enqueue `name` on the current stream of `ref`'s device (`label`: row name in the kernel timer, default `name`; `fn`: the call
+    where it is not the entry point itself)."""
+    if fn is None:
+        fn = _FN.get(name)
     if fn is None:
         fn = _FN[name] = getattr(_lib, name)
     dev = ref.device.index
@@ -430,14 +431,14 @@ def _call(name, ref, *args, alg_bytes=0, alg_flops=0, tag=None, label=None):
         if TIMER is not None and TIMER.enabled:
             ev0, ev1 = TIMER.event(), TIMER.event()
             _lib.pn2_event_record(ev0, stream)
-            rc = getattr(_lib, name)(*args, stream)
+            rc = fn(*args, stream)
             _lib.pn2_event_record(ev1, stream)
             label = (label or name) if tag is None else f"{label or name}[{tag}]"
             if TIMER.main_stream is not None and stream != TIMER.main_stream:
                 label += "@side"
             TIMER.records.append((label, ev0, ev1, int(alg_bytes), int(alg_flops)))
         else:
-            rc = getattr(_lib, name)(*args, stream)
+            rc = fn(*args, stream)
     if rc != 0:
         detail = _lib.pn2_strerror(rc).decode()
         _fail(f"{name} failed: {detail} (rc={rc}, hipError={_lib.pn2_last_hip_error()})")
@@ -2265,223 +2266,9 @@ def gen_edge_input(max_dist, path, edge_feat):
 
 
 # ------------------------------------------------------------------------------------------------------- dense heads
-_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/pn2_hip.h: PN2_DT_*
-ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-MAX_TOP = 64
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}      # `act` of include/pn2_hip.h
 
 
-def _rows(t, name, cols=None, dtype=None, like="the logits"):
-    """Check a matrix of floating rows -> (dtype code, row stride): last axis contiguous, any row stride."""
-    if not isinstance(t, torch.Tensor):
-        _fail(f"{name} must be a torch.Tensor")
-    code = _DT.get(t.dtype)
-    if code is None:
-        _fail(f"{name} must be a float32, bfloat16 or float16 tensor")
-    if dtype is not None and t.dtype != dtype:
-        _fail(f"{name} must have the type of {like} ({dtype})")
-    shape = t.shape
-    if len(shape) != 2 or (cols is not None and shape[1] != cols):
-        _fail(f"{name} must have shape (rows, {'columns' if cols is None else cols})")
-    if shape[1] < 1:
-        _fail(f"{name} must have at least one column")
-    stride = t.stride()
-    if stride[1] != 1 and shape[1] > 1 and shape[0] > 0:
-        _fail(f"{name} must have a contiguous last axis")
-    return code, stride[0] if shape[0] > 1 else shape[1]
-
-
-def _on_one_device(lead, *others):
-    """_same_device for tensors that are, the slow form where they are not."""
-    device = lead[0].device
-    if device.type != "cuda" or any(t is not None and t.device != device for t, _ in others):
-        _same_device(lead, *others)
-
-
-@functools.lru_cache(maxsize=4096)
-def _linear_workspace(M, N, K, dt, x, ldx, w, ldw):
-    """(addresses modulo 16: only the operands' alignment counts)"""
-    return _lib.pn2_linear_act_workspace_bytes(M, N, K, dt, x, ldx, w, ldw)
-
-
-@functools.lru_cache(maxsize=4096)
-def _linear_grad_workspace(M, N, K, dt, dy, ldy, slope, x, ldx, w, ldw, want):
-    return _lib.pn2_linear_act_grad_workspace_bytes(M, N, K, dt, dy, ldy, slope, x, ldx, w, ldw, want)
-
-
-def _slope_dtype(dtype):
-    return torch.float32 if dtype == torch.float32 else torch.int16
-
-
-def linear_act(x, weight, bias=None, activation="none", residual=None, want_slope=False):
-    """act(x weight^T + bias) + residual: x (M,K), weight (N,K), bias (N) of x's type or fp32, residual (M,N) -> y (M,N) of x's
-    type and, if wanted, the slope act'(z) for linear_act_grad (fp32, or int16 in steps of 2^-14 for 16-bit types; None for activation "none").  fp32 accumulation, one rounding."""
-    dt, ldx = _rows(x, "x")
-    M, K = x.shape
-    _, ldw = _rows(weight, "weight", K, x.dtype, "x")
-    N = weight.size(0)
-    if N < 1:
-        _fail("weight must have at least one row")
-    act = ACTIVATIONS.get(activation)
-    if act is None:
-        _fail(f"activation must be one of {', '.join(ACTIVATIONS)}")
-    if bias is not None:
-        if bias.shape != (N,) or not bias.is_contiguous():
-            _fail(f"bias must be a contiguous tensor of shape ({N},)")
-        if bias.dtype not in (x.dtype, torch.float32):
-            _fail(f"bias must have the type of x ({x.dtype}) or float32")
-    ldr = 0
-    if residual is not None:
-        _, ldr = _rows(residual, "residual", N, x.dtype, "x")
-        if residual.size(0) != M:
-            _fail(f"residual must have shape ({M}, {N})")
-    _on_one_device((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"))
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    slope = torch.empty(M, N, dtype=_slope_dtype(x.dtype), device=x.device) if want_slope and act else None
-    if M == 0:
-        return y, slope
-    px, pw = x.data_ptr(), weight.data_ptr()
-    nb = _linear_workspace(M, N, K, dt, px & 15, ldx, pw & 15, ldw)
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
-    es = x.element_size()
-    _call("pn2_linear_act", x, M, N, K, dt, px, ldx, pw, ldw, _ptr(bias), dt if bias is None else _DT[bias.dtype],
-          act, _ptr(residual), ldr, y.data_ptr(), _ptr(slope), _ptr(ws), nb,
-          alg_bytes=es * (M * K + N * K + M * N * (1 + (residual is not None) + (slope is not None))), alg_flops=2 * M * N * K)
-    return y, slope
-
-
-def linear_act_grad(dy, slope, x, weight, want_dx=True, want_dw=True, bias_dtype=None):
-    """Gradients of linear_act for dy (M,N): (dx, dw, db), None where not wanted (`bias_dtype` None: no db).  dx needs the weight,
-    dw needs x; the other may be None."""
-    dt, ldy = _rows(dy, "dy")
-    M, N = dy.shape
-    if (want_dx and weight is None) or (want_dw and x is None):
-        _fail("dx needs weight, dw needs x")
-    K, ldx, ldw = 1, 0, 0
-    if x is not None:
-        _, ldx = _rows(x, "x", None, dy.dtype, "dy")
-        K = x.size(1)
-    if weight is not None:
-        _, ldw = _rows(weight, "weight", None if x is None else K, dy.dtype, "dy")
-        K = weight.size(1)
-    if (x is not None and x.size(0) != M) or (weight is not None and weight.size(0) != N):
-        _fail("dy, x and weight do not belong together")
-    if slope is not None and (slope.shape != dy.shape or slope.dtype != _slope_dtype(dy.dtype) or not slope.is_contiguous()):
-        _fail("slope must be the tensor linear_act returned")
-    if bias_dtype is not None and bias_dtype not in (dy.dtype, torch.float32):
-        _fail(f"bias must have the type of x ({dy.dtype}) or float32")
-    _on_one_device((dy, "dy"), (slope, "slope"), (x, "x"), (weight, "weight"))
-    want_dx, want_dw = bool(want_dx), bool(want_dw)
-    new = torch.zeros if M == 0 else torch.empty
-    dx = new(M, K, dtype=dy.dtype, device=dy.device) if want_dx else None
-    dw = new(N, K, dtype=dy.dtype, device=dy.device) if want_dw else None
-    db = new(N, dtype=bias_dtype, device=dy.device) if bias_dtype is not None else None
-    want = (1 if want_dx else 0) | (2 if want_dw else 0) | (4 if db is not None else 0)
-    if M == 0 or want == 0:
-        return dx, dw, db
-    pdy, px, pw = dy.data_ptr(), _ptr(x) or 0, _ptr(weight) or 0
-    nb = _linear_grad_workspace(M, N, K, dt, pdy & 15, ldy, int(slope is not None), px & 15, ldx, pw & 15, ldw, want)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
-    es = dy.element_size()
-    _call("pn2_linear_act_grad", dy, M, N, K, dt, pdy, ldy, _ptr(slope), px, ldx, pw, ldw, _ptr(dx),
-          _ptr(dw), _ptr(db), dt if db is None else _DT[bias_dtype], _ptr(ws), nb,
-          alg_bytes=es * (M * N * (1 + (slope is not None)) + M * K * (want_dx + want_dw) + N * K * (want_dx + want_dw)),
-          alg_flops=2 * M * N * K * (want_dx + want_dw))
-    return dx, dw, db
-
-
-def _check_labels(logits, labels):
-    _check(labels, "labels", torch.int64)
-    if labels.shape != logits.shape[:1]:
-        _fail(f"labels must have shape ({logits.size(0)},)")
-
-
-def label_logprobs(logits, labels, top=0, ignore_index=-100, want_stats=False):
-    """logits (T,V), labels (T) int64 -> (log_prob (T) f32, entropy (T) f32, top_log_prob (T,top) f32 | None, top_index (T,top) i64 |
-    None, stats (T,2) f32 | None); include/pn2_hip.h: pn2_label_logprobs."""
-    dt, ld = _rows(logits, "logits")
-    _check_labels(logits, labels)
-    T, V = logits.shape
-    top = int(top)
-    if top < 0 or top > min(V, MAX_TOP):
-        _fail(f"top must lie in 0 .. min(columns, {MAX_TOP})")
-    _on_one_device((logits, "logits"), (labels, "labels"))
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    lp, ent = torch.empty(T, **f32), torch.empty(T, **f32)
-    tlp = torch.empty(T, top, **f32) if top else None
-    tix = torch.empty(T, top, dtype=torch.int64, device=logits.device) if top else None
-    stats = torch.empty(T, 2, **f32) if want_stats else None
-    if T:
-        _call("pn2_label_logprobs", logits, T, V, ld, dt, logits.data_ptr(), labels.data_ptr(), int(ignore_index), top, lp.data_ptr(),
-              ent.data_ptr(), _ptr(stats), _ptr(tlp), _ptr(tix), alg_bytes=T * V * logits.element_size() + T * (16 + 12 * top))
-    return lp, ent, tlp, tix, stats
-
-
-def label_logprobs_grad(logits, labels, stats, entropy, g_log_prob, g_entropy, ignore_index=-100):
-    """-> dlogits (T,V) of logits' type; g_log_prob / g_entropy (T) f32 or None."""
-    dt, ld = _rows(logits, "logits")
-    _check_labels(logits, labels)
-    T, V = logits.shape
-    _f32(stats, "stats"); _f32(entropy, "entropy")
-    for g, name in ((g_log_prob, "g_log_prob"), (g_entropy, "g_entropy")):
-        if g is not None:
-            _f32(g, name)
-            if g.shape != (T,):
-                _fail(f"{name} must have shape ({T},)")
-    if stats.shape != (T, 2) or entropy.shape != (T,):
-        _fail("stats and entropy must be the tensors label_logprobs returned")
-    _on_one_device((logits, "logits"), (labels, "labels"), (stats, "stats"), (entropy, "entropy"), (g_log_prob, "g_log_prob"),
-                 (g_entropy, "g_entropy"))
-    out = torch.empty(T, V, dtype=logits.dtype, device=logits.device)
-    if T:
-        _call("pn2_label_logprobs_grad", logits, T, V, ld, dt, logits.data_ptr(), labels.data_ptr(), int(ignore_index), stats.data_ptr(),
-              entropy.data_ptr(), _ptr(g_log_prob), _ptr(g_entropy), out.data_ptr(), alg_bytes=2 * T * V * logits.element_size())
-    return out
-
-
-def _check_teacher(logits, index, values, temperature):
-    T = logits.size(0)
-    _check(index, "teacher_index", torch.int64)
-    if not isinstance(values, torch.Tensor) or values.dtype not in _DT:
-        _fail("teacher_logits must be a float32, bfloat16 or float16 tensor")
-    if not values.is_contiguous():
-        _fail("teacher_logits must be a contiguous tensor")
-    if index.dim() != 2 or index.size(0) != T or index.size(1) < 1 or values.shape != index.shape:
-        _fail(f"teacher_index and teacher_logits must have shape ({T}, k), k >= 1")
-    t = float(temperature)
-    if not 0.0 < t < float("inf"):
-        _fail("temperature must be positive and finite")
-    return t
-
-
-def distill_topk(logits, teacher_index, teacher_logits, temperature=1.0, want_stats=False):
-    """logits (T,V), teacher_index (T,k) int64, teacher_logits (T,k) -> (loss (T) f32, stats (T,4) f32 | None);
-    include/pn2_hip.h: pn2_distill_topk."""
-    dt, ld = _rows(logits, "logits")
-    t = _check_teacher(logits, teacher_index, teacher_logits, temperature)
-    T, V = logits.shape
-    _on_one_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"))
-    loss = torch.empty(T, dtype=torch.float32, device=logits.device)
-    stats = torch.empty(T, 4, dtype=torch.float32, device=logits.device) if want_stats else None
-    if T:
-        _call("pn2_distill_topk", logits, T, V, ld, dt, logits.data_ptr(), teacher_index.size(1), teacher_index.data_ptr(),
-              _DT[teacher_logits.dtype], teacher_logits.data_ptr(), t, loss.data_ptr(), _ptr(stats),
-              alg_bytes=T * V * logits.element_size())
-    return loss, stats
-
-
-def distill_topk_grad(logits, teacher_index, teacher_logits, temperature, stats, g_loss):
-    """-> dlogits (T,V) of logits' type for the gradient g_loss (T) f32 of the row losses."""
-    dt, ld = _rows(logits, "logits")
-    t = _check_teacher(logits, teacher_index, teacher_logits, temperature)
-    T, V = logits.shape
-    _f32(stats, "stats"); _f32(g_loss, "g_loss")
-    if stats.shape != (T, 4) or g_loss.shape != (T,):
-        _fail("stats must be the tensor distill_topk returned, g_loss one gradient per row")
-    _on_one_device((logits, "logits"), (teacher_index, "teacher_index"), (teacher_logits, "teacher_logits"), (stats, "stats"),
-                 (g_loss, "g_loss"))
-    out = torch.empty(T, V, dtype=logits.dtype, device=logits.device)
-    if T:
-        _call("pn2_distill_topk_grad", logits, T, V, ld, dt, logits.data_ptr(), teacher_index.size(1), teacher_index.data_ptr(),
-              _DT[teacher_logits.dtype], teacher_logits.data_ptr(), t, stats.data_ptr(), g_loss.data_ptr(), out.data_ptr(),
-              alg_bytes=2 * T * V * logits.element_size())
-    return out
+def address(name):
+    """Address of an entry point of the loaded library (for pointnet2_ops._heads, whose nodes call it without the interpreter)."""
+    return ctypes.cast(getattr(_lib, name), ctypes.c_void_p).value

@@ -13,55 +13,35 @@ Leading axes are free; tensors must be on the GPU (RuntimeError otherwise), work
 nothing is synchronised or kept between calls.  Each operator is differentiable once.
 """
 import collections
+import os
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from pointnet2_ops import _ext
+
+try:
+    from pointnet2_ops import _heads
+except ImportError as e:
+    raise ImportError(f"pointnet2_ops._heads: {e}. Build it with `make -C {os.path.join(_ext._PKG_DIR, 'csrc')}` (or "
+                      "__graft_entry__.build()); there is no CPU/PyTorch fallback.") from e
 
 ACTIVATIONS = tuple(_ext.ACTIVATIONS)
 
 LabelLogProbs = collections.namedtuple("LabelLogProbs", "log_prob entropy top_log_prob top_index")
 
-
-def _once(backward):
-    """once_differentiable, without its price where no graph of the backward pass is being built."""
-    guarded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
+# arguments, allocation and autograd nodes: csrc/head_binding.cpp, around the entry points of the library that _ext has loaded
+_heads.bind(_ext.address, _ext._call)
 
 
-def _matrix(t, name):
-    """(..., C) -> (rows, C) with a contiguous last axis; a copy only where the strides allow no view."""
-    if not isinstance(t, torch.Tensor) or t.dim() < 1:
-        _ext._fail(f"{name} must be a tensor with at least one axis")
-    if t.dim() != 2:
-        t = t.reshape(-1, t.size(-1)) if t.size(-1) else t.reshape(t.shape[:-1].numel(), 0)
-    return t if t.size(1) == 1 or t.stride(1) == 1 else t.contiguous()
+def _timed():
+    return _ext.TIMER is not None and _ext.TIMER.enabled
 
 
-class _LinearAct(Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
-        y, slope = _ext.linear_act(x, weight, bias, activation, residual, want_slope=need_dx or need_dw or need_db)
-        ctx.save_for_backward(x if need_dw else None, weight if need_dx else None, slope)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        need_dx, need_dw, need_db, need_dr, _ = ctx.needs_input_grad
-        dx = dw = db = None
-        if need_dx or need_dw or need_db:
-            x, weight, slope = ctx.saved_tensors
-            dx, dw, db = _ext.linear_act_grad(_matrix(dy, "dy"), slope, x, weight, need_dx, need_dw,
-                                              ctx.bias_dtype if need_db else None)
-        return dx, dw, db, dy if need_dr else None, None
+def _tensors(**named):
+    """The reason of a refused call whose arguments are no tensors."""
+    for name, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            _ext._fail(f"{name} must be a torch.Tensor")
 
 
 def linear_act(x, weight, bias=None, activation="none", residual=None):
@@ -71,43 +51,14 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     activation one of ``ACTIVATIONS``: none, relu, gelu (erf), gelu_tanh, silu.  -> (..., N) of x's type.
     Products accumulate in fp32; bias, activation and residual are applied to the accumulator and the result is rounded once.
     The backward pass keeps the activation's slope (one tensor like y); all its sums run in a fixed order."""
-    xm, wm = _matrix(x, "x"), _matrix(weight, "weight")
-    if weight.dim() != 2:
-        _ext._fail("weight must have shape (N, K)")
-    shape = x.shape[:-1] + weight.shape[:1]
-    rm = None
-    if residual is not None:
-        try:
-            rm = _matrix(residual.expand(shape), "residual")
-        except RuntimeError:
-            _ext._fail(f"residual must broadcast to {tuple(shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
-        y = _LinearAct.apply(xm, wm, bias, rm, activation)
-    else:
-        y, _ = _ext.linear_act(xm, wm, bias, activation, rm)
-    return y if x.dim() == 2 else y.view(shape)
-
-
-class _LabelLogProbs(Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top, ignore_index):
-        lp, ent, tlp, tix, stats = _ext.label_logprobs(logits, labels, top, ignore_index, want_stats=True)
-        ctx.save_for_backward(logits, labels, stats, ent)
-        ctx.ignore_index = ignore_index
-        ctx.set_materialize_grads(False)
-        if top:
-            ctx.mark_non_differentiable(tlp, tix)
-        return lp, ent, tlp, tix
-
-    @staticmethod
-    @_once
-    def backward(ctx, g_lp, g_ent, _tlp, _tix):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        logits, labels, stats, ent = ctx.saved_tensors
-        g_lp, g_ent = (None if g is None else g.contiguous() for g in (g_lp, g_ent))
-        return _ext.label_logprobs_grad(logits, labels, stats, ent, g_lp, g_ent, ctx.ignore_index), None, None, None
+    act = _ext.ACTIVATIONS.get(activation)
+    if act is None:
+        _ext._fail(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    try:
+        return _heads.linear_act(x, weight, bias, act, residual, _timed())
+    except TypeError:
+        _tensors(x=x, weight=weight, **{n: t for n, t in (("bias", bias), ("residual", residual)) if t is not None})
+        raise
 
 
 def label_log_probs(logits, labels, top=0, ignore_index=-100):
@@ -120,37 +71,12 @@ def label_log_probs(logits, labels, top=0, ignore_index=-100):
       (None, None for top = 0).  A masked entry (-inf) has probability 0 and is no alternative: unused slots hold -inf and -1.
     A row of nothing but -inf has log_prob -inf, entropy 0, no alternatives and gradient 0; a row with NaN or +inf is NaN.
     log_prob and entropy are differentiable in the logits, the alternatives are not."""
-    lm = _matrix(logits, "logits")
-    shape = logits.shape[:-1]
-    if not isinstance(labels, torch.Tensor) or labels.shape != shape:
-        _ext._fail(f"labels must be a tensor of shape {tuple(shape)}")
-    ym = labels.reshape(-1)
-    if not ym.is_contiguous():
-        ym = ym.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        lp, ent, tlp, tix = _LabelLogProbs.apply(lm, ym, int(top), int(ignore_index))
-    else:
-        lp, ent, tlp, tix, _ = _ext.label_logprobs(lm, ym, top, ignore_index)
-    if logits.dim() != 2:
-        lp, ent = lp.view(shape), ent.view(shape)
-        if tlp is not None:
-            tlp, tix = tlp.view(shape + (-1,)), tix.view(shape + (-1,))
-    return LabelLogProbs(lp, ent, tlp, tix)
-
-
-class _DistillTopK(Function):
-    @staticmethod
-    def forward(ctx, logits, index, values, temperature):
-        loss, stats = _ext.distill_topk(logits, index, values, temperature, want_stats=True)
-        ctx.save_for_backward(logits, index, values, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @_once
-    def backward(ctx, g):
-        logits, index, values, stats = ctx.saved_tensors
-        return _ext.distill_topk_grad(logits, index, values, ctx.temperature, stats, g.contiguous()), None, None, None
+    top, ignore_index = int(top), int(ignore_index)
+    try:
+        return LabelLogProbs(*_heads.label_log_probs(logits, labels, top, ignore_index, _timed()))
+    except TypeError:
+        _tensors(logits=logits, labels=labels)
+        raise
 
 
 def distill_top_k(logits, teacher_index, teacher_logits, temperature=1.0):
@@ -161,17 +87,8 @@ def distill_top_k(logits, teacher_index, teacher_logits, temperature=1.0):
     all V.  -> (...) fp32, differentiable in the logits; the teacher is a constant (RuntimeError if it requires a gradient).
     A slot with a negative index or the value -inf is unused; a row without a used slot has loss 0 and gradient 0 (so padded rows
     take teacher_index = -1).  An index >= V makes its row NaN; an index may occur more than once."""
-    lm = _matrix(logits, "logits")
-    shape = logits.shape[:-1]
-    for t, name in ((teacher_index, "teacher_index"), (teacher_logits, "teacher_logits")):
-        if not isinstance(t, torch.Tensor) or t.dim() != logits.dim() or t.shape[:-1] != shape:
-            _ext._fail(f"{name} must be a tensor of shape {tuple(shape) + ('k',)}")
-    if teacher_logits.requires_grad:
-        _ext._fail("teacher_logits must not require a gradient (detach the teacher)")
-    im, vm = (t.reshape(-1, t.size(-1)) if t.dim() != 2 and t.size(-1) else t for t in (teacher_index, teacher_logits))
-    im, vm = im.contiguous(), vm.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        loss = _DistillTopK.apply(lm, im, vm, float(temperature))
-    else:
-        loss, _ = _ext.distill_topk(lm, im, vm, temperature)
-    return loss if logits.dim() == 2 else loss.view(shape)
+    try:
+        return _heads.distill_top_k(logits, teacher_index, teacher_logits, float(temperature), _timed())
+    except TypeError:
+        _tensors(logits=logits, teacher_index=teacher_index, teacher_logits=teacher_logits)
+        raise

@@ -176,9 +176,10 @@ def test_linear_act_infinities_nan_and_frozen_inputs():
         assert (y[3] == (-INF if act == "none" else 0)).all()
     # only what needs a gradient is computed; nothing else is held
     b = torch.zeros(48, device="cuda", requires_grad=True)
-    y = ho.linear_act(x[:1], w, b, "relu")
-    saved_x, saved_w, slope = y.grad_fn.saved_tensors
-    assert saved_x is None and saved_w is None and slope.dtype == torch.int16
+    held = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append(t) or t, lambda t: t):
+        y = ho.linear_act(x[:1], w, b, "relu")
+    assert [t.dtype for t in held] == [torch.int16]
     y.sum().backward()
     assert b.grad.shape == (48,)
     with pytest.raises(RuntimeError):
@@ -650,6 +651,63 @@ def test_rows_past_two_to_the_32_elements():
     check(r.log_prob[rows.cuda()], *want["log_prob"])
     assert torch.equal(r.top_index[rows.cuda()].cpu(), want["top_index"])
     assert float((r.entropy[1:1000] - math.log(V)).abs().max()) < 1e-5
+
+
+def test_kernel_timer_records_the_heads_and_their_gradients(monkeypatch):
+    """Under the timer every launch is one record with its bytes and operations; results stay what they are without it."""
+    gen = torch.Generator().manual_seed(3)
+    x, w = rnd(gen, 72, 256).requires_grad_(), rnd(gen, 15, 256).requires_grad_()
+    y, best, val = torch.arange(72).cuda() % 15, torch.arange(72 * 5).view(72, 5).cuda() % 15, rnd(gen, 72, 5)
+
+    def step():
+        z = ho.linear_act(x, w)
+        r = ho.label_log_probs(z, y, top=3)
+        loss = ho.distill_top_k(z, best, val)
+        return (r.log_prob, r.top_index, loss, *torch.autograd.grad(loss.sum() - r.log_prob.sum() - r.entropy.sum(), (x, w)))
+    want = step()
+    timer = _ext.KernelTimer(pool=16)
+    monkeypatch.setattr(_ext, "TIMER", timer)
+    got = step()
+    monkeypatch.setattr(_ext, "TIMER", None)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    names = ["linear_act", "linear_act_grad", "label_logprobs", "label_logprobs_grad", "distill_topk", "distill_topk_grad"]
+    rows = timer.summary()
+    assert sorted(rows) == sorted("pn2_" + n for n in names) and all(r["calls"] == 1 and r["ms"] > 0 for r in rows.values())
+    assert rows["pn2_linear_act"]["alg_flops"] * 2 == rows["pn2_linear_act_grad"]["alg_flops"] == 4 * 72 * 15 * 256
+    assert rows["pn2_distill_topk"]["alg_bytes"] == 72 * 15 * 4
+
+
+@pytest.mark.parametrize("frozen", range(16))
+def test_linear_act_any_inputs_frozen(frozen):
+    """Each set of inputs that need a gradient: the gradients of all of them up to the order of their sums (which kernels run depends
+    on what is wanted), none for the others.  Both sides hold the same fp32 slopes and sum n <= 33 products of fp32: either is off by
+    at most n + 2 roundings of sum |term|, and |silu'| < 1.1."""
+    gen = torch.Generator().manual_seed(4)
+    ts = [rnd(gen, 33, 40), rnd(gen, 24, 40), rnd(gen, 24), rnd(gen, 33, 24)]
+    dy = rnd(gen, 33, 24)
+
+    def grads(off):
+        leaves = [t.clone().requires_grad_(not off >> i & 1) for i, t in enumerate(ts)]
+        y = ho.linear_act(leaves[0], leaves[1], leaves[2], "silu", leaves[3])
+        assert y.requires_grad == (off != 15)
+        if y.requires_grad:
+            y.backward(dy)
+        return [t.grad for t in leaves]
+    d = 1.1 * dy.abs()
+    terms = [d @ ts[1].abs(), d.t() @ ts[0].abs(), d.sum(0), torch.zeros_like(dy)]
+    for i, (a, b, t) in enumerate(zip(grads(0), grads(frozen), terms)):
+        assert b is None if frozen >> i & 1 else bool(((a - b).abs() <= 2 * 35 * U * t).all())
+
+
+def test_each_operator_is_differentiable_once():
+    gen = torch.Generator().manual_seed(6)
+    x, w, r = (t.requires_grad_() for t in (rnd(gen, 4, 8), rnd(gen, 8, 8), rnd(gen, 4, 8)))
+    y, best, val = torch.arange(4).cuda(), torch.arange(8).view(4, 2).cuda(), rnd(gen, 4, 2)
+    for out, leaf in ((ho.linear_act(x, w, None, "gelu", r), x), (ho.linear_act(x, w, None, "none", r), r),
+                      (ho.label_log_probs(x, y).log_prob, x), (ho.distill_top_k(x, best, val), x)):
+        g, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            g.sum().backward()
 
 
 # ------------------------------------------------------------------------------------------------- the model's own paths

@@ -54,6 +54,22 @@ def test_refusals(match, call):
         call()
 
 
+@pytest.mark.parametrize("match,call", [
+    ("x must be a torch.Tensor", lambda: ho.linear_act([1.0], f(4, 3))),
+    ("weight must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), None)),
+    ("bias must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), f(4, 3), 1.0)),
+    ("residual must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), f(4, 3), residual=0)),
+    ("labels must be a torch.Tensor", lambda: ho.label_log_probs(f(2, 3), [0, 1])),
+    ("teacher_logits must be a torch.Tensor", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), None)),
+    ("teacher_index must be a tensor of shape", lambda: ho.distill_top_k(f(3), torch.zeros(2, 2, dtype=torch.int64), f(2, 2))),
+    ("at most 4194304", lambda: ho.linear_act(f(1, 1).expand(1, 2 ** 22 + 1), f(1, 1).expand(1, 2 ** 22 + 1))),
+    ("residual must broadcast", lambda: ho.linear_act(f(2, 3), f(4, 3), residual=f(1, 2, 4))),
+])
+def test_refusals_of_other_objects_and_shapes(match, call):
+    with pytest.raises(RuntimeError, match=match):
+        call()
+
+
 def test_entry_points_refuse_bad_arguments_before_any_launch():
     """Every argument check of the C entry points returns its code on the host (the pointers are never followed)."""
     lib = _ext._lib
