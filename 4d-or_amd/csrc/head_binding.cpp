@@ -91,7 +91,7 @@ Tensor matrix(const Tensor &t, const char *name) {
   const int64_t c = t.size(-1);
   TORCH_CHECK(c >= 1, name, " must have at least one column");
   const Tensor m = t.dim() == 2 ? t : t.reshape({t.numel() / c, c});
-  return c == 1 || m.stride(1) == 1 ? m : m.contiguous();
+  return (c == 1 || m.stride(1) == 1 ? m : m.contiguous()).resolve_neg();
 }
 int64_t row_stride(const Tensor &m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
 
@@ -199,7 +199,7 @@ Tensor linear_act(const Tensor &x, const Tensor &weight, const std::optional<Ten
   const Tensor wm = matrix(weight, "weight");
   Tensor b, r;
   if (bias) {
-    b = *bias;
+    b = bias->resolve_neg();
     TORCH_CHECK(b.dim() == 1 && b.size(0) == N && b.is_contiguous(), "bias must be a contiguous tensor of shape (", N, ",)");
     TORCH_CHECK(b.scalar_type() == x.scalar_type() || b.scalar_type() == at::kFloat, "bias must have the type of x (", x.dtype(),
                 ") or float32");
@@ -244,7 +244,7 @@ Labels run_labels(const Tensor &x, const Tensor &y, int64_t top, int64_t ignore,
   return o;
 }
 Tensor grad_rows(const Tensor &g) {                    // the gradient of a row statistic, or undefined
-  return g.defined() ? g.contiguous() : g;
+  return g.defined() ? g.contiguous().resolve_neg() : g;
 }
 
 struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
@@ -368,7 +368,7 @@ Tensor distill_top_k(const Tensor &logits, const Tensor &teacher_index, const Te
   TORCH_CHECK(!teacher_logits.requires_grad(), "teacher_logits must not require a gradient (detach the teacher)");
   TORCH_CHECK(temperature > 0 && std::isfinite((float)temperature) && (float)temperature > 0, "temperature must be positive and finite");
   TORCH_CHECK(x.size(1) <= 0x7fffffff && x.size(0) <= 0x7fffffff, "logits must have fewer than 2^31 rows and columns");
-  const Tensor index = teacher_index.reshape({x.size(0), k}).contiguous(), values = teacher_logits.reshape({x.size(0), k}).contiguous();
+  const Tensor index = teacher_index.reshape({x.size(0), k}).contiguous(), values = teacher_logits.reshape({x.size(0), k}).contiguous().resolve_neg();
   check_device(x, {{&index, "teacher_index"}, {&values, "teacher_logits"}});
   Tensor loss = at::GradMode::is_enabled() && logits.requires_grad() ? DistillTopK::apply(x, index, values, temperature, timed)
                                                                      : run_distill(x, index, values, temperature, false, timed).first;

@@ -408,7 +408,7 @@ __device__ __forceinline__ void la_epilogue(const Product &a, const la_f32x4 (&a
 
 // ... -> the partial sums of a split contraction
 template <int TI, int TJ>
-__device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&acc)[TI][TJ], long long i, long long j) {
+__device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&acc)[TI][TJ], int split, long long i, long long j) {
   la_each<TI * TJ / 2>([&](auto n_) __attribute__((always_inline)) {
     constexpr int t = decltype(n_)::value / (TJ / 2), u = decltype(n_)::value % (TJ / 2) * 2;
     const long long row = i + t * 16, c = j + u * 16, left = row < a.M ? a.N - c : 0;
@@ -416,29 +416,29 @@ __device__ __forceinline__ void la_partial(const Product &a, const la_f32x4 (&ac
     float y[8];
 #pragma unroll
     for (int n = 0; n < 8; ++n) y[n] = acc[t][u + n / 4][n % 4];
-    la_store8<HdF32, false>(a.partial + ((long long)blockIdx.z * a.M + row) * a.N + c, left, y);
+    la_store8<HdF32, false>(a.partial + ((long long)split * a.M + row) * a.N + c, left, y);
   });
 }
 
+// workgroup `id` of a product's gi x gj tiles, part `split` of the contraction; ring: the LDS, 2 (BI + BJ) 128 bytes
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
-__global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int gi, int gj) {
+__device__ __forceinline__ void la_tile(const Product &a, int gi, int gj, int id, int split, char *ring) {
   constexpr int NT = 64 * WI * WJ, BI = WI * TI * 16, BJ = WJ * TJ * 16, KB = 8 * T::kPerVec, SLOT = (BI + BJ) * 128;
   typedef Operand<T, PROWS, false, BI, NT> OP;
   typedef Operand<T, QROWS, true, BJ, NT> OQ;
-  __shared__ __align__(1024) char ring[2 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups go round robin over the 8 XCDs: give each XCD a contiguous run of tiles, walked in bands of 8 tile rows, so that the
   // operand panels of a band are shared in its L2
   int ti, tj;
   {
-    const int n = gi * gj, id = blockIdx.x, per = n / 8, rem = n % 8, x = id % 8, q = id / 8;
+    const int n = gi * gj, per = n / 8, rem = n % 8, x = id % 8, q = id / 8;
     const int at = x * per + (x < rem ? x : rem) + q;
     const int band = at / (8 * gj), rows = gi - band * 8 < 8 ? gi - band * 8 : 8, in = at - band * 8 * gj;
     ti = band * 8 + in % rows;
     tj = in / rows;
   }
   const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
-  const long long k0 = (long long)blockIdx.z * a.kchunk, k1 = k0 + a.kchunk < a.K ? k0 + a.kchunk : a.K;
+  const long long k0 = (long long)split * a.kchunk, k1 = k0 + a.kchunk < a.K ? k0 + a.kchunk : a.K;
   const int tiles = (int)((k1 - k0) / KB), rest = (int)((k1 - k0) % KB);
   const int wi = (wave % WI) * TI * 16, wj = (wave / WI) * TJ * 16;
   constexpr int L = OP::PER + OQ::PER;                 // direct loads per wave and tile
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
     if (rest > KB / 2) half(LaInt<1>{});
   }
   const long long i = i0 + wi + (lane & 15), j = j0 + wj + (lane >> 4) * 8;
-  if (a.splits > 1) la_partial(a, acc, i, j);
+  if (a.splits > 1) la_partial(a, acc, split, i, j);
   else if (i0 + BI > a.M || j0 + BJ > a.N) {
     if (a.e.res) la_epilogue<T, ACT, false, true>(a, acc, i, j);
     else la_epilogue<T, ACT, false, false>(a, acc, i, j);
@@ -532,6 +532,12 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
     if (a.e.res) la_epilogue<T, ACT, true, true>(a, acc, i, j);
     else la_epilogue<T, ACT, true, false>(a, acc, i, j);
   }
+}
+
+template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int gi, int gj) {
+  __shared__ __align__(1024) char ring[2 * (WI * TI + WJ * TJ) * 16 * 128];
+  la_tile<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT>(a, gi, gj, blockIdx.x, blockIdx.z, ring);
 }
 
 // the split contraction joined in a fixed order, then the epilogue: four consecutive results per thread
@@ -567,13 +573,17 @@ struct Copy {
   const void *src;
   void *dst;
 };
-// both operands of a product in one launch: the first `first` workgroups copy a, the others b
+// both operands of a product in one launch: the first `blocks` workgroups copy a, the others b
+struct Copies {
+  Copy a, b;
+  unsigned blocks, all;
+};
 template <class T>
-__global__ __launch_bounds__(256) void la_pad_kernel(Copy a, Copy b, unsigned first) {
+__device__ __forceinline__ void la_pad(const Copies &c_, unsigned id) {
   typedef typename T::elem elem;
   constexpr int VE = T::kPerVec;
-  const Copy &o = blockIdx.x < first ? a : b;
-  const long long pieces = o.to / VE, at = (long long)(blockIdx.x < first ? blockIdx.x : blockIdx.x - first) * 256 + threadIdx.x;
+  const Copy &o = id < c_.blocks ? c_.a : c_.b;
+  const long long pieces = o.to / VE, at = (long long)(id < c_.blocks ? id : id - c_.blocks) * 256 + threadIdx.x;
   if (at >= o.rows * pieces) return;
   const long long r = at / pieces, c = (at - r * pieces) * VE;
   const elem *src = (const elem *)o.src + r * o.ld + c;
@@ -585,6 +595,11 @@ __global__ __launch_bounds__(256) void la_pad_kernel(Copy a, Copy b, unsigned fi
     for (int n = 0; n < VE; ++n) f[n] = c + n < o.cols ? T::load(src + n) : 0.f;
     hd_store16<T>((elem *)o.dst + r * o.to + c, T::pack(f));
   }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void la_pad_kernel(Copies c) {
+  la_pad<T>(c, blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------------- the small kernels
@@ -776,17 +791,23 @@ __global__ __launch_bounds__(256) void la_small_grad_kernel(Small x, Small w, in
 }
 
 // dz = dy slope (or dy, SLOPE false) at row stride ldz, or NULL, and column sums: a workgroup takes 64 x VE columns and a strip of rows, its four
-// waves every fourth row; part (strips, N) fp32, or NULL.  Bound by its bytes (read dy and slope, write dz).
+// waves every fourth row; part (strips, N) fp32, or NULL.  Bound by its bytes (read dy and slope, write dz).  The workgroups behind
+// those `blocks` make the padded copies that the products need.
 template <class T, bool SLOPE>
 __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, int strip, const void *dy_, long long ldy,
-                                                    const void *slope_, void *dz_, long long ldz, float *part) {
+                                                    const void *slope_, void *dz_, long long ldz, float *part, unsigned blocks, Copies copies) {
+  if (blockIdx.x >= blocks) {
+    la_pad<T>(copies, blockIdx.x - blocks);
+    return;
+  }
   typedef typename T::elem elem;
   typedef typename SlopeOf<T>::type S;
   constexpr int VE = T::kPerVec, U = 4;
   __shared__ float sum[3][64][VE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long j = ((long long)blockIdx.x * 64 + lane) * VE, left = N - j;
-  const long long i0 = (long long)blockIdx.y * strip, i1 = i0 + strip < M ? i0 + strip : M;
+  const unsigned across = (unsigned)((N + 64 * VE - 1) / (64 * VE)), down = blockIdx.x / across;
+  const long long j = ((long long)(blockIdx.x - down * across) * 64 + lane) * VE, left = N - j;
+  const long long i0 = (long long)down * strip, i1 = i0 + strip < M ? i0 + strip : M;
   float s[VE];
 #pragma unroll
   for (int n = 0; n < VE; ++n) s[n] = 0.f;
@@ -840,25 +861,46 @@ __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, in
   if (wave == 0) {
 #pragma unroll
     for (int n = 0; n < VE; ++n)
-      if (n < left) part[(long long)blockIdx.y * N + j + n] = (s[n] + sum[0][lane][n]) + (sum[1][lane][n] + sum[2][lane][n]);
+      if (n < left) part[(long long)down * N + j + n] = (s[n] + sum[0][lane][n]) + (sum[1][lane][n] + sum[2][lane][n]);
   }
 }
 
 // the strips' sums joined: 64 columns per workgroup, its four waves every fourth strip
+struct Sums {
+  const float *part;
+  long long N;
+  int strips, db_f32;
+  void *db;
+};
 template <class T>
-__global__ __launch_bounds__(256) void la_db_kernel(long long N, int strips, const float *part, void *db, int db_f32) {
-  __shared__ float sum[3][64];
+__device__ __forceinline__ void la_db(const Sums &a, unsigned id, float (*sum)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long j = (long long)blockIdx.x * 64 + lane;
+  const long long j = (long long)id * 64 + lane;
   float s = 0.f;
-  if (j < N)
-    for (int i = wave; i < strips; i += 4) s += part[(long long)i * N + j];
+  if (j < a.N)
+    for (int i = wave; i < a.strips; i += 4) s += a.part[(long long)i * a.N + j];
   if (wave) sum[wave - 1][lane] = s;
   __syncthreads();
-  if (wave || j >= N) return;
+  if (wave || j >= a.N) return;
   s = (s + sum[0][lane]) + (sum[1][lane] + sum[2][lane]);
-  if (db_f32) ((float *)db)[j] = s;
-  else ((typename T::elem *)db)[j] = T::round(s);
+  if (a.db_f32) ((float *)a.db)[j] = s;
+  else ((typename T::elem *)a.db)[j] = T::round(s);
+}
+template <class T>
+__global__ __launch_bounds__(256) void la_db_kernel(Sums a) {
+  __shared__ float sum[3][64];
+  la_db<T>(a, blockIdx.x, sum);
+}
+
+// dx, dW and db of a layer in the middle in one launch, on 64 x 64 tiles: `nx` workgroups for dx, `nw` for dW, the others for db.  Each
+// of the products alone leaves the chip half idle and takes as long as its own loop.
+template <class T>
+__global__ __launch_bounds__(256, 2) void la_pair_kernel(Product x, int xi, int xj, Product w, int wi, int wj, Sums b) {
+  __shared__ __align__(1024) char ring[2 * 128 * 128];
+  const int id = blockIdx.x, nx = xi * xj, nw = wi * wj;
+  if (id < nx) la_tile<T, false, true, 2, 2, 2, 2, ACT_NONE>(x, xi, xj, id, 0, ring);
+  else if (id < nx + nw) la_tile<T, true, true, 2, 2, 2, 2, ACT_NONE>(w, wi, wj, id - nx, 0, ring);
+  else la_db<T>(b, id - nx - nw, (float (*)[64])ring);
 }
 
 constexpr long long kMaxDim = 1LL << 31, kMaxStride = 1LL << 22;
@@ -936,23 +978,24 @@ struct Space {              // the caller's workspace, handed out piece by piece
   }
 };
 
-// those of a and b that need it become padded copies (b may be NULL)
+// those of a and b that need it become padded copies (either may be NULL), which a kernel has yet to make
 template <class T>
-void la_pad(Matrix *a, Matrix *b, int dtype, Space &ws, hipStream_t st) {
-  Copy job[2] = {};
-  unsigned blocks[2] = {0, 0};
+Copies la_copies(Matrix *a, Matrix *b, int dtype, Space &ws) {
+  Copies c{};
   for (int n = 0; n < 2; ++n) {
     Matrix *o = n ? b : a;
     const size_t bytes = o ? la_copy_bytes(*o, dtype) : 0;
-    if (!bytes) continue;
-    const long long to = la_whole(o->cols, dtype);
-    job[n] = {o->rows, o->cols, o->ld, to, o->p, ws.take(bytes)};
-    blocks[n] = (unsigned)la_div(o->rows * (to / T::kPerVec), 256);
-    o->p = job[n].dst;
-    o->ld = to;
-    if (o->R) o->cols = to;
+    if (bytes) {
+      const long long to = la_whole(o->cols, dtype);
+      (n ? c.b : c.a) = {o->rows, o->cols, o->ld, to, o->p, ws.take(bytes)};
+      c.all += (unsigned)la_div(o->rows * (to / T::kPerVec), 256);
+      o->p = (n ? c.b : c.a).dst;
+      o->ld = to;
+      if (o->R) o->cols = to;
+    }
+    if (!n) c.blocks = c.all;
   }
-  if (blocks[0] + blocks[1]) la_pad_kernel<T><<<blocks[0] + blocks[1], 256, 0, st>>>(job[0], job[1], blocks[0]);
+  return c;
 }
 
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
@@ -979,18 +1022,23 @@ void la_small_as(const Product &a, hipStream_t st) {
   la_small_kernel<T, TI, TJ, W><<<(unsigned)(la_div(a.M, 16 * TI) * la_div(a.N, 16 * TJ)), 64 * W, 0, st>>>(a);
 }
 
-// C = P Q^T by the plan; P and Q are fit for it (padded where a tile kernel reads them)
-template <class T, bool PROWS, bool QROWS>
-int la_product(const Plan &plan, const Matrix &p, const Matrix &q, long long M, long long N, long long K, const Epilogue &e,
-               Space ws, hipStream_t st) {
+Product la_arguments(const Plan &plan, const Matrix &p, const Matrix &q, long long M, long long N, long long K, const Epilogue &e, Space ws) {
   Product a{};
   a.M = M; a.N = N; a.K = K;
-  a.p = p.p; a.ldp = p.ld; a.rp = PROWS ? p.cols : p.rows;
-  a.q = q.p; a.ldq = q.ld; a.rq = QROWS ? q.cols : q.rows;
+  a.p = p.p; a.ldp = p.ld; a.rp = p.R ? p.cols : p.rows;
+  a.q = q.p; a.ldq = q.ld; a.rq = q.R ? q.cols : q.rows;
   a.splits = plan.splits;
   a.kchunk = plan.kchunk;
   a.partial = (float *)ws.take(la_partial_bytes(plan, M, N));
   a.e = e;
+  return a;
+}
+
+// C = P Q^T by the plan; P and Q are fit for it (padded where a tile kernel reads them)
+template <class T, bool PROWS, bool QROWS>
+int la_product(const Plan &plan, const Matrix &p, const Matrix &q, long long M, long long N, long long K, const Epilogue &e,
+               Space ws, hipStream_t st) {
+  const Product a = la_arguments(plan, p, q, M, N, K, e, ws);
   switch (plan.kernel) {
     case TILE_256:
       if constexpr (sizeof(typename T::elem) == 2) { la_tile_as<T, PROWS, QROWS, 2, 4, 8, 4>(a, st); break; }
@@ -1032,7 +1080,8 @@ template <class T>
 int la_forward(Forward f, long long M, long long N, long long K, int dtype, const Epilogue &e, void *ws, hipStream_t st) {
   Space space{(char *)ws};
   if (f.plan.kernel >= TILE_64) {
-    la_pad<T>(&f.x, &f.w, dtype, space, st);
+    const Copies c = la_copies<T>(&f.x, &f.w, dtype, space);
+    if (c.all) la_pad_kernel<T><<<c.all, 256, 0, st>>>(c);
   }
   return la_product<T, false, false>(f.plan, f.x, f.w, M, N, K, e, space, st);
 }
@@ -1049,7 +1098,7 @@ inline int la_strip(long long M, long long N, int dtype) {
 // The backward pass: one launch where everything is small (contractions of at most 2048 and 4096, 2^27 products: 512^3 10 us against 27
 // for the launches of the general path, whose launches a host thread also has to make), otherwise dz and db's strips, dx, dW.
 struct Backward {
-  bool small, own_dz;       // own_dz: dz is written (it is not dy itself)
+  bool small, pair, own_dz;  // own_dz: dz is written (it is not dy itself)
   Plan px, pw;
   Matrix dz, dzr, w, x;   // dz as the K operand of dx and as the R operand of dW
   size_t dz_bytes, part, bytes;
@@ -1069,6 +1118,7 @@ Backward la_backward_plan(long long M, long long N, long long K, int dtype, cons
   b.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
   b.px = la_plan(M, K, N, dtype, false);
   b.pw = la_plan(N, K, M, dtype, false);
+  b.pair = (want & 3) == 3 && b.px.kernel == TILE_64 && b.pw.kernel == TILE_64 && b.px.splits == 1 && b.pw.splits == 1;
   const size_t copies = ((want & 1) ? la_copy_bytes(b.w, dtype) : 0) + ((want & 2) ? la_copy_bytes(b.x, dtype) : 0);
   // the two products use the rest one after the other
   const size_t dx = (want & 1) ? la_partial_bytes(b.px, M, K) : 0, dw = (want & 2) ? la_partial_bytes(b.pw, N, K) : 0;
@@ -1092,31 +1142,35 @@ int la_backward(Backward b, long long M, long long N, long long K, int dtype, co
   void *dz = space.take(b.dz_bytes);
   float *part = (float *)space.take(b.part);
   const long long ldz = la_whole(N, dtype);
+  const Copies c = la_copies<T>(dx ? &b.w : nullptr, dw ? &b.x : nullptr, dtype, space);
+  const int strip = la_strip(M, N, dtype);
+  const Sums sums{part, N, (int)la_div(M, strip), db_f32, db};
   if (b.own_dz || db) {
-    const int strip = la_strip(M, N, dtype), strips = (int)la_div(M, strip);
-    const dim3 grid((unsigned)la_div(N, 64 * T::kPerVec), (unsigned)strips);
-    if (slope) la_dz_kernel<T, true><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, ldz, part);
-    else la_dz_kernel<T, false><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, dz, ldz, part);
-    if (db) la_db_kernel<T><<<(unsigned)la_div(N, 64), 256, 0, st>>>(N, strips, part, db, db_f32);
-    const int rc = pn2_check_launch();
-    if (rc != PN2_OK) return rc;
+    const unsigned blocks = (unsigned)(la_div(N, 64 * T::kPerVec) * sums.strips);
+    if (slope) la_dz_kernel<T, true><<<blocks + c.all, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, ldz, part, blocks, c);
+    else la_dz_kernel<T, false><<<blocks + c.all, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, dz, ldz, part, blocks, c);
+  } else if (c.all) {
+    la_pad_kernel<T><<<c.all, 256, 0, st>>>(c);
   }
   if (b.own_dz) {
     b.dz.p = b.dzr.p = dz;
     b.dz.ld = b.dzr.ld = b.dzr.cols = ldz;
   }
-  la_pad<T>(dx ? &b.w : nullptr, dw ? &b.x : nullptr, dtype, space, st);
-  Epilogue e{};
-  if (dx) {
-    e.y = dx;
-    const int rc = la_product<T, false, true>(b.px, b.dz, b.w, M, K, N, e, space, st);
-    if (rc != PN2_OK) return rc;
+  const unsigned joins = db ? (unsigned)la_div(N, 64) : 0;
+  Epilogue ex{}, ew{};
+  ex.y = dx;
+  ew.y = dw;
+  if (b.pair) {
+    const int xi = (int)la_div(M, 64), xj = (int)la_div(K, 64), wi = (int)la_div(N, 64);
+    la_pair_kernel<T><<<(unsigned)(xi * xj + wi * xj) + joins, 256, 0, st>>>(la_arguments(b.px, b.dz, b.w, M, K, N, ex, space), xi, xj,
+                                                                          la_arguments(b.pw, b.dzr, b.x, N, K, M, ew, space), wi, xj, sums);
+    return pn2_check_launch();
   }
-  if (dw) {
-    e.y = dw;
-    return la_product<T, true, true>(b.pw, b.dzr, b.x, N, K, M, e, space, st);
-  }
-  return PN2_OK;
+  if (db) la_db_kernel<T><<<joins, 256, 0, st>>>(sums);
+  int rc = pn2_check_launch();
+  if (rc == PN2_OK && dx) rc = la_product<T, false, true>(b.px, b.dz, b.w, M, K, N, ex, space, st);
+  if (rc == PN2_OK && dw) rc = la_product<T, true, true>(b.pw, b.dzr, b.x, N, K, M, ew, space, st);
+  return rc;
 }
 
 }  // namespace
