@@ -540,10 +540,12 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int
   la_tile<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT>(a, gi, gj, blockIdx.x, blockIdx.z, ring);
 }
 
-// the split contraction joined in a fixed order, then the epilogue: four consecutive results per thread
+// the split contraction joined in a fixed order, then the epilogue: four consecutive results per thread; the first `blocks`
+// workgroups join x, the others w
 template <class T>
-__global__ __launch_bounds__(256) void la_join_kernel(Product a) {
-  const long long n = a.M * a.N, at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256) void la_join_kernel(Product x, Product w, unsigned blocks) {
+  const Product &a = blockIdx.x < blocks ? x : w;
+  const long long n = a.M * a.N, at = ((long long)(blockIdx.x < blocks ? blockIdx.x : blockIdx.x - blocks) * 256 + threadIdx.x) * 4;
   if (at >= n) return;
   float z[4] = {0.f, 0.f, 0.f, 0.f};
   if (at + 4 <= n) {
@@ -874,11 +876,18 @@ struct Sums {
 };
 template <class T>
 __device__ __forceinline__ void la_db(const Sums &a, unsigned id, float (*sum)[64]) {
+  constexpr int U = 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long j = (long long)id * 64 + lane;
   float s = 0.f;
   if (j < a.N)
-    for (int i = wave; i < a.strips; i += 4) s += a.part[(long long)i * a.N + j];
+    for (int i = wave; i < a.strips; i += 4 * U) {     // a wave's round trips are what this costs: 128 strips each, 34 us one by one
+      float f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = a.part[(long long)(i + 4 * u < a.strips ? i + 4 * u : i) * a.N + j];
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += i + 4 * u < a.strips ? f[u] : 0.f;
+    }
   if (wave) sum[wave - 1][lane] = s;
   __syncthreads();
   if (wave || j >= a.N) return;
@@ -897,9 +906,9 @@ __global__ __launch_bounds__(256) void la_db_kernel(Sums a) {
 template <class T>
 __global__ __launch_bounds__(256, 2) void la_pair_kernel(Product x, int xi, int xj, Product w, int wi, int wj, Sums b) {
   __shared__ __align__(1024) char ring[2 * 128 * 128];
-  const int id = blockIdx.x, nx = xi * xj, nw = wi * wj;
-  if (id < nx) la_tile<T, false, true, 2, 2, 2, 2, ACT_NONE>(x, xi, xj, id, 0, ring);
-  else if (id < nx + nw) la_tile<T, true, true, 2, 2, 2, 2, ACT_NONE>(w, wi, wj, id - nx, 0, ring);
+  const int tx = xi * xj, tw = wi * wj, nx = tx * x.splits, nw = tw * w.splits, id = blockIdx.x;
+  if (id < nx) la_tile<T, false, true, 2, 2, 2, 2, ACT_NONE>(x, xi, xj, id % tx, id / tx, ring);
+  else if (id < nx + nw) la_tile<T, true, true, 2, 2, 2, 2, ACT_NONE>(w, wi, wj, (id - nx) % tw, (id - nx) / tw, ring);
   else la_db<T>(b, id - nx - nw, (float (*)[64])ring);
 }
 
@@ -998,6 +1007,8 @@ Copies la_copies(Matrix *a, Matrix *b, int dtype, Space &ws) {
   return c;
 }
 
+inline unsigned la_joins(const Product &a) { return a.splits > 1 ? (unsigned)la_div(a.M * a.N, 1024) : 0; }
+
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
 void la_tile_as(const Product &a, hipStream_t st) {
   const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
@@ -1014,7 +1025,7 @@ void la_tile_as(const Product &a, hipStream_t st) {
       default: la_tile_kernel<T, false, false, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
     }
   }
-  if (a.splits > 1) la_join_kernel<T><<<(unsigned)la_div(a.M * a.N, 1024), 256, 0, st>>>(a);
+  if (a.splits > 1) la_join_kernel<T><<<la_joins(a), 256, 0, st>>>(a, a, la_joins(a));
 }
 
 template <class T, int TI, int TJ, int W>
@@ -1095,8 +1106,11 @@ inline int la_strip(long long M, long long N, int dtype) {
   return (int)(s < 16 ? 16 : s);
 }
 
-// The backward pass: one launch where everything is small (contractions of at most 2048 and 4096, 2^27 products: 512^3 10 us against 27
-// for the launches of the general path, whose launches a host thread also has to make), otherwise dz and db's strips, dx, dW.
+// The backward pass: one launch where everything is small (contractions of at most 2048 and 4096); otherwise dz, db's strips and padded
+// copies, then dx, dW and db: at once on 64 x 64 tiles, one after the other on larger ones.  Forward and backward in a graph, one launch
+// against the others: fp32 up to 2^27 products (512^3 23 against 29 us, 1000 x 512 -> 256 31 against 42); 16-bit types, whose operands
+// in row order the small kernel reads value by value, up to 2^24 (72 x 256 -> 512 13.6 against 13.3, and two launches fewer for the
+// host; 512^3 18 against 16, 1000 x 512 -> 256 38 against 19).
 struct Backward {
   bool small, pair, own_dz;  // own_dz: dz is written (it is not dy itself)
   Plan px, pw;
@@ -1106,7 +1120,7 @@ struct Backward {
 Backward la_backward_plan(long long M, long long N, long long K, int dtype, const void *dy, long long ldy, bool slope, const void *x,
                           long long ldx, const void *w, long long ldw, int want) {
   Backward b{};
-  b.small = (double)M * N * K <= (double)(1 << 27) && M <= 2048 && N <= 4096 && (want & 3) && !((want & 4) && !(want & 2));
+  b.small = (double)M * N * K <= (double)(1 << (dtype == PN2_DT_F32 ? 27 : 24)) && M <= 2048 && N <= 4096 && (want & 3) && !((want & 4) && !(want & 2));
   if (b.small) return b;
   const bool products = (want & 3) != 0;
   b.dz = {dy, M, N, ldy, false};
@@ -1118,11 +1132,11 @@ Backward la_backward_plan(long long M, long long N, long long K, int dtype, cons
   b.part = (want & 4) ? la_align((size_t)la_div(M, la_strip(M, N, dtype)) * N * 4) : 0;
   b.px = la_plan(M, K, N, dtype, false);
   b.pw = la_plan(N, K, M, dtype, false);
-  b.pair = (want & 3) == 3 && b.px.kernel == TILE_64 && b.pw.kernel == TILE_64 && b.px.splits == 1 && b.pw.splits == 1;
+  b.pair = (want & 3) == 3 && b.px.kernel == TILE_64 && b.pw.kernel == TILE_64;
   const size_t copies = ((want & 1) ? la_copy_bytes(b.w, dtype) : 0) + ((want & 2) ? la_copy_bytes(b.x, dtype) : 0);
-  // the two products use the rest one after the other
+  // the two products use the rest one after the other, or at once
   const size_t dx = (want & 1) ? la_partial_bytes(b.px, M, K) : 0, dw = (want & 2) ? la_partial_bytes(b.pw, N, K) : 0;
-  b.bytes = b.dz_bytes + b.part + copies + (dx > dw ? dx : dw);
+  b.bytes = b.dz_bytes + b.part + copies + (b.pair ? dx + dw : dx > dw ? dx : dw);
   return b;
 }
 
@@ -1162,8 +1176,11 @@ int la_backward(Backward b, long long M, long long N, long long K, int dtype, co
   ew.y = dw;
   if (b.pair) {
     const int xi = (int)la_div(M, 64), xj = (int)la_div(K, 64), wi = (int)la_div(N, 64);
-    la_pair_kernel<T><<<(unsigned)(xi * xj + wi * xj) + joins, 256, 0, st>>>(la_arguments(b.px, b.dz, b.w, M, K, N, ex, space), xi, xj,
-                                                                          la_arguments(b.pw, b.dzr, b.x, N, K, M, ew, space), wi, xj, sums);
+    const Product px = la_arguments(b.px, b.dz, b.w, M, K, N, ex, space);
+    space.take(la_partial_bytes(b.px, M, K));
+    const Product pw = la_arguments(b.pw, b.dzr, b.x, N, K, M, ew, space);
+    la_pair_kernel<T><<<(unsigned)(xi * xj * px.splits + wi * xj * pw.splits) + joins, 256, 0, st>>>(px, xi, xj, pw, wi, xj, sums);
+    if (la_joins(px) + la_joins(pw)) la_join_kernel<T><<<la_joins(px) + la_joins(pw), 256, 0, st>>>(px, pw, la_joins(px));
     return pn2_check_launch();
   }
   if (db) la_db_kernel<T><<<joins, 256, 0, st>>>(sums);

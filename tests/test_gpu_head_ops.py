@@ -699,6 +699,43 @@ def test_linear_act_any_inputs_frozen(frozen):
         assert b is None if frozen >> i & 1 else bool(((a - b).abs() <= 2 * 35 * U * t).all())
 
 
+@pytest.mark.parametrize("frozen", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("M,N,K", [(300, 136, 520), (2051, 72, 190), (4100, 264, 33)])
+def test_linear_act_products_at_once_and_alone(M, N, K, frozen):
+    """fp16 layers of the general route: with everything wanted dx, dW and db are one launch, otherwise each has its own.  The same dz
+    and n products on both sides: sums off by n + 2 roundings of sum |term| each, results by one more rounding each."""
+    gen = torch.Generator().manual_seed(7)
+    ts = [rnd(gen, M, K, dtype=torch.float16), rnd(gen, N, K, scale=0.1, dtype=torch.float16), rnd(gen, N)]
+    dy = rnd(gen, M, N, dtype=torch.float16)
+
+    def grads(off):
+        leaves = [t.clone().requires_grad_(not off >> i & 1) for i, t in enumerate(ts)]
+        ho.linear_act(*leaves, "gelu").backward(dy)
+        return [t.grad for t in leaves]
+    d, x, w = 1.2 * dy.float().abs(), ts[0].float().abs(), ts[1].float().abs()
+    terms = [((N + 2) * U, d @ w), ((M + 2) * U, d.t() @ x), ((M + 2) * U, d.sum(0))]
+    for i, (a, b, (u, t)) in enumerate(zip(grads(0), grads(frozen), terms)):
+        assert (b is None) == bool(frozen >> i & 1)
+        if b is not None:
+            tol = 2 * u * t + 2 * half(a.dtype) * (a.float().abs() + u * t) + tiny(a.dtype)
+            assert bool(((a.float() - b.float()).abs() <= tol).all())
+
+
+def test_views_with_the_negative_bit():
+    gen = torch.Generator().manual_seed(8)
+    z = torch.complex(rnd(gen, 9, 1), rnd(gen, 9, 1))
+    x, w = z.conj().imag, rnd(gen, 5, 1)
+    assert x.is_neg()
+    assert torch.equal(ho.linear_act(x, w), ho.linear_act(x.clone().resolve_neg(), w))
+    z = torch.complex(rnd(gen, 4, 6), rnd(gen, 4, 6))
+    x, y, best = z.conj().imag, torch.arange(4).cuda(), torch.arange(8).view(4, 2).cuda()
+    assert torch.equal(ho.label_log_probs(x, y).log_prob, ho.label_log_probs(-z.imag.contiguous(), y).log_prob)
+    v = torch.complex(rnd(gen, 4, 2), rnd(gen, 4, 2))
+    # (the last row's indices lie outside the columns: NaN on both sides)
+    torch.testing.assert_close(ho.distill_top_k(x, best, v.conj().imag),
+                               ho.distill_top_k(-z.imag.contiguous(), best, -v.imag.contiguous()), rtol=0, atol=0, equal_nan=True)
+
+
 def test_each_operator_is_differentiable_once():
     gen = torch.Generator().manual_seed(6)
     x, w, r = (t.requires_grad_() for t in (rnd(gen, 4, 8), rnd(gen, 8, 8), rnd(gen, 4, 8)))
