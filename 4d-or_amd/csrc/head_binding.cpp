@@ -29,8 +29,10 @@ struct {
   decltype(&pn2_linear_act) linear;
   decltype(&pn2_linear_act_grad_workspace_bytes) linear_grad_bytes;
   decltype(&pn2_linear_act_grad) linear_grad;
+  decltype(&pn2_label_logprobs_workspace_bytes) labels_bytes;
   decltype(&pn2_label_logprobs) labels;
   decltype(&pn2_label_logprobs_grad) labels_grad;
+  decltype(&pn2_distill_topk_workspace_bytes) distill_bytes;
   decltype(&pn2_distill_topk) distill;
   decltype(&pn2_distill_topk_grad) distill_grad;
   decltype(&pn2_strerror) strerror;
@@ -45,8 +47,10 @@ void bind(const py::function &address, py::object timed) {
   take(lib.linear, "pn2_linear_act");
   take(lib.linear_grad_bytes, "pn2_linear_act_grad_workspace_bytes");
   take(lib.linear_grad, "pn2_linear_act_grad");
+  take(lib.labels_bytes, "pn2_label_logprobs_workspace_bytes");
   take(lib.labels, "pn2_label_logprobs");
   take(lib.labels_grad, "pn2_label_logprobs_grad");
+  take(lib.distill_bytes, "pn2_distill_topk_workspace_bytes");
   take(lib.distill, "pn2_distill_topk");
   take(lib.distill_grad, "pn2_distill_topk_grad");
   take(lib.strerror, "pn2_strerror");
@@ -235,12 +239,15 @@ Labels run_labels(const Tensor &x, const Tensor &y, int64_t top, int64_t ignore,
     o.top_index = at::empty({T, top}, x.options().dtype(at::kLong));
   }
   if (want_stats) o.stats = at::empty({T, 2}, f32);
-  if (T)
-    launch("pn2_label_logprobs", x, timed, (double)T * V * x.element_size() + T * (16.0 + 12.0 * top), 0, [&](void *stream) {
-      return lib.labels(T, (int)V, row_stride(x), dtype_code(x, "logits"), x.data_ptr(), ptr_as<long long>(y), ignore, (int)top,
-                        ptr_as<float>(o.log_prob), ptr_as<float>(o.entropy), ptr_as<float>(o.stats), ptr_as<float>(o.top_log_prob),
-                        ptr_as<long long>(o.top_index), stream);
-    });
+  if (T == 0) return o;
+  const int dt = dtype_code(x, "logits");
+  const size_t bytes = lib.labels_bytes(T, (int)V, dt, (int)top);
+  const Tensor ws = workspace(bytes, x);
+  launch("pn2_label_logprobs", x, timed, (double)T * V * x.element_size() + T * (16.0 + 12.0 * top), 0, [&](void *stream) {
+    return lib.labels(T, (int)V, row_stride(x), dt, x.data_ptr(), ptr_as<long long>(y), ignore, (int)top, ptr_as<float>(o.log_prob),
+                      ptr_as<float>(o.entropy), ptr_as<float>(o.stats), ptr_as<float>(o.top_log_prob), ptr_as<long long>(o.top_index),
+                      ptr(ws), bytes, stream);
+  });
   return o;
 }
 Tensor grad_rows(const Tensor &g) {                    // the gradient of a row statistic, or undefined
@@ -322,11 +329,15 @@ std::pair<Tensor, Tensor> run_distill(const Tensor &x, const Tensor &index, cons
   const auto f32 = x.options().dtype(at::kFloat);
   Tensor loss = at::empty({T}, f32), stats;
   if (want_stats) stats = at::empty({T, 4}, f32);
-  if (T)
-    launch("pn2_distill_topk", x, timed, (double)T * V * x.element_size(), 0, [&](void *stream) {
-      return lib.distill(T, (int)V, row_stride(x), dtype_code(x, "logits"), x.data_ptr(), (int)index.size(1), ptr_as<long long>(index),
-                         dtype_code(values, "teacher_logits"), values.data_ptr(), (float)t, ptr_as<float>(loss), ptr_as<float>(stats), stream);
-    });
+  if (T == 0) return {loss, stats};
+  const int dt = dtype_code(x, "logits");
+  const size_t bytes = lib.distill_bytes(T, (int)V, dt);
+  const Tensor ws = workspace(bytes, x);
+  launch("pn2_distill_topk", x, timed, (double)T * V * x.element_size(), 0, [&](void *stream) {
+    return lib.distill(T, (int)V, row_stride(x), dt, x.data_ptr(), (int)index.size(1), ptr_as<long long>(index),
+                       dtype_code(values, "teacher_logits"), values.data_ptr(), (float)t, ptr_as<float>(loss), ptr_as<float>(stats),
+                       ptr(ws), bytes, stream);
+  });
   return {loss, stats};
 }
 

@@ -118,6 +118,9 @@ struct FwdArgs {
   const void *t_val;
   int t_dtype;
   float *loss;
+  int nseg, seg;                   // a row in nseg segments of seg entries (the last one shorter): their sums (T, nseg, 4), the keys
+  float *part;                     // of threads (T, nseg, 256)
+  u64 *keys;
 };
 
 __device__ __forceinline__ float lp_teacher(const FwdArgs &a, long long at) {
@@ -212,6 +215,12 @@ __device__ __forceinline__ void lp_finish_distill(const FwdArgs &a, long long ro
 }
 
 enum { MODE_LABEL, MODE_DISTILL };
+
+// alternative `slot` of a row, should no entry take it
+__device__ __forceinline__ void lp_clear(const FwdArgs &a, long long row, int slot, const RowStat &st) {
+  a.top_lp[row * a.top + slot] = st.nan ? __builtin_nanf("") : -kHdInf;
+  a.top_idx[row * a.top + slot] = -1;
+}
 
 // one of the n candidates in LDS takes the place its rank gives it
 __device__ __forceinline__ void lp_place(const FwdArgs &a, long long row, const u64 *cand, int n, u64 mine, const RowStat &st) {
@@ -313,56 +322,186 @@ __global__ __launch_bounds__(256) void lp_small_kernel(FwdArgs a) {
 // --------------------------------------------------------------------------------------------- V > 2048: a workgroup per row
 constexpr int kCand = 1024;              // elements kept in LDS for the final ranking
 
-template <class T, int MODE, bool TOP, int BT, int U>
+// a row (or a segment of one) in vectors of 16 bytes; what lies behind its end reads as -inf
+template <class T>
+struct Vectors {
+  const typename T::elem *x;
+  int nfull, tail, nvec;
+  __device__ __forceinline__ Vectors(const typename T::elem *x_, int V) : x(x_), nfull(V / T::kPerVec), tail(V % T::kPerVec) {
+    nvec = nfull + (tail != 0);
+  }
+  __device__ __forceinline__ hd_u32x4 nothing() const {
+    float g[T::kPerVec];
+#pragma unroll
+    for (int j = 0; j < T::kPerVec; ++j) g[j] = -kHdInf;
+    return T::pack(g);
+  }
+  // the last, partial vector
+  __device__ __forceinline__ hd_u32x4 last() const {
+    float g[T::kPerVec];
+#pragma unroll
+    for (int j = 0; j < T::kPerVec; ++j) g[j] = j < tail ? T::load(x + (long long)nfull * T::kPerVec + j) : -kHdInf;
+    return T::pack(g);
+  }
+  // vector i if it is a whole one.  (A load at a clamped place and a choice: no branch in front of the loads.)
+  __device__ __forceinline__ hd_u32x4 whole(int i) const {
+    const hd_u32x4 w = hd_load16<T>(x + (long long)(i < nfull ? i : nfull - 1) * T::kPerVec);
+    return i < nfull ? w : nothing();
+  }
+  __device__ __forceinline__ hd_u32x4 fetch(int i) const {
+    hd_u32x4 w = whole(i);
+    if (tail && i == nfull) w = last();
+    return w;
+  }
+};
+
+// The alternatives of a row by a whole workgroup: `mine` is the best key of a thread's share of shares, winners(low, push) names its
+// shares whose key reaches `low` (WIN in all at most), share(w) says where one lies: every STRIDE-th vector of a stretch.
+struct Share {
+  int first, end;
+};
+template <class T, int BT, int STRIDE, int WIN, class Winners, class ShareOf>
+__device__ __forceinline__ void lp_select(const FwdArgs &a, long long row, const Vectors<T> &v, const RowStat &st, u64 mine, Winners winners,
+                                          ShareOf share) {
+  constexpr int VE = T::kPerVec, W = BT / PN2_WAVE;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  __shared__ u64 sh_group[64], sh_low;
+  __shared__ int sh_win[WIN], sh_count[2];            // winners, candidates
+  __shared__ u64 sh_cand[kCand + 1], sh_best[W];
+  // the best key of each of 64 groups of neighbouring threads; the k-th best of them bounds the k best elements from below
+  u64 g = mine;
+  {
+    u64 o = pn2_dpp_u64<PN2_DPP_QUAD_XOR1>(g);
+    g = o > g ? o : g;
+    o = pn2_dpp_u64<PN2_DPP_QUAD_XOR2>(g);
+    g = o > g ? o : g;
+    if constexpr (BT >= 512) { o = pn2_dpp_u64<PN2_DPP_ROW_HALF_MIRROR>(g); g = o > g ? o : g; }
+    if constexpr (BT >= 1024) { o = pn2_dpp_u64<PN2_DPP_ROW_MIRROR>(g); g = o > g ? o : g; }
+  }
+  if (tid % (BT / 64) == 0) sh_group[tid / (BT / 64)] = g;
+  if (tid < 2) sh_count[tid] = 0;
+  if (tid < a.top) lp_clear(a, row, tid, st);
+  __syncthreads();
+  if (st.nan) return;                                // uniform over the workgroup
+  if (wave == 0) {
+    const u64 k = sh_group[lane];
+    const int rank = lp_rank64(k, 64);               // (keys of non-empty groups differ: their vectors do)
+    const u64 hit = __ballot(rank == a.top - 1 && k != 0u);
+    const u64 low = hit ? pn2_readlane_u64(k, __ffsll((unsigned long long)hit) - 1) : (u64)(kKeyNegInf + 1) << 32;
+    if (lane == 0) sh_low = low;
+  }
+  __syncthreads();
+  const u64 low = sh_low;
+  winners(low, [&](int w) { sh_win[atomicAdd(&sh_count[0], 1)] = w; });        // (any order: the ranking below is total)
+  __syncthreads();
+  const int nwin = sh_count[0];
+  // (one share at a time: a single row's time is this code's trip through the instruction cache, 15.1 us against 16.5 us unrolled)
+  for (int w = wave; w < nwin; w += W) {
+    const Share s = share(sh_win[w]);
+    for (int i = s.first + lane * STRIDE; __builtin_amdgcn_readfirstlane(i) < s.end; i += STRIDE * PN2_WAVE) {   // its vectors, one per lane
+      float f[VE];
+      T::unpack(i < s.end ? v.fetch(i) : v.nothing(), f);
+      unsigned k[VE], hits = 0u;
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        k[j] = lp_key(f[j]);
+        // (what lies behind the row's end reads as -inf, below any bound)
+        if ((((u64)k[j] << 32) | (unsigned)~i) >= low) hits |= 1u << j;
+      }
+      if (hits) {
+        const int at = atomicAdd(&sh_count[1], __popc(hits));
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {               // (what is no candidate, or one too many, goes to a slot that nobody reads)
+          const int to = at + __popc(hits & ((1u << j) - 1u));
+          sh_cand[((hits >> j) & 1u) && to < kCand ? to : kCand] = ((u64)k[j] << 32) | (unsigned)~(i * VE + j);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh_count[1];
+  if (n <= kCand) {
+    for (int e = tid; e < n; e += BT) lp_place(a, row, sh_cand, n, sh_cand[e], st);
+    return;
+  }
+  // rows with very many equal entries at the bound: one pass over the row per alternative, each the best below the last
+  u64 last = ~(u64)0;
+  for (int q = 0; q < a.top; ++q) {
+    u64 best = 0u;
+    for (int i = tid; i < v.nvec; i += BT) {
+      float f[VE];
+      T::unpack(v.fetch(i), f);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const unsigned k = lp_key(f[j]);
+        const u64 key = ((u64)k << 32) | (unsigned)~(i * VE + j);
+        if (k > kKeyNegInf && key < last && key > best) best = key;
+      }
+    }
+    best = pn2_wave_max_u64(best);
+    if (lane == 0) sh_best[wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) best = sh_best[w] > best ? sh_best[w] : best;
+    __syncthreads();
+    if (best == 0u) break;                           // uniform over the workgroup
+    if (tid == 0) {
+      a.top_lp[row * a.top + q] = lp_logp(lp_unkey((unsigned)(best >> 32)), st);
+      a.top_idx[row * a.top + q] = (int)~(unsigned)best;
+    }
+    last = best;
+  }
+}
+
+// (x - m) c summed again where x c may overflow; by the whole workgroup, behind a barrier
+template <class T, bool ENT, int BT>
+__device__ __forceinline__ void lp_sum_again(RowSum &r, const typename T::elem *x, int V, float c, float *sh_s, float *sh_se) {
+  constexpr int W = BT / PN2_WAVE;
+  float s = 0.f, se = 0.f;
+  for (int i = threadIdx.x; i < V; i += BT) {
+    const float t = (T::load(x + i) - r.m) * c, e = hd_exp2(t);
+    s += e;
+    if constexpr (ENT) se += e * fmaxf(t, -1e30f);
+  }
+  s = hd_wave_sum(s);
+  se = hd_wave_sum(se);
+  __syncthreads();
+  if (pn2_lane() == 0) { sh_s[threadIdx.x >> 6] = s; sh_se[threadIdx.x >> 6] = se; }
+  __syncthreads();
+  r.s = r.se = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) { r.s += sh_s[w]; r.se += sh_se[w]; }
+}
+
+// SEG: a workgroup per segment of a row instead, which leaves its sums and its best entries' keys for lp_join_kernel.
+template <class T, int MODE, bool TOP, int BT, int U, bool SEG>
 __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
   constexpr int VE = T::kPerVec, W = BT / PN2_WAVE;
   constexpr bool ENT = MODE == MODE_LABEL;
   typedef typename T::elem elem;
   __shared__ float sh_m[W], sh_s[W], sh_se[W];
-  const long long row = blockIdx.x;
+  const long long unit = blockIdx.x, row = SEG ? unit / a.nseg : unit;
+  const int from = SEG ? (int)(unit - row * a.nseg) * a.seg : 0, V = SEG ? (a.V - from < a.seg ? a.V - from : a.seg) : a.V;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const elem *x = (const elem *)a.logits + row * a.ld;
+  const elem *x = (const elem *)a.logits + row * a.ld + from;
   RowSum r{-kHdInf, 0.f, 0.f, 0.f};
   if constexpr (MODE == MODE_DISTILL) {
     if (!lp_teacher_any(a, row)) {                     // the same answer in every wave
-      if (wave == 0) lp_finish_distill<T>(a, row, x, RowStat{}, false);
+      if (!SEG && wave == 0) lp_finish_distill<T>(a, row, x, RowStat{}, false);
       return;
     }
   }
   Label label{};
-  if constexpr (MODE == MODE_LABEL) {
+  if constexpr (MODE == MODE_LABEL && !SEG) {
     if (wave == W - 1) label = lp_label<T>(a, row, x);
   }
   const float c = a.c, lim = lp_lim(c);
   r.M2 = lp_ref(r.m, c, lim);
-  const int nfull = a.V / VE, tail = a.V % VE, nvec = nfull + (tail != 0);
+  const Vectors<T> v(x, V);
+  const int nfull = v.nfull, tail = v.tail;
   int ord = 0x7fffffff;                                // first vector that holds the thread's maximum
-  // the row's last, partial vector, filled up with nothing (-inf)
-  auto last_vector = [&]() -> hd_u32x4 {
-    float g[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) g[j] = j < tail ? T::load(x + (long long)nfull * VE + j) : -kHdInf;
-    return T::pack(g);
-  };
-  hd_u32x4 nothing;
-  {
-    float g[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) g[j] = -kHdInf;
-    nothing = T::pack(g);
-  }
-  // vector i of the row; behind the row's end: nothing.  (A load at a clamped place and a choice: no branch in front of the loads.)
-  auto whole = [&](int i) -> hd_u32x4 {
-    const hd_u32x4 w = hd_load16<T>(x + (long long)(i < nfull ? i : nfull - 1) * VE);
-    return i < nfull ? w : nothing;
-  };
-  auto fetch = [&](int i) -> hd_u32x4 {
-    hd_u32x4 w = whole(i);
-    if (tail && i == nfull) w = last_vector();
-    return w;
-  };
-  hd_u32x4 behind = nothing;
-  if (tail && tid == nfull % BT) behind = last_vector();
+  hd_u32x4 behind = v.nothing();
+  if (tail && tid == nfull % BT) behind = v.last();
   for (int b = 0; b < nfull; b += BT * U) {
     hd_u32x4 w[U];
     if (b + BT * U <= nfull) {
@@ -370,7 +509,7 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
       for (int u = 0; u < U; ++u) w[u] = hd_load16<T>(x + (long long)(b + u * BT + tid) * VE);
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = whole(b + u * BT + tid);
+      for (int u = 0; u < U; ++u) w[u] = v.whole(b + u * BT + tid);
     }
     float f[U * VE];
     float bm = -kHdInf;
@@ -418,122 +557,98 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
       if constexpr (ENT) r.se = __fmaf_rn(__fmaf_rn(sh_s[w], d, sh_se[w]), f, r.se);
     }
   }
-  float res = __fmaf_rn(r.m, c, -r.M2);
-  if (fabsf(r.m) > lim && fabsf(r.m) < kHdInf) {
-    // x c may overflow: sum again with (x - m) c.  Uniform over the workgroup; every wave has passed the barrier above.
-    float s = 0.f, se = 0.f;
-    for (int i = tid; i < a.V; i += BT) {
-      const float t = (T::load(x + i) - r.m) * c, e = hd_exp2(t);
-      s += e;
-      if constexpr (ENT) se += e * fmaxf(t, -1e30f);
+  RowStat st{};
+  if constexpr (SEG) {
+    if (tid == 0) hd_store16<HdF32>(a.part + unit * 4, HdF32::pack({r.m, r.s, r.se, 0.f}));
+  } else {
+    float res = __fmaf_rn(r.m, c, -r.M2);
+    if (fabsf(r.m) > lim && fabsf(r.m) < kHdInf) {     // uniform over the workgroup; every wave has passed the barrier above
+      lp_sum_again<T, ENT, BT>(r, x, V, c, sh_s, sh_se);
+      res = 0.f;
     }
-    s = hd_wave_sum(s);
-    se = hd_wave_sum(se);
-    __syncthreads();
-    if (lane == 0) { sh_s[wave] = s; sh_se[wave] = se; }
-    __syncthreads();
-    r.s = r.se = 0.f;
+    st = lp_stat(r, res);
+    if constexpr (MODE == MODE_DISTILL) {
+      if (wave == 0) lp_finish_distill<T>(a, row, x, st, true);
+      return;
+    }
+    if (wave == W - 1) lp_finish_label(a, row, label, st);
+  }
+  if constexpr (TOP) {
+    // keys as one number: value above, vector below, earlier ones larger
+    const u64 mine = own == -kHdInf ? 0u : ((u64)lp_key(own) << 32) | (unsigned)~(ord + (SEG ? from / VE : 0));
+    if constexpr (SEG) {
+      a.keys[unit * BT + tid] = mine;
+    } else {
+      lp_select<T, BT, BT, BT>(
+          a, row, v, st, mine,
+          [&](u64 low, auto push) { if (mine >= low && mine != 0u) push(tid); },
+          [&](int w) { return Share{w, v.nvec}; });
+    }
+  }
+}
+
+// A row's segments joined: their sums by every wave (one segment per lane), then the alternatives, from the keys of the segments' threads.
+constexpr int kSegThreads = 256, kMaxSeg = 32;
+template <class T, int MODE, bool TOP, int BT>
+__global__ __launch_bounds__(BT) void lp_join_kernel(FwdArgs a) {
+  constexpr bool ENT = MODE == MODE_LABEL;
+  constexpr int W = BT / PN2_WAVE, NK = kMaxSeg * kSegThreads / BT;
+  __shared__ float sh_s[W], sh_se[W];
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const Vectors<T> v((const typename T::elem *)a.logits + row * a.ld, a.V);
+  if constexpr (MODE == MODE_DISTILL) {
+    if (!lp_teacher_any(a, row)) {
+      if (wave == 0) lp_finish_distill<T>(a, row, v.x, RowStat{}, false);
+      return;
+    }
+  }
+  u64 key[TOP ? NK : 1] = {}, mine = 0u;
+  if constexpr (TOP) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) { r.s += sh_s[w]; r.se += sh_se[w]; }
+    for (int q = 0; q < NK; ++q) {                     // (loads at clamped places)
+      const int at = q * BT + tid, n = a.nseg * kSegThreads;
+      const u64 k = a.keys[row * n + (at < n ? at : 0)];
+      key[q] = at < n ? k : 0u;
+    }
+  }
+  const float c = a.c, lim = lp_lim(c);
+  float f[4];
+  HdF32::unpack(hd_load16<HdF32>(a.part + (row * a.nseg + (lane < a.nseg ? lane : 0)) * 4), f);
+  Label label{};
+  if constexpr (MODE == MODE_LABEL) {
+    if (wave == W - 1) label = lp_label<T>(a, row, v.x);
+  }
+  const bool on = lane < a.nseg;
+  RowSum r{on ? f[0] : -kHdInf, 0.f, on ? f[1] : 0.f, on ? f[2] : 0.f};
+  r.M2 = lp_ref(r.m, c, lim);
+  r = lp_wave_combine<ENT>(r, c, lim);
+  float res = __fmaf_rn(r.m, c, -r.M2);
+  if (fabsf(r.m) > lim && fabsf(r.m) < kHdInf) {       // uniform over the workgroup
+    lp_sum_again<T, ENT, BT>(r, v.x, a.V, c, sh_s, sh_se);
     res = 0.f;
   }
   const RowStat st = lp_stat(r, res);
   if constexpr (MODE == MODE_DISTILL) {
-    if (wave == 0) lp_finish_distill<T>(a, row, x, st, true);
+    if (wave == 0) lp_finish_distill<T>(a, row, v.x, st, true);
     return;
   }
   if (wave == W - 1) lp_finish_label(a, row, label, st);
   if constexpr (TOP) {
-    __shared__ u64 sh_group[64], sh_low;
-    __shared__ int sh_win[BT], sh_count[2];            // winners, candidates
-    __shared__ u64 sh_cand[kCand + 1], sh_best[W];
-    // keys as one number: value above, vector (or element) below, earlier ones larger
-    const u64 mine = own == -kHdInf ? 0u : ((u64)lp_key(own) << 32) | (unsigned)~ord;
-    // the best key of each of 64 groups of neighbouring threads; the k-th best of them bounds the k best elements from below
-    u64 g = mine;
-    {
-      u64 o = pn2_dpp_u64<PN2_DPP_QUAD_XOR1>(g);
-      g = o > g ? o : g;
-      o = pn2_dpp_u64<PN2_DPP_QUAD_XOR2>(g);
-      g = o > g ? o : g;
-      if constexpr (BT >= 512) { o = pn2_dpp_u64<PN2_DPP_ROW_HALF_MIRROR>(g); g = o > g ? o : g; }
-      if constexpr (BT >= 1024) { o = pn2_dpp_u64<PN2_DPP_ROW_MIRROR>(g); g = o > g ? o : g; }
-    }
-    if (tid % (BT / 64) == 0) sh_group[tid / (BT / 64)] = g;
-    if (tid < 2) sh_count[tid] = 0;
-    if (tid < a.top) {                                 // slots that no entry will take
-      a.top_lp[row * a.top + tid] = st.nan ? __builtin_nanf("") : -kHdInf;
-      a.top_idx[row * a.top + tid] = -1;
-    }
-    __syncthreads();
-    if (st.nan) return;                                // uniform over the workgroup
-    if (wave == 0) {
-      const u64 k = sh_group[lane];
-      const int rank = lp_rank64(k, 64);               // (keys of non-empty groups differ: their vectors do)
-      const u64 hit = __ballot(rank == a.top - 1 && k != 0u);
-      const u64 low = hit ? pn2_readlane_u64(k, __ffsll((unsigned long long)hit) - 1) : (u64)(kKeyNegInf + 1) << 32;
-      if (lane == 0) sh_low = low;
-    }
-    __syncthreads();
-    const u64 low = sh_low;
-    if (mine >= low && mine != 0u) sh_win[atomicAdd(&sh_count[0], 1)] = tid;     // (any order: the ranking below is total)
-    __syncthreads();
-    const int nwin = sh_count[0];
-    // (one share at a time: a single row's time is this code's trip through the instruction cache, 15.1 us against 16.5 us unrolled)
-    for (int w = wave; w < nwin; w += W) {
-      for (int i = sh_win[w] + lane * BT; __builtin_amdgcn_readfirstlane(i) < nvec; i += BT * PN2_WAVE) {   // its vectors, one per lane
-        float f[VE];
-        T::unpack(fetch(i), f);
-        unsigned k[VE], hits = 0u;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          k[j] = lp_key(f[j]);
-          // (what lies behind the row's end reads as -inf, below any bound)
-          if ((((u64)k[j] << 32) | (unsigned)~i) >= low) hits |= 1u << j;
-        }
-        if (hits) {
-          const int at = atomicAdd(&sh_count[1], __popc(hits));
+    for (int q = 0; q < NK; ++q) mine = key[q] > mine ? key[q] : mine;
+    const int each = a.seg / T::kPerVec;
+    lp_select<T, BT, kSegThreads, kMaxSeg * kSegThreads>(
+        a, row, v, st, mine,
+        [&](u64 low, auto push) {
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {               // (what is no candidate, or one too many, goes to a slot that nobody reads)
-            const int to = at + __popc(hits & ((1u << j) - 1u));
-            sh_cand[((hits >> j) & 1u) && to < kCand ? to : kCand] = ((u64)k[j] << 32) | (unsigned)~(i * VE + j);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    const int n = sh_count[1];
-    if (n <= kCand) {
-      for (int e = tid; e < n; e += BT) lp_place(a, row, sh_cand, n, sh_cand[e], st);
-      return;
-    }
-    // rows with very many equal entries at the bound: one pass over the row per alternative, each the best below the last
-    u64 last = ~(u64)0;
-    for (int q = 0; q < a.top; ++q) {
-      u64 best = 0u;
-      for (int i = tid; i < nvec; i += BT) {
-        float f[VE];
-        T::unpack(fetch(i), f);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const unsigned k = lp_key(f[j]);
-          const u64 key = ((u64)k << 32) | (unsigned)~(i * VE + j);
-          if (k > kKeyNegInf && key < last && key > best) best = key;
-        }
-      }
-      best = pn2_wave_max_u64(best);
-      if (lane == 0) sh_best[wave] = best;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < W; ++w) best = sh_best[w] > best ? sh_best[w] : best;
-      __syncthreads();
-      if (best == 0u) break;                           // uniform over the workgroup
-      if (tid == 0) {
-        a.top_lp[row * a.top + q] = lp_logp(lp_unkey((unsigned)(best >> 32)), st);
-        a.top_idx[row * a.top + q] = (int)~(unsigned)best;
-      }
-      last = best;
-    }
+          for (int q = 0; q < NK; ++q)
+            if (key[q] >= low && key[q] != 0u) push(q * BT + tid);
+        },
+        [&](int w) {
+          const int seg = w / kSegThreads, end = (seg + 1) * each;
+          return Share{seg * each + w % kSegThreads, end < v.nvec ? end : v.nvec};
+        });
   }
 }
 
@@ -691,16 +806,39 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
   }
 }
 
+// Segments of a row: where rows are few and long, the workgroup that owned one would be bound by its own arithmetic while most of the
+// chip idles.  Whole rows against segments, us: 1 x 131072 bf16 10.2 - 4.4, with 20 alternatives 14.6 - 10.4, distillation 8.6 - 6.0;
+// 64 x 131072 10.7 - 6.6, 15.7 - 13.8, 9.1 - 7.8.  The second launch costs the host 3 us, and shorter rows win less than that (65536
+// bf16 6.7 - 4.4, with alternatives 11.3 - 10.4); 128 rows fill half the chip by themselves (16.1 - 17.5 with alternatives).
+struct Split {
+  int nseg, seg;
+  size_t keys, part;        // bytes
+};
+Split lp_split(long long T, int V, int dtype, int top) {
+  const int ve = dtype == PN2_DT_F32 ? 4 : 8, nvec = V / ve + (V % ve != 0);
+  if (T < 1 || T > 64 || nvec < 16384) return Split{1, V, 0, 0};
+  int n = nvec / 1024;
+  if (n > kMaxSeg) n = kMaxSeg;
+  const int each = (nvec + n - 1) / n;
+  n = (nvec + each - 1) / each;
+  return Split{n, each * ve, top ? (size_t)T * n * kSegThreads * 8 : 0, (size_t)T * n * 16};
+}
+
 template <class T, int MODE, bool TOP>
 void lp_row_launch(const FwdArgs &a, hipStream_t st) {
+  if (a.nseg > 1) {
+    lp_row_kernel<T, MODE, TOP, kSegThreads, 4, true><<<(unsigned)(a.T * a.nseg), kSegThreads, 0, st>>>(a);
+    lp_join_kernel<T, MODE, TOP, TOP ? 1024 : 256><<<(unsigned)a.T, TOP ? 1024 : 256, 0, st>>>(a);
+    return;
+  }
   // Fewer rows than CUs: one big workgroup per row with its loads on their way at once (1 x 131072 bf16 with 20 alternatives 15 us, 25
   // with 512 threads).  Otherwise several workgroups per CU, smaller ones for short rows, whose time is the selection's round trips
   // (8192 x 16384 bf16 with 20 alternatives: 95 us with 256 threads, 122 with 512; 8192 x 131072: 0.43 ms with 512).
   const unsigned grid = (unsigned)a.T;
   const int nvec = (a.V + T::kPerVec - 1) / T::kPerVec;
-  if (nvec > 1024 && a.T <= 256) lp_row_kernel<T, MODE, TOP, 1024, 8><<<grid, 1024, 0, st>>>(a);
-  else if (nvec <= 4096) lp_row_kernel<T, MODE, TOP, 256, 4><<<grid, 256, 0, st>>>(a);
-  else lp_row_kernel<T, MODE, TOP, 512, 4><<<grid, 512, 0, st>>>(a);
+  if (nvec > 1024 && a.T <= 256) lp_row_kernel<T, MODE, TOP, 1024, 8, false><<<grid, 1024, 0, st>>>(a);
+  else if (nvec <= 4096) lp_row_kernel<T, MODE, TOP, 256, 4, false><<<grid, 256, 0, st>>>(a);
+  else lp_row_kernel<T, MODE, TOP, 512, 4, false><<<grid, 512, 0, st>>>(a);
 }
 
 template <class T, int MODE>
@@ -713,8 +851,13 @@ int lp_forward(const FwdArgs &a, hipStream_t st) {
     else lp_small_kernel<T, MODE, 32><<<grid, 256, 0, st>>>(a);
     return pn2_check_launch();
   }
-  if (MODE == MODE_LABEL && a.top) lp_row_launch<T, MODE, true>(a, st);
-  else lp_row_launch<T, MODE, false>(a, st);
+  if constexpr (MODE == MODE_LABEL) {
+    if (a.top) {
+      lp_row_launch<T, MODE, true>(a, st);
+      return pn2_check_launch();
+    }
+  }
+  lp_row_launch<T, MODE, false>(a, st);
   return pn2_check_launch();
 }
 
@@ -752,11 +895,34 @@ inline bool lp_bad(long long T, int V, long long ld, int dtype) {
   return T < 0 || V < 1 || ld < 0 || T > 0x7fffffffLL || dtype < PN2_DT_F32 || dtype > PN2_DT_F16;
 }
 
+// the caller's workspace divided
+int lp_segments(FwdArgs &a, int dtype, void *workspace, size_t bytes) {
+  const Split p = lp_split(a.T, a.V, dtype, a.top);
+  if (bytes < p.keys + p.part) return PN2_ENOSPC;
+  if (p.nseg > 1 && !workspace) return PN2_ENULL;
+  a.nseg = p.nseg;
+  a.seg = p.seg;
+  a.keys = (u64 *)workspace;
+  a.part = (float *)((char *)workspace + p.keys);
+  return PN2_OK;
+}
+
 }  // namespace
+
+extern "C" size_t pn2_label_logprobs_workspace_bytes(long long T, int V, int dtype, int top) {
+  if (lp_bad(T, V, 0, dtype) || top < 0 || top > kMaxTop || top > V) return 0;
+  const Split p = lp_split(T, V, dtype, top);
+  return p.keys + p.part;
+}
+
+extern "C" size_t pn2_distill_topk_workspace_bytes(long long T, int V, int dtype) {
+  if (lp_bad(T, V, 0, dtype)) return 0;
+  return lp_split(T, V, dtype, 0).part;
+}
 
 extern "C" int pn2_label_logprobs(long long T, int V, long long ld, int dtype, const void *logits, const long long *labels,
                                   long long ignore_index, int top, float *log_prob, float *entropy, float *stats,
-                                  float *top_log_prob, long long *top_index, void *stream) {
+                                  float *top_log_prob, long long *top_index, void *workspace, size_t workspace_bytes, void *stream) {
   if (lp_bad(T, V, ld, dtype) || top < 0 || top > kMaxTop || top > V) return PN2_EINVAL;
   if (T == 0) return PN2_OK;
   if (!logits || !labels || !log_prob || !entropy || (top && (!top_log_prob || !top_index))) return PN2_ENULL;
@@ -764,6 +930,8 @@ extern "C" int pn2_label_logprobs(long long T, int V, long long ld, int dtype, c
   a.T = T; a.ld = ld; a.V = V; a.top = top; a.c = kHdLog2e; a.tau = 1.f;
   a.logits = logits; a.labels = labels; a.ignore = ignore_index;
   a.log_prob = log_prob; a.entropy = entropy; a.stats = stats; a.top_lp = top_log_prob; a.top_idx = top_index;
+  const int rc = lp_segments(a, dtype, workspace, workspace_bytes);
+  if (rc != PN2_OK) return rc;
   return lp_forward_any<MODE_LABEL>(dtype, a, (hipStream_t)stream);
 }
 
@@ -782,7 +950,7 @@ extern "C" int pn2_label_logprobs_grad(long long T, int V, long long ld, int dty
 
 extern "C" int pn2_distill_topk(long long T, int V, long long ld, int dtype, const void *logits, int k, const long long *teacher_index,
                                 int teacher_dtype, const void *teacher_logits, float temperature, float *loss, float *stats,
-                                void *stream) {
+                                void *workspace, size_t workspace_bytes, void *stream) {
   if (lp_bad(T, V, ld, dtype) || k < 1 || teacher_dtype < PN2_DT_F32 || teacher_dtype > PN2_DT_F16 || !(temperature > 0.f) ||
       !(temperature < kHdInf))
     return PN2_EINVAL;
@@ -791,6 +959,8 @@ extern "C" int pn2_distill_topk(long long T, int V, long long ld, int dtype, con
   FwdArgs a{};
   a.T = T; a.ld = ld; a.V = V; a.k = k; a.tau = temperature; a.c = kHdLog2e / temperature;
   a.logits = logits; a.t_idx = teacher_index; a.t_val = teacher_logits; a.t_dtype = teacher_dtype; a.loss = loss; a.stats = stats;
+  const int rc = lp_segments(a, dtype, workspace, workspace_bytes);
+  if (rc != PN2_OK) return rc;
   return lp_forward_any<MODE_DISTILL>(dtype, a, (hipStream_t)stream);
 }
 

@@ -163,10 +163,11 @@ _SIGNATURES = {
                        ctypes.c_longlong] + [_c_vp] * 3 + [_c_sz, _c_vp],
     "pn2_linear_act_grad": [ctypes.c_longlong, _c_int, _c_int, _c_int, _c_vp, ctypes.c_longlong, _c_vp] +
                            [_c_vp, ctypes.c_longlong] * 2 + [_c_vp] * 3 + [_c_int, _c_vp, _c_sz, _c_vp],
-    "pn2_label_logprobs": [ctypes.c_longlong, _c_int, ctypes.c_longlong, _c_int, _c_vp, _c_vp, ctypes.c_longlong, _c_int] + [_c_vp] * 6,
+    "pn2_label_logprobs": [ctypes.c_longlong, _c_int, ctypes.c_longlong, _c_int, _c_vp, _c_vp, ctypes.c_longlong, _c_int] +
+                          [_c_vp] * 6 + [_c_sz, _c_vp],
     "pn2_label_logprobs_grad": [ctypes.c_longlong, _c_int, ctypes.c_longlong, _c_int, _c_vp, _c_vp, ctypes.c_longlong] + [_c_vp] * 6,
     "pn2_distill_topk": [ctypes.c_longlong, _c_int, ctypes.c_longlong, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_f32] +
-                        [_c_vp] * 3,
+                        [_c_vp] * 3 + [_c_sz, _c_vp],
     "pn2_distill_topk_grad": [ctypes.c_longlong, _c_int, ctypes.c_longlong, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_f32] +
                              [_c_vp] * 4,
     # batched scans with per-scan statistics (segment table)
@@ -279,6 +280,10 @@ _lib.pn2_linear_act_workspace_bytes.restype = _c_sz
 _lib.pn2_linear_act_grad_workspace_bytes.argtypes = ([ctypes.c_longlong] + [_c_int] * 3 + [_c_vp, ctypes.c_longlong, _c_int] +
                                                      [_c_vp, ctypes.c_longlong] * 2 + [_c_int])
 _lib.pn2_linear_act_grad_workspace_bytes.restype = _c_sz
+_lib.pn2_label_logprobs_workspace_bytes.argtypes = [ctypes.c_longlong] + [_c_int] * 3
+_lib.pn2_label_logprobs_workspace_bytes.restype = _c_sz
+_lib.pn2_distill_topk_workspace_bytes.argtypes = [ctypes.c_longlong] + [_c_int] * 2
+_lib.pn2_distill_topk_workspace_bytes.restype = _c_sz
 _lib.pn2_abi_version.restype = _c_int
 _lib.pn2_last_hip_error.restype = _c_int
 _lib.pn2_strerror.argtypes = [_c_int]
@@ -302,6 +307,7 @@ EXPORTED_SYMBOLS = sorted(list(_SIGNATURES) + ["pn2_fps_workspace_bytes", "pn2_a
                                                "pn2_mlp_bwd_bf16_supported", "pn2_pool_bwd_supported",
                                                "pn2_pool_bwd_workspace_bytes", "pn2_x3_weight_bytes", "pn2_sa_eval_x3_supported", "pn2_x3_gemm_supported", "pn2_x3_gemm_first_supported",
                                                "pn2_linear_act_workspace_bytes", "pn2_linear_act_grad_workspace_bytes",
+                                               "pn2_label_logprobs_workspace_bytes", "pn2_distill_topk_workspace_bytes",
                                                "pn2_last_hip_error", "pn2_strerror"])
 #: the python layer may use the point-major fused entry points of this backend
 HAS_ROWS = True

@@ -941,10 +941,12 @@ int pn2_x3_pool_bwd(long long M, int N, int K, int ns, const float *Yp, const fl
  *       entries of -inf are no alternatives: such slots hold -inf and the index -1.  top = 0: both may be NULL
  *   stats (T, 2) f32 for the gradient, or NULL
  * A row of nothing but -inf: log_prob -inf, entropy 0, no alternatives, gradient 0.  A row with NaN or +inf: NaN, indices -1.
+ * Few long rows are summed in segments, whose results meet in the workspace (16-byte aligned; 0 bytes: none, NULL).
  * The gradient: dlogits (T, V) dense, every element written, rounded once;  g_log_prob / g_entropy (T) f32, NULL = zero. */
+size_t pn2_label_logprobs_workspace_bytes(long long T, int V, int dtype, int top);
 int pn2_label_logprobs(long long T, int V, long long ld, int dtype, const void *logits, const long long *labels,
                        long long ignore_index, int top, float *log_prob, float *entropy, float *stats, float *top_log_prob,
-                       long long *top_index, void *stream);
+                       long long *top_index, void *workspace, size_t workspace_bytes, void *stream);
 int pn2_label_logprobs_grad(long long T, int V, long long ld, int dtype, const void *logits, const long long *labels,
                             long long ignore_index, const float *stats, const float *entropy, const float *g_log_prob,
                             const float *g_entropy, void *dlogits, void *stream);
@@ -954,9 +956,12 @@ int pn2_label_logprobs_grad(long long T, int V, long long ld, int dtype, const v
  * p = softmax(logits / temperature) over all V:   loss (T) f32 = temperature^2 sum_j q_j (log q_j - log p[index_j]).
  * A slot with a negative index or the value -inf is unused; a row without a used slot has loss 0 and gradient 0 (its logits are
  * not read).  An index >= V makes the row NaN.  An index may occur more than once.  stats (T, 4) f32 for the gradient, or NULL.
+ * The workspace: as above.
  * The gradient: dlogits (T, V) dense = g_loss temperature (p - sum_j q_j [index_j = v]), every element written, rounded once. */
+size_t pn2_distill_topk_workspace_bytes(long long T, int V, int dtype);
 int pn2_distill_topk(long long T, int V, long long ld, int dtype, const void *logits, int k, const long long *teacher_index,
-                     int teacher_dtype, const void *teacher_logits, float temperature, float *loss, float *stats, void *stream);
+                     int teacher_dtype, const void *teacher_logits, float temperature, float *loss, float *stats,
+                     void *workspace, size_t workspace_bytes, void *stream);
 int pn2_distill_topk_grad(long long T, int V, long long ld, int dtype, const void *logits, int k, const long long *teacher_index,
                           int teacher_dtype, const void *teacher_logits, float temperature, const float *stats,
                           const float *g_loss, void *dlogits, void *stream);

@@ -485,6 +485,90 @@ def test_distill_top_k_unused_slots_repeats_and_masks(V, dtype):
     assert ho.distill_top_k(x[:0], idx[:0], val[:0]).shape == (0,)
 
 
+# few long rows: in segments, joined by a second launch
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [131072, 131077, 270001, 600011])
+def test_few_long_rows(V, dtype):
+    gen = torch.Generator().manual_seed(V)
+    x = rnd(gen, 3, V, scale=3.0, dtype=dtype)
+    x[1, torch.rand(V, generator=gen).cuda() < 0.6] = -INF
+    x[2, :V - 40000] = -INF                                         # whole segments without an entry
+    y = torch.tensor([V - 1, 3, V - 7]).cuda()
+    for top in (0, 1, 20, 64):
+        run_labels(x, y, top, seed=top)
+    idx = torch.randint(V, (3, 64), generator=gen).cuda()
+    idx[2] = V - 1 - torch.arange(64).cuda()
+    idx[1, :60] = -1
+    x[1, idx[1, 60:]] = 1.0
+    run_distill(x, idx, rnd(gen, 3, 64, scale=2.0), 1.5)
+    # a row alone, and out of a wider matrix
+    a, b = ho.label_log_probs(x[1:2], y[1:2], top=20), ho.label_log_probs(x, y, top=20)
+    assert all(torch.equal(p[0], q[1]) for p, q in zip(a, b))
+    wide = torch.full((3, V + 3), 50.0, device="cuda", dtype=dtype)
+    wide[:, 1:V + 1] = x
+    c = ho.label_log_probs(wide[:, 1:V + 1], y, top=20)
+    assert all(torch.equal(p, q) for p, q in zip(b, c))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [131077, 262144 + 5])
+def test_few_long_hard_rows(V, dtype):
+    test_label_log_probs_hard_rows(V, dtype)
+    test_distill_top_k_unused_slots_repeats_and_masks(V, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_few_long_rows_best_entries_in_one_share(dtype):
+    """Every thread's share of the segments in turn holds the best entries: those of one thread, neighbours', the row's ends."""
+    per = 128 // torch.finfo(dtype).bits
+    V = 16384 * per + 3
+    x = torch.zeros(4, V)
+    share = (torch.arange(0, 1024 * per, 256 * per)[:, None] + torch.arange(per)).flatten()
+    x[0, share] = 2.0 + torch.arange(share.numel()) % 5
+    x[1, share + 7 * 1024 * per] = 1.0
+    x[1, share + 7 * 1024 * per + 3 * per] = 1.0
+    x[2, -50:] = 3.0
+    x[3, ::1024] = 4.0
+    run_labels(x.to(dtype).cuda(), torch.tensor([0, 1, V - 1, 1024]).cuda(), 40)
+
+
+def test_few_long_rows_in_two_graphs_and_on_two_streams():
+    """Segments' workspaces belong to their call: two captured graphs replayed in turn with eager work between, two streams at once."""
+    gen = torch.Generator().manual_seed(9)
+    V = 140001
+    x, y = rnd(gen, 2, V, dtype=torch.bfloat16), torch.tensor([5, V - 1]).cuda()
+    idx, val = torch.randint(V, (2, 20), generator=gen).cuda(), rnd(gen, 2, 20)
+
+    def step():
+        r = ho.label_log_probs(x, y, top=20)
+        return [*r, ho.distill_top_k(x, idx, val)]
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for n in range(4):
+        x.copy_(rnd(torch.Generator().manual_seed(70 + n), 2, V, dtype=torch.bfloat16))
+        g, out = graphs[n % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, e) for a, e in zip(got, step()))
+    want = step()
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        both = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                both.append(step())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for out in both for a, b in zip(out, want))
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the row statistics in fp32: cut-off e^2 / 6 times a third derivative bounded by 6 |v|^3 for the
     log-sum-exp (twice that times 1 + log V for the entropy), rounding of the two forward values over e."""

@@ -96,13 +96,19 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert grad(dy=None) == grad(x=None) == grad(w=None) == ENULL
     assert lib.pn2_linear_act_grad_workspace_bytes(4096, 512, 512, 0, some, 512, 1, some, 512, some, 512, 7) >= 4096 * 512 * 4
 
-    def labels(T=4, V=8, dt=0, x=some, y=some, top=0, lp=some, tl=None):
-        return lib.pn2_label_logprobs(T, V, V, dt, x, y, -100, top, lp, some, None, tl, tl, None)
+    def labels(T=4, V=8, dt=0, x=some, y=some, top=0, lp=some, tl=None, ws=None, nb=0):
+        return lib.pn2_label_logprobs(T, V, V, dt, x, y, -100, top, lp, some, None, tl, tl, ws, nb, None)
     assert labels(T=-1) == labels(V=0) == labels(dt=7) == labels(top=9) == labels(top=-1) == labels(V=100, top=65) == EINVAL
     assert labels(x=None) == labels(y=None) == labels(lp=None) == labels(top=1) == ENULL
     assert labels(T=0, x=None) == 0
+    # few long rows are summed in segments, whose results meet in a workspace
+    need = lib.pn2_label_logprobs_workspace_bytes(1, 131072, 1, 20)
+    assert need > 0 and lib.pn2_label_logprobs_workspace_bytes(1000, 131072, 1, 20) == 0
+    assert lib.pn2_label_logprobs_workspace_bytes(-1, 131072, 1, 20) == lib.pn2_label_logprobs_workspace_bytes(1, 2048, 1, 20) == 0
+    assert labels(T=1, V=131072, dt=1, top=20, tl=some, nb=need - 1) == ENOSPC
+    assert labels(T=1, V=131072, dt=1, top=20, tl=some, nb=need) == ENULL
 
-    def distill(k=2, t=1.0, tdt=0, x=some):
-        return lib.pn2_distill_topk(4, 8, 8, 0, x, k, some, tdt, some, t, some, None, None)
+    def distill(k=2, t=1.0, tdt=0, x=some, T=4, V=8, nb=0):
+        return lib.pn2_distill_topk(T, V, V, 0, x, k, some, tdt, some, t, some, None, None, nb, None)
     assert distill(k=0) == distill(t=0.0) == distill(t=-1.0) == distill(t=float("nan")) == distill(t=float("inf")) == EINVAL
     assert distill(tdt=3) == EINVAL and distill(x=None) == ENULL
