@@ -221,7 +221,8 @@ Tensor linear_act(const Tensor &x, const Tensor &weight, const std::optional<Ten
   check_device(xm, {{&wm, "weight"}, {&b, "bias"}, {&r, "residual"}});
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
                                                    (residual && residual->requires_grad()));
-  Tensor y = grad ? LinearAct::apply(xm, wm, bias, residual ? std::make_optional(r) : std::nullopt, act, timed)
+  Tensor y = grad ? LinearAct::apply(xm, wm, bias ? std::make_optional(b) : std::nullopt, residual ? std::make_optional(r) : std::nullopt, act,
+                                    timed)
                   : run_linear(xm, wm, b, r, act, false, timed).y;
   return x.dim() == 2 ? y : y.view(shape);
 }

@@ -51,7 +51,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     activation one of ``ACTIVATIONS``: none, relu, gelu (erf), gelu_tanh, silu.  -> (..., N) of x's type.
     Products accumulate in fp32; bias, activation and residual are applied to the accumulator and the result is rounded once.
     The backward pass keeps the activation's slope (one tensor like y); all its sums run in a fixed order."""
-    act = _ext.ACTIVATIONS.get(activation)
+    act = _ext.ACTIVATIONS.get(activation) if isinstance(activation, str) else None
     if act is None:
         _ext._fail(f"activation must be one of {', '.join(ACTIVATIONS)}")
     try:

@@ -57,7 +57,7 @@ class _Head(BaseNetwork):
         self.fc2 = nn.Linear(512, 256)
 
     def _trunk(self, x, use_bn, scan_ptr=None):
-        if self.fused_linear and x.is_cuda and not use_bn:
+        if self.fused_linear and x.is_cuda and not use_bn and x.dtype == self.fc1.weight.dtype:     # (autocast: the library's)
             from pointnet2_ops.head_ops import linear_act
             x = linear_act(x, self.fc1.weight, self.fc1.bias, "relu")
             if not (self.use_drop_out and self.training):          # dropout sits between fc2 and its ReLU

@@ -811,6 +811,11 @@ def test_views_with_the_negative_bit():
     x, w = z.conj().imag, rnd(gen, 5, 1)
     assert x.is_neg()
     assert torch.equal(ho.linear_act(x, w), ho.linear_act(x.clone().resolve_neg(), w))
+    b = torch.complex(rnd(gen, 1), rnd(gen, 1)).conj().imag
+    assert b.is_neg() and b.is_contiguous()
+    want = ho.linear_act(w, w[:1], b.resolve_neg())
+    assert torch.equal(ho.linear_act(w, w[:1], b), want)
+    assert torch.equal(ho.linear_act(w.clone().requires_grad_(), w[:1], b), want)
     z = torch.complex(rnd(gen, 4, 6), rnd(gen, 4, 6))
     x, y, best = z.conj().imag, torch.arange(4).cuda(), torch.arange(8).view(4, 2).cuda()
     assert torch.equal(ho.label_log_probs(x, y).log_prob, ho.label_log_probs(-z.imag.contiguous(), y).log_prob)
@@ -856,6 +861,17 @@ def test_fused_heads_equal_the_library_heads(train, monkeypatch):
         torch.testing.assert_close(a, b, atol=3 * 512 * U * float(a.abs().max()), rtol=0)
     for a, b in zip(grads, grads2):
         torch.testing.assert_close(a, b, atol=3 * 512 * U * float(a.abs().max()), rtol=0)
+
+
+def test_fused_heads_leave_autocast_to_the_library(monkeypatch):
+    from scene_graph_prediction.scene_graph_helpers.model.pointnets import network_PointNet as npn
+    torch.manual_seed(0)
+    head = npn.PointNetCls(12, in_size=256, batch_norm=False, drop_out=False).cuda().eval()
+    x = torch.randn(9, 256).cuda().bfloat16()
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        want = head(x)
+        monkeypatch.setattr(npn._Head, "fused_linear", True)
+        assert torch.equal(head(x), want)
 
 
 def test_model_alternatives_and_learning_from_a_teacher(tmp_path):

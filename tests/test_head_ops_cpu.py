@@ -59,6 +59,8 @@ def test_refusals(match, call):
     ("weight must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), None)),
     ("bias must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), f(4, 3), 1.0)),
     ("residual must be a torch.Tensor", lambda: ho.linear_act(f(2, 3), f(4, 3), residual=0)),
+    ("activation must be one of", lambda: ho.linear_act(f(2, 3), f(4, 3), activation=["relu"])),
+    ("activation must be one of", lambda: ho.linear_act(f(2, 3), f(4, 3), activation=None)),
     ("labels must be a torch.Tensor", lambda: ho.label_log_probs(f(2, 3), [0, 1])),
     ("teacher_logits must be a torch.Tensor", lambda: ho.distill_top_k(f(2, 3), torch.zeros(2, 1, dtype=torch.int64), None)),
     ("teacher_index must be a tensor of shape", lambda: ho.distill_top_k(f(3), torch.zeros(2, 2, dtype=torch.int64), f(2, 2))),
