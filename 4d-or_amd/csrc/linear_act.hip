@@ -902,7 +902,8 @@ __global__ __launch_bounds__(256) void la_db_kernel(Sums a) {
 }
 
 // dx, dW and db of a layer in the middle in one launch, on 64 x 64 tiles: `nx` workgroups for dx, `nw` for dW, the others for db.  Each
-// of the products alone leaves the chip half idle and takes as long as its own loop.
+// of the products alone leaves the chip half idle and takes as long as its own loop: 1003 x 1001 -> 777 fp16 15 us for the three (36 one
+// after the other), 2048 x 512 -> 512 bf16 forward and backward 28 us instead of 42.  Split contractions are joined by one more launch.
 template <class T>
 __global__ __launch_bounds__(256, 2) void la_pair_kernel(Product x, int xi, int xj, Product w, int wi, int wj, Sums b) {
   __shared__ __align__(1024) char ring[2 * 128 * 128];
