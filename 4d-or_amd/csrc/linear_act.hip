@@ -931,6 +931,8 @@ inline long long la_whole(long long n, int dtype) { return la_div(n, 16 / la_siz
 //   256 x 256     16-bit, tiles for three quarters of the CUs: 8192^3 784 against 1248 (128 x 128)
 // Splits only where a workgroup would walk a long contraction while CUs idle (a join costs a launch and the partial sums' traffic):
 // 128 x 8192 x 8192 58 -> 35 with four, 64 x 4096 x 4096 21 -> 15 with four instead of two; 1024^3 7.2 -> 12.5 with two.
+// Up to 64 fp32 tiles, whose products are slow, may split finer (forward and backward of 8192 x 64 -> 64 43 -> 32, 4096 x 512 -> 256 62
+// -> 51); 16-bit ones would lose (8192 x 256 -> 256 31 -> 38).
 enum { SMALL_11, SMALL_21, SMALL_22, TILE_64, TILE_128_64, TILE_128, TILE_256 };
 struct Plan {
   int kernel, splits;
@@ -955,7 +957,7 @@ Plan la_plan(long long M, long long N, long long K, int dtype, bool small_ok) {
   else if (t64 > 512) { p.kernel = TILE_128_64; tiles = t12864; }
   const long long kb = f32 ? 32 : 64, steps = la_div(K, kb);
   long long s = (p.kernel == TILE_256 ? 256 : 512) / tiles;
-  const long long least = f32 ? 32 : 16;               // tiles of 128 bytes a workgroup walks at least
+  const long long least = f32 && tiles > 64 ? 32 : f32 ? 8 : 16;      // tiles of 128 bytes a workgroup walks at least
   if (s > steps / least) s = steps / least;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
@@ -1107,11 +1109,11 @@ inline int la_strip(long long M, long long N, int dtype) {
   return (int)(s < 16 ? 16 : s);
 }
 
-// The backward pass: one launch where everything is small (contractions of at most 2048 and 4096); otherwise dz, db's strips and padded
+// The backward pass: one launch where everything is small (contractions of at most 4096); otherwise dz, db's strips and padded
 // copies, then dx, dW and db: at once on 64 x 64 tiles, one after the other on larger ones.  Forward and backward in a graph, one launch
 // against the others: fp32 up to 2^27 products (512^3 23 against 29 us, 1000 x 512 -> 256 31 against 42); 16-bit types, whose operands
 // in row order the small kernel reads value by value, up to 2^24 (72 x 256 -> 512 13.6 against 13.3, and two launches fewer for the
-// host; 512^3 18 against 16, 1000 x 512 -> 256 38 against 19).
+// host; 512^3 18 against 16, 1000 x 512 -> 256 38 against 19) and 512 rows (512 x 64 -> 64 15.5 against 14.6, 2000 x 64 -> 64 50 against 22).
 struct Backward {
   bool small, pair, own_dz;  // own_dz: dz is written (it is not dy itself)
   Plan px, pw;
@@ -1121,7 +1123,7 @@ struct Backward {
 Backward la_backward_plan(long long M, long long N, long long K, int dtype, const void *dy, long long ldy, bool slope, const void *x,
                           long long ldx, const void *w, long long ldw, int want) {
   Backward b{};
-  b.small = (double)M * N * K <= (double)(1 << (dtype == PN2_DT_F32 ? 27 : 24)) && M <= 2048 && N <= 4096 && (want & 3) && !((want & 4) && !(want & 2));
+  b.small = (double)M * N * K <= (double)(1 << (dtype == PN2_DT_F32 ? 27 : 24)) && M <= (dtype == PN2_DT_F32 ? 2048 : 512) && N <= 4096 && (want & 3) && !((want & 4) && !(want & 2));
   if (b.small) return b;
   const bool products = (want & 3) != 0;
   b.dz = {dy, M, N, ldy, false};
