@@ -109,6 +109,15 @@ __device__ __forceinline__ float hd_wave_max(float v) {
 
 __device__ __forceinline__ float hd_exp2(float v) { return __builtin_amdgcn_exp2f(v); }   // v_exp_f32: 1 ulp, flushes below 2^-126
 
+// n workgroups of `threads` threads.  The launch packet counts an axis in 32-bit threads, and 2^32 of them wrap without an error (67
+// million short rows had 3 of their results): what passes that goes to the second axis.  hd_block(): this workgroup's number, which
+// can then be n or more.
+inline dim3 hd_grid(long long n, unsigned threads) {
+  const long long most = 0xffffffffLL / threads, y = (n + most - 1) / most;
+  return y > 1 ? dim3((unsigned)((n + y - 1) / y), (unsigned)y) : dim3((unsigned)n);
+}
+__device__ __forceinline__ long long hd_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 constexpr float kHdInf = __builtin_huge_valf();
 constexpr float kHdLog2e = 1.4426950408889634f;
 constexpr float kHdLn2 = 0.6931471805599453f;

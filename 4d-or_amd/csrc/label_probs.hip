@@ -236,7 +236,7 @@ __device__ __forceinline__ void lp_place(const FwdArgs &a, long long row, const 
 // ------------------------------------------------------------------------------------------------ V <= 2048: a wave per row
 template <class T, int MODE, int EPL>
 __global__ __launch_bounds__(256) void lp_small_kernel(FwdArgs a) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long row = hd_block() * 4 + (threadIdx.x >> 6);
   if (row >= a.T) return;
   const int lane = pn2_lane();
   const typename T::elem *x = (const typename T::elem *)a.logits + row * a.ld;
@@ -480,7 +480,8 @@ __global__ __launch_bounds__(BT) void lp_row_kernel(FwdArgs a) {
   constexpr bool ENT = MODE == MODE_LABEL;
   typedef typename T::elem elem;
   __shared__ float sh_m[W], sh_s[W], sh_se[W];
-  const long long unit = blockIdx.x, row = SEG ? unit / a.nseg : unit;
+  const long long unit = hd_block(), row = SEG ? unit / a.nseg : unit;
+  if (row >= a.T) return;
   const int from = SEG ? (int)(unit - row * a.nseg) * a.seg : 0, V = SEG ? (a.V - from < a.seg ? a.V - from : a.seg) : a.V;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const elem *x = (const elem *)a.logits + row * a.ld + from;
@@ -700,9 +701,9 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
   constexpr int VE = T::kPerVec, U = 4;
   typedef typename T::elem elem;
   const int tid = threadIdx.x % GROUP;
-  const long long unit = GROUP == 256 ? (long long)blockIdx.x : (long long)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
+  const long long unit = GROUP == 256 ? hd_block() : hd_block() * (256 / GROUP) + threadIdx.x / GROUP;
   const long long nth = unit / a.nseg;
-  if (nth >= a.T) return;                              // (GROUP < 256 only: no barrier below is left behind)
+  if (nth >= a.T) return;                              // (a whole workgroup, or GROUP < 256: no barrier below is left behind)
   const long long row = a.T - 1 - nth;                 // the rows the forward pass read last may still be in the cache
   const int seg = (int)(unit - nth * a.nseg);
   const elem *x = (const elem *)a.logits + row * a.ld;
@@ -852,17 +853,16 @@ void lp_row_launch(const FwdArgs &a, hipStream_t st) {
   // Fewer rows than CUs: one big workgroup per row with its loads on their way at once (1 x 131072 bf16 with 20 alternatives 15 us, 25
   // with 512 threads).  Otherwise several workgroups per CU, smaller ones for short rows, whose time is the selection's round trips
   // (8192 x 16384 bf16 with 20 alternatives: 95 us with 256 threads, 122 with 512; 8192 x 131072: 0.43 ms with 512).
-  const unsigned grid = (unsigned)a.T;
   const int nvec = (a.V + T::kPerVec - 1) / T::kPerVec;
-  if (nvec > 1024 && a.T <= 256) lp_row_kernel<T, MODE, TOP, 1024, 8, false><<<grid, 1024, 0, st>>>(a);
-  else if (nvec <= 4096) lp_row_kernel<T, MODE, TOP, 256, 4, false><<<grid, 256, 0, st>>>(a);
-  else lp_row_kernel<T, MODE, TOP, 512, 4, false><<<grid, 512, 0, st>>>(a);
+  if (nvec > 1024 && a.T <= 256) lp_row_kernel<T, MODE, TOP, 1024, 8, false><<<hd_grid(a.T, 1024), 1024, 0, st>>>(a);
+  else if (nvec <= 4096) lp_row_kernel<T, MODE, TOP, 256, 4, false><<<hd_grid(a.T, 256), 256, 0, st>>>(a);
+  else lp_row_kernel<T, MODE, TOP, 512, 4, false><<<hd_grid(a.T, 512), 512, 0, st>>>(a);
 }
 
 template <class T, int MODE>
 int lp_forward(const FwdArgs &a, hipStream_t st) {
   if (a.V <= kSmallV) {
-    const unsigned grid = (unsigned)((a.T + 3) / 4);
+    const dim3 grid = hd_grid((a.T + 3) / 4, 256);
     if (a.V <= 64) lp_small_kernel<T, MODE, 1><<<grid, 256, 0, st>>>(a);
     else if (a.V <= 256) lp_small_kernel<T, MODE, 4><<<grid, 256, 0, st>>>(a);
     else if (a.V <= 1024) lp_small_kernel<T, MODE, 16><<<grid, 256, 0, st>>>(a);
@@ -886,12 +886,11 @@ int lp_backward(BwdArgs a, hipStream_t st) {
   if (a.V <= kSmallV) {
     a.nseg = (nvec + 255) / 256;                       // 64 lanes x 4 vectors
     const long long units = a.T * a.nseg;
-    lp_grad_kernel<T, MODE, 64><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a);
+    lp_grad_kernel<T, MODE, 64><<<hd_grid((units + 3) / 4, 256), 256, 0, st>>>(a);
   } else {
     a.nseg = (nvec + 1023) / 1024;
     const long long units = a.T * a.nseg;
-    if (units > 0x7fffffffLL) return PN2_EINVAL;
-    lp_grad_kernel<T, MODE, 256><<<(unsigned)units, 256, 0, st>>>(a);
+    lp_grad_kernel<T, MODE, 256><<<hd_grid(units, 256), 256, 0, st>>>(a);
   }
   return pn2_check_launch();
 }

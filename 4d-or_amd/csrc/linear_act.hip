@@ -537,7 +537,8 @@ __device__ __forceinline__ void la_tile(const Product &a, int gi, int gj, int id
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ, int ACT>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void la_tile_kernel(Product a, int gi, int gj) {
   __shared__ __align__(1024) char ring[2 * (WI * TI + WJ * TJ) * 16 * 128];
-  la_tile<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT>(a, gi, gj, blockIdx.x, blockIdx.z, ring);
+  const int id = (int)hd_block();
+  if (id < gi * gj) la_tile<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT>(a, gi, gj, id, blockIdx.z, ring);
 }
 
 // the split contraction joined in a fixed order, then the epilogue: four consecutive results per thread; the first `blocks`
@@ -601,7 +602,7 @@ __device__ __forceinline__ void la_pad(const Copies &c_, unsigned id) {
 
 template <class T>
 __global__ __launch_bounds__(256) void la_pad_kernel(Copies c) {
-  la_pad<T>(c, blockIdx.x);
+  la_pad<T>(c, (unsigned)hd_block());
 }
 
 // ----------------------------------------------------------------------------------------------------- the small kernels
@@ -774,8 +775,8 @@ template <class T, int TI, int TJ, int W>
 __global__ __launch_bounds__(64 * W) void la_small_kernel(Product a) {
   __shared__ __align__(16) float lds[W * TI * TJ * 256];
   const long long gi = (a.M + 16 * TI - 1) / (16 * TI);
-  la_small_tile<T, false, false, TI, TJ, W, false>(Small{a, nullptr, 0}, blockIdx.x % gi * (16 * TI), blockIdx.x / gi * (16 * TJ), nullptr, 0,
-                                                   lds);
+  const long long id = hd_block(), i0 = id % gi * (16 * TI), j0 = id / gi * (16 * TJ);
+  if (j0 < a.N) la_small_tile<T, false, false, TI, TJ, W, false>(Small{a, nullptr, 0}, i0, j0, nullptr, 0, lds);
 }
 
 // dx and dW (and db) in one launch: the first `ndx` workgroups take tiles of dx, the others of dW
@@ -798,8 +799,9 @@ __global__ __launch_bounds__(256) void la_small_grad_kernel(Small x, Small w, in
 template <class T, bool SLOPE>
 __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, int strip, const void *dy_, long long ldy,
                                                     const void *slope_, void *dz_, long long ldz, float *part, unsigned blocks, Copies copies) {
-  if (blockIdx.x >= blocks) {
-    la_pad<T>(copies, blockIdx.x - blocks);
+  const unsigned id = (unsigned)hd_block();
+  if (id >= blocks) {
+    la_pad<T>(copies, id - blocks);
     return;
   }
   typedef typename T::elem elem;
@@ -807,8 +809,8 @@ __global__ __launch_bounds__(256) void la_dz_kernel(long long M, long long N, in
   constexpr int VE = T::kPerVec, U = 4;
   __shared__ float sum[3][64][VE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const unsigned across = (unsigned)((N + 64 * VE - 1) / (64 * VE)), down = blockIdx.x / across;
-  const long long j = ((long long)(blockIdx.x - down * across) * 64 + lane) * VE, left = N - j;
+  const unsigned across = (unsigned)((N + 64 * VE - 1) / (64 * VE)), down = id / across;
+  const long long j = ((long long)(id - down * across) * 64 + lane) * VE, left = N - j;
   const long long i0 = (long long)down * strip, i1 = i0 + strip < M ? i0 + strip : M;
   float s[VE];
 #pragma unroll
@@ -1015,8 +1017,9 @@ inline unsigned la_joins(const Product &a) { return a.splits > 1 ? (unsigned)la_
 template <class T, bool PROWS, bool QROWS, int WI, int WJ, int TI, int TJ>
 void la_tile_as(const Product &a, hipStream_t st) {
   const int gi = (int)la_div(a.M, WI * TI * 16), gj = (int)la_div(a.N, WJ * TJ * 16);
-  const dim3 grid((unsigned)(gi * gj), 1, (unsigned)a.splits);
   constexpr int NT = 64 * WI * WJ;
+  dim3 grid = hd_grid(gi * gj, NT);
+  grid.z = (unsigned)a.splits;
   if constexpr (PROWS || QROWS) {
     la_tile_kernel<T, PROWS, QROWS, WI, WJ, TI, TJ, ACT_NONE><<<grid, NT, 0, st>>>(a, gi, gj);
   } else {
@@ -1033,7 +1036,7 @@ void la_tile_as(const Product &a, hipStream_t st) {
 
 template <class T, int TI, int TJ, int W>
 void la_small_as(const Product &a, hipStream_t st) {
-  la_small_kernel<T, TI, TJ, W><<<(unsigned)(la_div(a.M, 16 * TI) * la_div(a.N, 16 * TJ)), 64 * W, 0, st>>>(a);
+  la_small_kernel<T, TI, TJ, W><<<hd_grid(la_div(a.M, 16 * TI) * la_div(a.N, 16 * TJ), 64 * W), 64 * W, 0, st>>>(a);
 }
 
 Product la_arguments(const Plan &plan, const Matrix &p, const Matrix &q, long long M, long long N, long long K, const Epilogue &e, Space ws) {
@@ -1095,7 +1098,7 @@ int la_forward(Forward f, long long M, long long N, long long K, int dtype, cons
   Space space{(char *)ws};
   if (f.plan.kernel >= TILE_64) {
     const Copies c = la_copies<T>(&f.x, &f.w, dtype, space);
-    if (c.all) la_pad_kernel<T><<<c.all, 256, 0, st>>>(c);
+    if (c.all) la_pad_kernel<T><<<hd_grid(c.all, 256), 256, 0, st>>>(c);
   }
   return la_product<T, false, false>(f.plan, f.x, f.w, M, N, K, e, space, st);
 }
@@ -1164,10 +1167,11 @@ int la_backward(Backward b, long long M, long long N, long long K, int dtype, co
   const Sums sums{part, N, (int)la_div(M, strip), db_f32, db};
   if (b.own_dz || db) {
     const unsigned blocks = (unsigned)(la_div(N, 64 * T::kPerVec) * sums.strips);
-    if (slope) la_dz_kernel<T, true><<<blocks + c.all, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, ldz, part, blocks, c);
-    else la_dz_kernel<T, false><<<blocks + c.all, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, dz, ldz, part, blocks, c);
+    const dim3 grid = hd_grid((long long)blocks + c.all, 256);
+    if (slope) la_dz_kernel<T, true><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, slope, dz, ldz, part, blocks, c);
+    else la_dz_kernel<T, false><<<grid, 256, 0, st>>>(M, N, strip, dy, ldy, nullptr, dz, ldz, part, blocks, c);
   } else if (c.all) {
-    la_pad_kernel<T><<<c.all, 256, 0, st>>>(c);
+    la_pad_kernel<T><<<hd_grid(c.all, 256), 256, 0, st>>>(c);
   }
   if (b.own_dz) {
     b.dz.p = b.dzr.p = dz;

@@ -1,0 +1,80 @@
+"""Dense-head operators where the documentation allows a call that small sizes do not reach: launches past 2^32 threads, NaN before
+every activation, slots that are unused in two ways, the kernels of the largest tiles and rows.  Oracles and bounds: test_gpu_head_ops."""
+import math
+
+import pytest
+import torch
+
+from pointnet2_ops import head_ops as ho
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------- more threads than 32 bits count
+def test_label_rows_past_two_to_the_32_threads():
+    """2^26 + 5 rows of two columns: 64 threads a row.  Every row by its formula; expm1 and log1p of the difference in fp32 are good
+    to a few u, the kernels' sums of two terms to less than 16 u of 1 + |difference|."""
+    T = 2 ** 26 + 5
+    x = torch.zeros(T, 2, dtype=torch.bfloat16, device="cuda")
+    x[:, 1] = (torch.arange(T, device="cuda") % 7).to(torch.bfloat16)
+    y = torch.arange(T, device="cuda") % 2
+    leaf = x.requires_grad_()
+    r = ho.label_log_probs(leaf, y, top=1)
+    d = x.detach()[:, 1].float()
+    tol = 16 * 2.0 ** -24 * (1 + d)
+    lse = d + torch.log1p(torch.exp(-d))
+    assert bool(((r.log_prob - (torch.where(y == 1, d, 0.0) - lse)).abs() <= tol).all())
+    assert torch.equal(r.top_index[:, 0], (d > 0).long())
+    g, = torch.autograd.grad(r.log_prob, leaf, torch.ones(T, device="cuda"))
+    p1 = torch.sigmoid(d)
+    want = torch.where(y == 1, 1 - p1, -p1)                         # d log p_y / d x_1
+    assert bool(((g[:, 1].float() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * tol).all())
+    assert bool(((g[:, 0].float() + want).abs() <= 2.0 ** -8 * want.abs() + 4 * tol).all())
+
+
+def test_distillation_rows_past_two_to_the_32_threads():
+    """One entry of the teacher: q = 1, loss = -log p of it."""
+    T = 2 ** 26 + 5
+    x = torch.zeros(T, 2, dtype=torch.bfloat16, device="cuda")
+    x[:, 1] = (torch.arange(T, device="cuda") % 7).to(torch.bfloat16)
+    index, value = (torch.arange(T, device="cuda") % 2)[:, None], torch.zeros(T, 1, device="cuda")
+    leaf = x.requires_grad_()
+    loss = ho.distill_top_k(leaf, index, value)
+    d = x.detach()[:, 1].float()
+    tol = 16 * 2.0 ** -24 * (1 + d)
+    on = index[:, 0] == 1
+    assert bool(((loss - (d + torch.log1p(torch.exp(-d)) - torch.where(on, d, 0.0))).abs() <= tol).all())
+    g, = torch.autograd.grad(loss, leaf, torch.ones(T, device="cuda"))
+    p1 = torch.sigmoid(d)
+    want = torch.where(on, p1 - 1, p1)
+    assert bool(((g[:, 1].float() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * tol).all())
+
+
+def test_long_label_rows_past_two_to_the_32_threads():
+    """A workgroup per row: 2^24 + 3 rows that are one row of 2056 columns (row stride 0)."""
+    T, V = 2 ** 24 + 3, 2056
+    row = torch.randn(1, V, generator=torch.Generator().manual_seed(0)).to(torch.float16).cuda()
+    y = torch.arange(T, device="cuda") % V
+    r = ho.label_log_probs(row.expand(T, V), y)
+    want = ho.label_log_probs(row.expand(V, V), torch.arange(V, device="cuda"))
+    assert torch.equal(r.log_prob, want.log_prob[y]) and bool((r.entropy == want.entropy[0]).all())
+
+
+def test_linear_rows_past_two_to_the_32_threads():
+    """One column to one column: M results in M / 32 workgroups of the small kernel (products of small whole numbers: exact)."""
+    M = 2 ** 29 + 37
+    x = (torch.arange(M, device="cuda") % 5).to(torch.bfloat16)[:, None]
+    y = ho.linear_act(x, torch.full((1, 1), 3.0, dtype=torch.bfloat16, device="cuda"))
+    assert torch.equal(y, x * 3)
+
+
+def test_linear_gradient_rows_past_two_to_the_32_threads():
+    """dx of 2^31 - 1 rows: M / 128 tiles of 256 threads."""
+    M = 2 ** 31 - 1
+    leaf = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda").expand(M, 1).requires_grad_()
+    y = ho.linear_act(leaf, torch.full((1, 8), 3.0, dtype=torch.bfloat16, device="cuda")[:, :1])
+    dy = torch.zeros(M, 8, dtype=torch.bfloat16, device="cuda")[:, :1]          # (rows at whole 16 bytes: no copies)
+    dy[-200:, 0] = torch.arange(200, device="cuda").to(torch.bfloat16)
+    dy[:200, 0] = 1.0
+    dx, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(dx[-200:], 3 * dy[-200:]) and bool((dx[:200] == 3).all()) and not dx[200:-200].any()
