@@ -8,9 +8,13 @@
 // PN2_HIP_LIB stays in force.
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
@@ -99,6 +103,28 @@ Tensor matrix(const Tensor &t, const char *name) {
 }
 int64_t row_stride(const Tensor &m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
 
+// A launch goes around torch's dispatcher, so what the dispatcher would do beside it has to be refused here, or it would be left out
+// without a word: the tangent of a forward-mode dual tensor, the node of a recorded graph (which would hold the outputs' allocation and
+// no kernel), the code of a tensor subclass, the values of a tensor without memory of its own.
+void check_plain(const char *op, std::initializer_list<std::pair<const Tensor *, const char *>> inputs) {
+  bool recorded = torch::jit::tracer::isTracing();
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set()) {
+    using c10::impl::TorchDispatchModeKey;
+    for (const auto key : {TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL, TorchDispatchModeKey::FAKE})
+      recorded |= c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
+  }
+  recorded |= c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  TORCH_CHECK(!recorded, op, " cannot be recorded (torch.jit.trace, make_fx, export): its kernels run outside torch's dispatcher");
+  const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const auto &[t, name] : inputs) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(!t->unsafeGetTensorImpl()->is_python_dispatch(), name, " must be a plain tensor, not a subclass with __torch_dispatch__");
+    TORCH_CHECK(!forward_mode || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative (", name, " is a dual tensor)");
+    TORCH_CHECK(t->layout() == at::kStrided && t->has_storage() && (t->numel() == 0 || t->storage().data()), name,
+                " must be a dense tensor with memory of its own");
+  }
+}
+
 void check_device(const Tensor &lead, std::initializer_list<std::pair<const Tensor *, const char *>> others) {
   TORCH_CHECK(lead.is_cuda(), "CPU not supported");
   for (const auto &[t, name] : others) {
@@ -164,6 +190,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
     Tensor dx, dw, db;
     if (need & 7) {
+      check_plain("linear_act's gradient", {{&grads[0], "dy"}});
       const Tensor dy = matrix(grads[0], "dy");
       const int64_t M = dy.size(0), N = dy.size(1);
       const int dt = dtype_code(dy, "dy");
@@ -193,6 +220,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 
 Tensor linear_act(const Tensor &x, const Tensor &weight, const std::optional<Tensor> &bias, int64_t act,
                   const std::optional<Tensor> &residual, bool timed) {
+  const Tensor none;
+  check_plain("linear_act", {{&x, "x"}, {&weight, "weight"}, {bias ? &*bias : &none, "bias"}, {residual ? &*residual : &none, "residual"}});
   const Tensor xm = matrix(x, "x");
   dtype_code(xm, "x");
   const int64_t K = xm.size(1);
@@ -267,6 +296,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     return {o.log_prob, o.entropy, o.top_log_prob, o.top_index};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_plain("label_log_probs' gradient", {{&grads[0], "the gradient of log_prob"}, {&grads[1], "the gradient of entropy"}});
     const Tensor g = grad_rows(grads[0]), h = grad_rows(grads[1]);
     Tensor dx;
     if (g.defined() || h.defined()) {
@@ -287,6 +317,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
 
 std::tuple<Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>> label_log_probs(const Tensor &logits, const Tensor &labels,
                                                                                          int64_t top, int64_t ignore, bool timed) {
+  check_plain("label_log_probs", {{&logits, "logits"}, {&labels, "labels"}});
   const Tensor x = matrix(logits, "logits");
   dtype_code(x, "logits");
   TORCH_CHECK(labels.scalar_type() == at::kLong, "labels must be a long tensor");
@@ -353,6 +384,7 @@ struct DistillTopK : torch::autograd::Function<DistillTopK> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &index = saved[1], &values = saved[2], &stats = saved[3];
+    check_plain("distill_top_k's gradient", {{&grads[0], "the gradient of the loss"}});
     const Tensor g = grad_rows(grads[0]);
     const int64_t T = x.size(0), V = x.size(1);
     Tensor dx = at::empty({T, V}, x.options());
@@ -367,6 +399,7 @@ struct DistillTopK : torch::autograd::Function<DistillTopK> {
 };
 
 Tensor distill_top_k(const Tensor &logits, const Tensor &teacher_index, const Tensor &teacher_logits, double temperature, bool timed) {
+  check_plain("distill_top_k", {{&logits, "logits"}, {&teacher_index, "teacher_index"}, {&teacher_logits, "teacher_logits"}});
   const Tensor x = matrix(logits, "logits");
   dtype_code(x, "logits");
   TORCH_CHECK(teacher_index.scalar_type() == at::kLong, "teacher_index must be a long tensor");

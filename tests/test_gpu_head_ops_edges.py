@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from pointnet2_ops import head_ops as ho
 
@@ -78,3 +79,40 @@ def test_linear_gradient_rows_past_two_to_the_32_threads():
     dy[:200, 0] = 1.0
     dx, = torch.autograd.grad(y, leaf, dy)
     assert torch.equal(dx[-200:], 3 * dy[-200:]) and bool((dx[:200] == 3).all()) and not dx[200:-200].any()
+
+
+# -------------------------------------------------------------------------------------- what goes around torch's dispatcher
+@pytest.mark.filterwarnings("ignore")
+def test_forward_mode_and_recording_are_refused_and_onlookers_are_not():
+    import torch.autograd.forward_ad as fwd
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    gen = torch.Generator().manual_seed(1)
+    x, w = torch.randn(6, 40, generator=gen).cuda(), torch.randn(9, 40, generator=gen).cuda()
+    y, index, value = torch.arange(6).cuda(), torch.arange(12).view(6, 2).cuda() % 9, torch.randn(6, 2, generator=gen).cuda()
+    calls = [lambda t: ho.linear_act(t, w, None, "silu"), lambda t: ho.label_log_probs(t, y, top=2).log_prob,
+             lambda t: ho.distill_top_k(t, index, value)]
+    for call in calls:
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(fwd.make_dual(x, x))
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(call, (x,))
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(call)(x)
+        with pytest.raises(RuntimeError, match="memory of its own"):
+            torch.func.functionalize(call)(x)
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    def step(call):
+        leaf = x.clone().requires_grad_()
+        out = torch.utils.checkpoint.checkpoint(call, leaf, use_reentrant=False)
+        return out, torch.autograd.grad(out.sum(), leaf)[0]
+    for call in calls:
+        want = step(call)
+        with Watch():
+            got = step(call)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        assert torch.equal(torch.compile(call, backend="eager")(x), want[0])      # (compiled around the call, not through it)

@@ -114,3 +114,71 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
         return lib.pn2_distill_topk(T, V, V, 0, x, k, some, tdt, some, t, some, None, None, nb, None)
     assert distill(k=0) == distill(t=0.0) == distill(t=-1.0) == distill(t=float("nan")) == distill(t=float("inf")) == EINVAL
     assert distill(tdt=3) == EINVAL and distill(x=None) == ENULL
+
+
+# ------------------------------------------- what torch's dispatcher would do beside the launch is refused before the device is looked at
+def _calls():
+    y, i = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 1, dtype=torch.int64)
+    return {"linear_act x": lambda t: ho.linear_act(t, f(4, 3)), "linear_act weight": lambda t: ho.linear_act(f(2, 3), t),
+            "linear_act residual": lambda t: ho.linear_act(f(2, 3), f(3, 3), residual=t),
+            "linear_act bias": lambda t: ho.linear_act(f(2, 3), f(3, 3), t[0]), "linear_act grad": lambda t: ho.linear_act(t, f(4, 3).requires_grad_()),
+            "label_log_probs logits": lambda t: ho.label_log_probs(t, y).log_prob,
+            "distill_top_k logits": lambda t: ho.distill_top_k(t, i, f(2, 1)),
+            "distill_top_k teacher_logits": lambda t: ho.distill_top_k(f(2, 3), torch.zeros(2, 3, dtype=torch.int64), t)}
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_forward_mode_is_refused(name):
+    import torch.autograd.forward_ad as fwd
+    call = _calls()[name]
+    with fwd.dual_level():
+        dual = fwd.make_dual(f(2, 3), torch.ones(2, 3))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual)
+    with pytest.raises(RuntimeError, match="CPU not supported"):      # (the same call without a tangent gets as far as the device)
+        call(f(2, 3))
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+@pytest.mark.filterwarnings("ignore")
+def test_recording_is_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call = _calls()[name]
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        torch.jit.trace(call, (f(2, 3),))
+    for mode in ("real", "symbolic"):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(call, tracing_mode=mode, _allow_non_fake_inputs=True)(f(2, 3))
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        make_fx(call, pre_dispatch=True)(f(2, 3))
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_tensors_that_are_not_plain_memory_are_refused(name):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Sub(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*[torch.Tensor(a) if isinstance(a, cls) else a for a in args], **(kwargs or {}))
+    call = _calls()[name]
+    if name != "linear_act bias":                                     # (whose row is a plain tensor by then)
+        with pytest.raises(RuntimeError, match="plain tensor"):
+            call(torch.Tensor._make_subclass(Sub, f(2, 3)))
+    with pytest.raises(RuntimeError):
+        torch.func.functionalize(call)(f(2, 3))
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        call(torch._efficientzerotensor((3, 3))[1:])
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        call(f(2, 3).to_sparse())
+    for transform in (torch.vmap, torch.func.grad, lambda g: lambda t: torch.func.jvp(g, (t,), (t,))):
+        with pytest.raises(RuntimeError):
+            transform(call)(f(2, 2, 3) if transform is torch.vmap else f(2, 3))
+
+    class Watch(TorchDispatchMode):                                   # a mode that only looks on is none of these
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Watch(), pytest.raises(RuntimeError, match="CPU not supported"):
+        call(f(2, 3))
