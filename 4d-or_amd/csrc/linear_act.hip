@@ -73,8 +73,9 @@ __device__ __forceinline__ void la_act(float z, float &y, float &d) {
       d = __fmaf_rn(z * 0.3989422804014327f, e, cdf);
     }
   } else {
-    // (1 + tanh u) / 2 = 1 / (1 + e^(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3); beyond |z| = 30 the gate is 0 or 1
-    const float w = fminf(fmaxf(z, -30.f), 30.f), w2 = w * w;
+    // (1 + tanh u) / 2 = 1 / (1 + e^(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3); beyond |z| = 30 the gate is 0 or 1 (fminf and fmaxf
+    // would turn a NaN into -30, and its slope into 0)
+    const float w = z != z ? z : fminf(fmaxf(z, -30.f), 30.f), w2 = w * w;
     const float u2 = 1.5957691216057308f * w * __fmaf_rn(0.044715f, w2, 1.f);
     const float g = __builtin_amdgcn_rcpf(1.f + hd_exp2(-kHdLog2e * u2));
     y = z * g;

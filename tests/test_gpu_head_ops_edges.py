@@ -116,3 +116,47 @@ def test_forward_mode_and_recording_are_refused_and_onlookers_are_not():
             got = step(call)
         assert all(torch.equal(a, b) for a, b in zip(want, got))
         assert torch.equal(torch.compile(call, backend="eager")(x), want[0])      # (compiled around the call, not through it)
+
+
+# ------------------------------------------------------------------------------------------- NaN and infinities before an activation
+@pytest.mark.parametrize("act", ho.ACTIVATIONS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N", [(3, 8), (70, 130), (2100, 1040)], ids=["few", "small", "tiles"])
+def test_linear_act_nan_reaches_every_gradient(M, N, dtype, act):
+    """Row 2 of x is NaN in one place: y's row, d x's row through the slope and every entry of d bias are NaN; where the activation has
+    no slope of its own at NaN (none: 1, relu: 1, as torch's) d x stays that of a slope of 1.  The other rows are untouched."""
+    gen = torch.Generator().manual_seed(3)
+    x, w = torch.randn(M, 40, generator=gen).to(dtype).cuda(), (torch.randn(N, 40, generator=gen) / 6).to(dtype).cuda()
+    b, dy = torch.zeros(N, device="cuda", dtype=dtype), torch.randn(M, N, generator=gen).to(dtype).cuda()
+
+    def run(x):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = ho.linear_act(*leaves, act)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    clean = run(x)
+    x[2, 3] = float("nan")
+    y, dx, dw, db = run(x)
+    rest = torch.arange(M, device="cuda") != 2
+    assert torch.equal(y[rest], clean[0][rest]) and torch.equal(dx[rest], clean[1][rest])
+    assert y[2].isnan().all()
+    if act in ("none", "relu"):
+        assert dx[2].isfinite().all() and db.isfinite().all()
+    else:
+        assert dx[2].isnan().all() and db.isnan().all() and dw.isnan().all()
+    assert dw[:, 3].isnan().all()                                   # d w = d z^T x: x itself is NaN there
+    assert torch.equal(dw.isnan().all(1), torch.ones(N, dtype=torch.bool, device="cuda")) == (act not in ("none", "relu"))
+
+
+@pytest.mark.parametrize("act", ho.ACTIVATIONS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_linear_act_far_and_infinite_arguments(act, dtype):
+    """z from the bias: large finite values are exact (z or 0, slope 1 or 0), +inf stays +inf."""
+    big = 3e4 if dtype == torch.float16 else 1e30
+    b = torch.tensor([-big, -200.0, 200.0, big], device="cuda", dtype=dtype)
+    x, w = torch.zeros(3, 16, device="cuda", dtype=dtype), torch.ones(4, 16, device="cuda", dtype=dtype)
+    leaf = x.clone().requires_grad_()
+    y = ho.linear_act(leaf, w, b, act)
+    assert torch.equal(y, (b if act == "none" else b.clamp_min(0)).expand(3, 4))
+    g, = torch.autograd.grad(y, leaf, torch.ones(3, 4, device="cuda", dtype=dtype))
+    assert torch.equal(g, torch.full_like(g, 4.0 if act == "none" else 2.0))
+    assert (ho.linear_act(x, w, b.new_full((4,), math.inf), act) == math.inf).all()
