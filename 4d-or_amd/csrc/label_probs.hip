@@ -156,7 +156,7 @@ __device__ __forceinline__ void lp_finish_label(const FwdArgs &a, long long row,
 }
 
 // One wave finishes a distillation row.  An unused slot has a negative index or the value -inf; a row without a used slot
-// has no loss (and its logits were not read: r is not looked at).  An index >= V makes the row NaN.
+// has no loss (and its logits were not read: r is not looked at).  An index >= V of a used slot makes the row NaN.
 __device__ __forceinline__ bool lp_teacher_any(const FwdArgs &a, long long row) {
   bool any = false;
   for (int j = pn2_lane(); j < a.k; j += PN2_WAVE)
@@ -182,8 +182,9 @@ __device__ __forceinline__ void lp_finish_distill(const FwdArgs &a, long long ro
   bool bad = false;
   for (int j = lane; j < a.k; j += PN2_WAVE) {
     const long long i = a.t_idx[at + j];
-    if (i >= 0) tm = fmaxf(tm, lp_teacher(a, at + j));
-    bad |= i >= a.V;
+    const float t = lp_teacher(a, at + j);
+    if (i >= 0) tm = fmaxf(tm, t);
+    bad |= i >= a.V && !(t == -kHdInf);
   }
   tm = hd_wave_max(tm);
   bad = __ballot(bad) != 0;

@@ -955,7 +955,7 @@ int pn2_label_logprobs_grad(long long T, int V, long long ld, int dtype, const v
  * teacher_logits (T, k) of `teacher_dtype`;  with q = softmax(teacher / temperature) over the row's used slots and
  * p = softmax(logits / temperature) over all V:   loss (T) f32 = temperature^2 sum_j q_j (log q_j - log p[index_j]).
  * A slot with a negative index or the value -inf is unused; a row without a used slot has loss 0 and gradient 0 (its logits are
- * not read).  An index >= V makes the row NaN.  An index may occur more than once.  stats (T, 4) f32 for the gradient, or NULL.
+ * not read).  An index >= V of a used slot makes the row NaN.  An index may occur more than once.  stats (T, 4) f32 for the gradient, or NULL.
  * The workspace: as above.
  * The gradient: dlogits (T, V) dense = g_loss temperature (p - sum_j q_j [index_j = v]), every element written, rounded once. */
 size_t pn2_distill_topk_workspace_bytes(long long T, int V, int dtype);

@@ -160,3 +160,24 @@ def test_linear_act_far_and_infinite_arguments(act, dtype):
     g, = torch.autograd.grad(y, leaf, torch.ones(3, 4, device="cuda", dtype=dtype))
     assert torch.equal(g, torch.full_like(g, 4.0 if act == "none" else 2.0))
     assert (ho.linear_act(x, w, b.new_full((4,), math.inf), act) == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [15, 700, 5000, 140000])
+def test_distillation_slots_unused_by_value_at_any_index(V, dtype):
+    """A slot of value -inf is unused whatever its index, past the columns too: losses and gradients of the row without it."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(3, V, generator=gen).to(dtype).cuda()
+    index = torch.tensor([[3, 7, V, V + 9, 2 ** 40], [V - 1, V, V, V, V], [V, V, V, V, V]]).cuda()
+    value = torch.tensor([[0.5, -1.0] + [-math.inf] * 3, [2.0] + [-math.inf] * 4, [-math.inf] * 5]).cuda()
+    as_padding = torch.where(value == -math.inf, -1, index)
+
+    def run(index, value):
+        leaf = x.clone().requires_grad_()
+        loss = ho.distill_top_k(leaf, index, value, 1.5)
+        return loss.detach(), torch.autograd.grad(loss, leaf, torch.ones(3, device="cuda"))[0]
+    got, want = run(index, value), run(as_padding, value)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0].isfinite().all()
+    # a used slot past the columns still says so
+    bad = run(torch.where(index == V + 9, V, index), torch.where(index == V + 9, 0.0, value))
+    assert bad[0][0].isnan() and bad[1][0].isnan().all() and torch.equal(bad[0][1:], want[0][1:])
