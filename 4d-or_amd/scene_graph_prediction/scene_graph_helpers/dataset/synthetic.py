@@ -51,7 +51,13 @@ def synthetic_scan(n_obj=9, points_obj=4000, points_rel=8000, num_class=12, num_
 
 
 def to_device(batch, device):
-    return {k: (v.to(device) if (torch.is_tensor(v) or hasattr(v, "node_ptr")) else v) for k, v in batch.items()}
+    def move(v):
+        if torch.is_tensor(v) or hasattr(v, "node_ptr"):
+            return v.to(device)
+        if type(v) in (tuple, list) and any(torch.is_tensor(t) for t in v):      # (teacher_rels)
+            return type(v)(move(t) for t in v)
+        return v
+    return {k: move(v) for k, v in batch.items()}
 
 
 def collate_scans(scans):
