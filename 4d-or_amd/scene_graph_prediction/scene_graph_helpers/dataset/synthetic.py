@@ -65,7 +65,7 @@ def collate_scans(scans):
     main.py:54-56, and leaves 90 % of the GPU idle on 9 + 72 small clouds).  Clouds are concatenated along the batch
     axis, `edge_indices` are offset by each scan's first node row, and `scenes` (a SceneBatch) records the node / edge
     row ranges so that the GCN's BatchNorm statistics and the loss average stay PER SCAN.  Per-scan metadata becomes
-    lists (`scan_ids`, `objs_jsons`, `take_idxs`)."""
+    lists (`scan_ids`, `objs_jsons`, `take_idxs`).  A teacher's predicates (`teacher_rels`) are concatenated by edge."""
     from scene_graph_prediction.scene_graph_helpers.model.gcns.network_TripletGCN import SceneBatch
     node_ptr, edge_ptr = [0], [0]
     for s in scans:
@@ -80,4 +80,10 @@ def collate_scans(scans):
     batch["take_idxs"] = [s.get("take_idx", 0) for s in scans]
     if all("full_image_features" in s for s in scans):
         batch["full_image_features"] = torch.stack([s["full_image_features"] for s in scans])     # (S, 6, F)
+    teachers = [s["teacher_rels"] for s in scans if s.get("teacher_rels") is not None]
+    if teachers:
+        # all of them with the same number of alternatives: a scan without would train without its term unnoticed
+        if len(teachers) != len(scans) or len({t.size(1) for pair in teachers for t in pair}) != 1:
+            raise ValueError("collate_scans: teacher_rels must be there for every scan, with one number of alternatives, or for none")
+        batch["teacher_rels"] = tuple(torch.cat(parts, dim=0) for parts in zip(*teachers))
     return batch

@@ -19,3 +19,18 @@ def test_to_device_moves_a_teachers_tensors():
     assert moved["obj_points"].device.type == "meta" and moved["objs_json"] is s["objs_json"] and moved["scan_id"] == "s1"
     assert [t.device.type for t in to_device(dict(s, teacher_rels=list(s["teacher_rels"])), "meta")["teacher_rels"]] == ["meta"] * 2
     assert to_device(dict(s, crop=(1, 2)), "meta")["crop"] == (1, 2)
+
+
+def test_collate_scans_keeps_a_teachers_predicates():
+    from scene_graph_prediction.scene_graph_helpers.dataset.synthetic import collate_scans
+    scans = [scan(3, 1), scan(2, 2), scan(4, 3)]
+    batch = collate_scans(scans)
+    for got, parts in zip(batch["teacher_rels"], zip(*[s["teacher_rels"] for s in scans])):
+        assert torch.equal(got, torch.cat(parts)) and got.size(0) == batch["rel_points"].size(0)
+    plain = [{k: v for k, v in s.items() if k != "teacher_rels"} for s in scans]
+    assert "teacher_rels" not in collate_scans(plain)
+    assert "teacher_rels" not in collate_scans([dict(s, teacher_rels=None) for s in plain])
+    with pytest.raises(ValueError, match="teacher_rels"):
+        collate_scans([scans[0], plain[1]])
+    with pytest.raises(ValueError, match="teacher_rels"):
+        collate_scans([scans[0], scan(3, 4, k=3)])
