@@ -234,7 +234,14 @@ class SGPNModelWrapper(nn.Module):
         if teacher is not None:                                     # another model's best predicates (teacher_relations below)
             from pointnet2_ops.head_ops import distill_top_k
             t = float(self.mconfig.get("distill_temperature", 1.0))
-            total = total + float(self.mconfig.get("lambda_distill", 1.0)) * distill_top_k(rel_pred, teacher[0], teacher[1], t).mean()
+            rows = distill_top_k(rel_pred, teacher[0], teacher[1], t)
+            if scenes is None:
+                loss_distill = rows.mean()
+            else:
+                # the mean of every scan's mean, like the terms above (weights and one sum: no atomics; a scan has an edge at least)
+                edges = scenes.edge_ptr[1:] - scenes.edge_ptr[:-1]
+                loss_distill = (rows / (edges * scenes.num_scenes)[scenes.edge_scene].to(rows.dtype)).sum()
+            total = total + float(self.mconfig.get("lambda_distill", 1.0)) * loss_distill
         return total
 
     @torch.no_grad()
