@@ -57,7 +57,8 @@ class _Head(BaseNetwork):
         self.fc2 = nn.Linear(512, 256)
 
     def _trunk(self, x, use_bn, scan_ptr=None):
-        if self.fused_linear and x.is_cuda and not use_bn and x.dtype == self.fc1.weight.dtype:     # (autocast: the library's)
+        if (self.fused_linear and x.is_cuda and not use_bn and x.dtype == self.fc1.weight.dtype
+                and not torch.is_autocast_enabled("cuda")):            # (autocast chooses the types of the library's products)
             from pointnet2_ops.head_ops import linear_act
             x = linear_act(x, self.fc1.weight, self.fc1.bias, "relu")
             if not (self.use_drop_out and self.training):          # dropout sits between fc2 and its ReLU

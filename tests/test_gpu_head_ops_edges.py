@@ -181,3 +181,27 @@ def test_distillation_slots_unused_by_value_at_any_index(V, dtype):
     # a used slot past the columns still says so
     bad = run(torch.where(index == V + 9, V, index), torch.where(index == V + 9, 0.0, value))
     assert bad[0][0].isnan() and bad[1][0].isnan().all() and torch.equal(bad[0][1:], want[0][1:])
+
+
+# ------------------------------------------------------------------------------------------------- the heads' opt-in route
+def _heads(monkeypatch, drop_out=False):
+    """(head, library's answer, fused answer) for heads on 9 and 72 rows; the fused one under the class's switch."""
+    from scene_graph_prediction.scene_graph_helpers.model.pointnets import network_PointNet as npn
+    torch.manual_seed(0)
+    head = npn.PointNetCls(12, in_size=256, batch_norm=False, drop_out=drop_out).cuda().eval()
+    x = torch.randn(9, 256).cuda()
+
+    def run(fused, x=x):
+        monkeypatch.setattr(npn._Head, "fused_linear", fused)
+        with torch.no_grad():
+            return head(x)
+    return head, x, run
+
+
+def test_fused_heads_leave_fp32_inputs_under_autocast_to_the_library(monkeypatch):
+    head, x, run = _heads(monkeypatch)
+    exact = run(True)
+    for dtype in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", dtype):
+            assert torch.equal(run(True), run(False)) and not torch.equal(run(True), exact)
+    assert torch.equal(run(True), exact)                              # (outside: the kernel again)
