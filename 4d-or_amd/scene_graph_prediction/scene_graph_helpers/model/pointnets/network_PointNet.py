@@ -46,10 +46,20 @@ def scan_batch_norm(bn: nn.BatchNorm1d, x, ptr):
     return y
 
 
+def _plain_module(m, kind):
+    """`m` is a `kind` of torch's whose call is its forward and nothing else: no subclass (a parametrisation makes one), no forward of
+    its own, no hook (torch's weight_norm and spectral_norm are hooks that form the weight)."""
+    g = nn.modules.module
+    return type(m) is kind and "forward" not in m.__dict__ and not (
+        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or g._global_forward_hooks
+        or g._global_forward_pre_hooks or g._global_backward_hooks or g._global_backward_pre_hooks)
+
+
 class _Head(BaseNetwork):
     #: heads without BatchNorm on the GPU: Linear + bias + ReLU of the trunk as one kernel each, forward and (layers of this size) the
     #: whole backward pass (pointnet2_ops/head_ops.py linear_act) instead of torch's library product and elementwise kernels.  Same
-    #: fp32 mathematics, another order of sums.  Off by default: results stay bit for bit what they were.
+    #: fp32 mathematics, another order of sums.  Off by default: results stay bit for bit what they were.  Layers that are more than
+    #: nn.Linear and nn.ReLU by themselves (replaced, parametrised, hooked) and types without a kernel stay with torch.
     fused_linear = os.environ.get("PN2_FUSED_HEADS", "0") == "1"
 
     def _make_trunk(self, in_size, batch_norm, drop_out):
@@ -57,8 +67,10 @@ class _Head(BaseNetwork):
         self.fc2 = nn.Linear(512, 256)
 
     def _trunk(self, x, use_bn, scan_ptr=None):
-        if (self.fused_linear and x.is_cuda and not use_bn and x.dtype == self.fc1.weight.dtype
-                and not torch.is_autocast_enabled("cuda")):            # (autocast chooses the types of the library's products)
+        if (self.fused_linear and x.is_cuda and not use_bn and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
+                and not torch.is_autocast_enabled("cuda")              # (autocast chooses the types of the library's products)
+                and all(_plain_module(m, nn.Linear) and m.weight.dtype == x.dtype for m in (self.fc1, self.fc2))
+                and _plain_module(self.relu, nn.ReLU)):
             from pointnet2_ops.head_ops import linear_act
             x = linear_act(x, self.fc1.weight, self.fc1.bias, "relu")
             if not (self.use_drop_out and self.training):          # dropout sits between fc2 and its ReLU

@@ -205,3 +205,44 @@ def test_fused_heads_leave_fp32_inputs_under_autocast_to_the_library(monkeypatch
         with torch.autocast("cuda", dtype):
             assert torch.equal(run(True), run(False)) and not torch.equal(run(True), exact)
     assert torch.equal(run(True), exact)                              # (outside: the kernel again)
+
+
+@pytest.mark.parametrize("how", ["hook", "pre-hook", "global hook", "weight_norm", "parametrised", "spectral_norm", "replaced", "own forward",
+                                 "other activation", "float64"])
+def test_fused_heads_leave_layers_that_are_more_than_a_product_to_torch(how, monkeypatch):
+    """Whatever a program hung onto fc1, fc2 or their activation takes part on both routes: equal bit for bit, one route by then."""
+    import torch.nn as nn
+    head, x, run = _heads(monkeypatch)
+    before, handle = run(True), None
+    if how == "hook":
+        head.fc2.register_forward_hook(lambda m, a, out: out * 2)
+    elif how == "pre-hook":
+        head.fc1.register_forward_pre_hook(lambda m, a: (a[0] + 1,))
+    elif how == "global hook":
+        handle = nn.modules.module.register_module_forward_hook(lambda m, a, out: out + 1 if m is head.fc1 else None)
+    elif how == "weight_norm":
+        nn.utils.weight_norm(head.fc1)
+        head.fc1.weight_g.data.mul_(3)                                # (the hook forms the weight anew at the next call)
+    elif how == "parametrised":
+        class Twice(nn.Module):
+            def forward(self, w):
+                return 2 * w
+        nn.utils.parametrize.register_parametrization(head.fc2, "weight", Twice())
+    elif how == "spectral_norm":
+        nn.utils.spectral_norm(head.fc2)
+    elif how == "replaced":
+        head.fc1 = nn.Sequential(nn.Linear(256, 256), nn.Linear(256, 512)).cuda()
+    elif how == "own forward":
+        head.fc1.forward = lambda t: nn.functional.linear(t, head.fc1.weight) * 2
+    elif how == "other activation":
+        head.relu = nn.Tanh()
+    else:
+        head.double()
+        x = x.double()
+    try:
+        got = run(True, x)
+        assert torch.equal(got, run(False, x))
+        assert how == "float64" or not torch.allclose(got, before, atol=1e-4)
+    finally:
+        if handle is not None:
+            handle.remove()
