@@ -237,10 +237,11 @@ def main(argv=None):
     with torch.no_grad():
         for i, scan in enumerate(scans):
             batch = to_device(scan, device)
-            scan_id, rels = model.predict_step(batch, i)
+            rel_pred = model(batch)[1]
+            scan_id, rels = model.predict_step(batch, i, rel_pred=rel_pred)
             results[scan_id] = rels
             if args.alternatives > 0:
-                alternatives[scan_id] = model.predict_alternatives(batch, args.alternatives)[1]
+                alternatives[scan_id] = model.predict_alternatives(batch, args.alternatives, rel_pred=rel_pred)[1]
     if args.alternatives > 0:
         with open(args.out + ".alternatives.json", "w") as f:
             json.dump(alternatives, f)

@@ -271,21 +271,23 @@ class SGPNModelWrapper(nn.Module):
     def validation_step(self, batch, batch_idx=0):
         return self._step(batch, "val")
 
-    def predict_alternatives(self, batch, top=3):
+    def predict_alternatives(self, batch, top=3, rel_pred=None):
         """-> (scan_id, [(subject_name, object_name, entropy, [(predicate, log probability), ...]), ...]) for EVERY edge of one scan,
-        best predicate first: the answer of predict_step with what else the model held possible."""
+        best predicate first: the answer of predict_step with what else the model held possible.  `rel_pred`: the model's second result
+        for this batch, where the caller has it."""
         if batch.get("scenes") is not None:
             raise ValueError("predict_alternatives takes one scan at a time")
-        r = self.relation_alternatives(self(batch)[1], top)
+        r = self.relation_alternatives(self(batch)[1] if rel_pred is None else rel_pred, top)
         edges = batch["edge_indices"].transpose(0, 1).cpu().tolist()
         objs, out = batch["objs_json"], []
         for (start, end), h, names, lps in zip(edges, r.entropy.cpu().tolist(), r.top_index.cpu().tolist(), r.top_log_prob.cpu().tolist()):
             out.append((objs[start + 1], objs[end + 1], h, [(self.relationNames[n], lp) for n, lp in zip(names, lps) if n >= 0]))
         return batch["scan_id"], out
 
-    def predict_step(self, batch, batch_idx=0, dataloader_idx=0):
-        """-> (scan_id, [(subject_name, predicate, object_name), ...]); 'none' edges dropped."""
-        _, rel_pred, *_ = self(batch, return_meta_data=True)
+    def predict_step(self, batch, batch_idx=0, dataloader_idx=0, rel_pred=None):
+        """-> (scan_id, [(subject_name, predicate, object_name), ...]); 'none' edges dropped.  `rel_pred` as above."""
+        if rel_pred is None:
+            _, rel_pred, *_ = self(batch, return_meta_data=True)
         predicted = torch.max(rel_pred.detach(), 1)[1].cpu().tolist()
         none_id = self.relationNames.index("none")
         edges = batch["edge_indices"].transpose(0, 1).cpu().tolist()

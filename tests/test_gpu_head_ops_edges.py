@@ -246,3 +246,28 @@ def test_fused_heads_leave_layers_that_are_more_than_a_product_to_torch(how, mon
     finally:
         if handle is not None:
             handle.remove()
+
+
+def test_alternatives_come_from_the_pass_that_made_the_triples(tmp_path, monkeypatch):
+    """One forward pass per scan with --alternatives too, and the answers of the two methods on their own."""
+    import json
+    from scene_graph_prediction import main as runner
+    calls, models = [], []
+    forward = runner.SGPNModelWrapper.forward
+
+    def counted(self, batch, **kw):
+        calls.append(batch["scan_id"])
+        models.append(self)
+        return forward(self, batch, **kw)
+    monkeypatch.setattr(runner.SGPNModelWrapper, "forward", counted)
+    out = tmp_path / "rels.json"
+    runner.main(["--mode", "infer", "--scans", "2", "--objects", "3", "--out", str(out), "--alternatives", "2"])
+    assert calls == ["synthetic_000000", "synthetic_000001"]
+    model = models[0]
+    d = runner.config_loader("no_gt.json")["dataset"]
+    rels, more = json.load(open(out)), json.load(open(str(out) + ".alternatives.json"))
+    for i, name in enumerate(calls[:2]):
+        batch = runner.to_device(runner.synthetic_scan(3, d["num_points_objects"], d["num_points_relation"], seed=i, scan_id=name), "cuda")
+        with torch.no_grad():
+            assert json.loads(json.dumps(model.predict_step(batch)[1])) == rels[name]
+            assert json.loads(json.dumps(model.predict_alternatives(batch, 2)[1])) == more[name]
