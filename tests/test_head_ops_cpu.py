@@ -182,3 +182,17 @@ def test_tensors_that_are_not_plain_memory_are_refused(name):
             return func(*args, **(kwargs or {}))
     with Watch(), pytest.raises(RuntimeError, match="CPU not supported"):
         call(f(2, 3))
+
+
+def test_objects_are_built_again_when_the_flags_change():
+    """`make` with a newer Makefile names every source again (asked for, not run)."""
+    import glob
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "4d-or_amd", "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc], capture_output=True, text=True, check=True).stdout
+    sources = [os.path.basename(p) for p in glob.glob(os.path.join(csrc, "*.hip"))]
+    assert len(sources) >= 15
+    for name in sources:
+        assert any(f"-c {name} " in line and "-packed-fp32-ops" in line for line in plan.splitlines()), name
+    assert "head_binding.cpp" in plan
