@@ -827,16 +827,21 @@ __global__ __launch_bounds__(256) void lp_grad_kernel(BwdArgs a) {
 }
 
 // Segments of a row: where rows are few and long, the workgroup that owned one would be bound by its own arithmetic while most of the
-// chip idles.  Whole rows against segments, us: 1 x 131072 bf16 10.2 - 4.4, with 20 alternatives 14.6 - 10.4, distillation 8.6 - 6.0;
-// 64 x 131072 10.7 - 6.6, 15.7 - 13.8, 9.1 - 7.8.  The second launch costs the host 3 us, and shorter rows win less than that (65536
-// bf16 6.7 - 4.4, with alternatives 11.3 - 10.4); 128 rows fill half the chip by themselves (16.1 - 17.5 with alternatives).
+// chip idles.  The second launch costs about 3 us, so a row has to pass what 1024 threads read in one round (16-bit) or two (fp32).
+// One row, whole against segments, us a call (label statistics; with 20 alternatives; distillation):
+//   bf16   65536  6.7 -  9.3, 10.9 - 10.8, 6.0 - 7.2     fp32   65536  6.7 - 8.1, 11.0 - 10.2, 6.3 - 7.6
+//          65544 10.2 -  9.0, 15.0 - 11.3, 8.9 - 7.7            70000  8.5 - 8.3, 12.8 - 10.4, 7.8 - 7.9
+//         100000 10.4 -  7.6, 15.8 - 11.2, 9.0 - 7.0           100000 10.2 - 8.0, 15.0 - 10.7, 9.0 - 7.5
+//         131072 10.1 -  8.1, 15.0 - 10.9, 8.8 - 7.6           131072 10.1 - 8.1, 14.8 - 10.0, 8.9 - 7.7
+// 64 rows of 131072: bf16 10.7 - 7.9, 15.6 - 14.3, 9.2 - 8.4, fp32 11.1 - 8.3, 15.9 - 15.0, 10.1 - 9.4; 128 rows fill half the chip by
+// themselves (16.1 - 17.5 with alternatives).
 struct Split {
   int nseg, seg;
   size_t keys, part;        // bytes
 };
 Split lp_split(long long T, int V, int dtype, int top) {
   const int ve = dtype == PN2_DT_F32 ? 4 : 8, nvec = V / ve + (V % ve != 0);
-  if (T < 1 || T > 64 || nvec < 16384) return Split{1, V, 0, 0};
+  if (T < 1 || T > 64 || V <= 65536) return Split{1, V, 0, 0};
   int n = nvec / 1024;
   if (n > kMaxSeg) n = kMaxSeg;
   const int each = (nvec + n - 1) / n;

@@ -170,3 +170,22 @@ def test_distill_top_k_of_many_long_rows(V, dtype):
     value = rnd(gen, 280, 70, scale=2.0)
     value[7, ::2] = -INF
     run_distill(x, index, value, 1.5)
+
+
+# ---------------------------------------------------------------------------------- rows around the length from which they are segments
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T,V,segments", [(1, 65536, False), (2, 65537, True), (64, 65544, True), (65, 65544, False), (3, 70001, True), (2, 100003, True)])
+def test_rows_around_the_length_of_segments(T, V, segments, dtype):
+    gen = torch.Generator().manual_seed(V + T)
+    x = rnd(gen, T, V, scale=3.0, dtype=dtype)
+    x[T // 2, torch.rand(V, generator=gen).cuda() < 0.6] = -INF
+    y = torch.randint(V, (T,), generator=gen).cuda()
+    y[T // 2] = x[T // 2].argmax()
+    y[-1], x[-1, V - 1] = V - 1, 9.0                                  # the row's last entry, in a partial vector or a segment of its own
+    joined = [n.startswith("lp_join") for n in launched(lambda: ho.label_log_probs(x, y, top=3))]
+    assert joined == ([False, True] if segments else [False])
+    for top in (0, 20) if T < 10 else (20,):
+        run_labels(x, y, top, seed=top)
+    index = torch.randint(V, (T, 30), generator=gen).cuda()
+    index[T // 2], index[-1] = y[T // 2], V - 1
+    run_distill(x, index, rnd(gen, T, 30, scale=2.0), 1.5)
