@@ -40,8 +40,11 @@ __device__ __forceinline__ la_f32x4 la_mma(HdF32, hd_u32x4 q, hd_u32x4 p, la_f32
   return c;
 }
 
-// act(z) and its slope.  FAST (16-bit results): erf by Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7, half a step of fp32 where
-// it counts), which shares its exponential with the slope; erff costs twice the instructions.
+// act(z) and its slope.  FAST (16-bit results): erf by Abramowitz and Stegun 7.1.26, which shares its exponential with the slope; erff
+// costs twice the instructions.  Off by 1.5e-7 (2.5 u, u = 2^-24) in erf and 2.1e-7 in act(z), absolutely.  Relative to a result that
+// goes to zero, far below it: 5e-4 at z = -4 (fp16's half step there is 2.4e-4 to 4.9e-4), 1.6e-3 at -5, 3.6e-3 at -6 (bf16's half
+// step: 2e-3 to 3.9e-3), 1 % at -8, where act is 5e-15.  The fp32 form is erff's, whose 1 + erf cancels there: half a step of 1/2 is
+// 9e-4 of it at -4 and 10 % at -5.
 template <int ACT, bool FAST>
 __device__ __forceinline__ void la_act(float z, float &y, float &d) {
   if constexpr (ACT == ACT_NONE) {
