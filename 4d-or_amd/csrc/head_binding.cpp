@@ -13,12 +13,15 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/pn2_hip.h"
 
@@ -134,6 +137,41 @@ void check_device(const Tensor &lead, std::initializer_list<std::pair<const Tens
   }
 }
 
+// A backward pass that is being captured must not go on to a node of a stream outside the capture: torch would make that stream wait
+// for the captured one, which breaks the capture and can end the process.  It comes about where an eager graph of the same leaves is
+// still alive, because the node that accumulates a leaf's gradient belongs to the stream of the leaf's first living graph.  Called on
+// the node's own stream; looks at what lies behind the node (captures only).
+void check_capture(const char *op) {
+  auto capturing = [](hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &status) != hipSuccess) (void)hipGetLastError();
+    return status != hipStreamCaptureStatusNone;
+  };
+  const auto here = c10::hip::getCurrentHIPStream();
+  if (!capturing(here.stream())) return;
+  using torch::autograd::Node;
+  const auto first = torch::autograd::get_current_node();
+  std::vector<Node *> todo;
+  std::unordered_set<Node *> seen;
+  if (first) todo.push_back(first.get());
+  while (!todo.empty()) {
+    Node *node = todo.back();
+    todo.pop_back();
+    for (const auto &edge : node->next_edges()) {
+      Node *next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      todo.push_back(next);
+      const auto s = next->stream();
+      if (!s || s->device_index() != here.device_index() || s->id() == here.id()) continue;
+      // (the default stream is never captured; another one may have joined the capture)
+      const bool joined = s->id() != 0 && capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED,
+                                                                         c10::Stream(c10::Stream::UNSAFE, here.device(), s->id())).stream());
+      TORCH_CHECK(joined, op, "'s backward pass is being captured while an eager graph of the same leaves is alive on another stream: "
+                              "drop what holds that graph first, or give the captured pass leaves of its own (detach)");
+    }
+  }
+}
+
 // Each operator is differentiable once: where a graph of the backward pass is being built (create_graph), its results raise when
 // they are differentiated.
 variable_list once(variable_list out) {
@@ -185,6 +223,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     return o.y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_capture("linear_act");
     const int64_t need = ctx->saved_data["need"].toInt(), K = ctx->saved_data["k"].toInt();
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
@@ -296,6 +335,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     return {o.log_prob, o.entropy, o.top_log_prob, o.top_index};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_capture("label_log_probs");
     check_plain("label_log_probs' gradient", {{&grads[0], "the gradient of log_prob"}, {&grads[1], "the gradient of entropy"}});
     const Tensor g = grad_rows(grads[0]), h = grad_rows(grads[1]);
     Tensor dx;
@@ -382,6 +422,7 @@ struct DistillTopK : torch::autograd::Function<DistillTopK> {
     return loss;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    check_capture("distill_top_k");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &index = saved[1], &values = saved[2], &stats = saved[3];
     check_plain("distill_top_k's gradient", {{&grads[0], "the gradient of the loss"}});

@@ -12,7 +12,9 @@ such a head on hand-written kernels (csrc/linear_act.hip, csrc/label_probs.hip),
 Leading axes are free; tensors must be on the GPU (RuntimeError otherwise), work runs on the current stream of their device, and
 nothing is synchronised or kept between calls.  Each operator is differentiable once, in reverse mode.  The kernels run outside
 torch's dispatcher: dual tensors of forward mode, recording by ``torch.jit.trace`` / ``make_fx`` / export, subclasses with
-``__torch_dispatch__`` and tensors without memory of their own are refused (RuntimeError).
+``__torch_dispatch__`` and tensors without memory of their own are refused (RuntimeError).  So is a backward pass that is captured into
+a graph while an eager graph of the same leaves lives on another stream (torch would break the capture): drop that graph first, or
+capture with leaves of its own.
 """
 import collections
 import os

@@ -271,3 +271,69 @@ def test_alternatives_come_from_the_pass_that_made_the_triples(tmp_path, monkeyp
         with torch.no_grad():
             assert json.loads(json.dumps(model.predict_step(batch)[1])) == rels[name]
             assert json.loads(json.dumps(model.predict_alternatives(batch, 2)[1])) == more[name]
+
+
+# ------------------------------------------------------------------------- captured backward passes and what is alive outside of them
+def _captured_calls():
+    gen = torch.Generator().manual_seed(5)
+    x, w = torch.randn(30, 40, generator=gen).cuda(), torch.randn(20, 40, generator=gen).cuda()
+    logits, y = torch.randn(30, 20, generator=gen).cuda(), torch.arange(30).cuda() % 20
+    index, value = torch.arange(60).view(30, 2).cuda() % 20, torch.randn(30, 2, generator=gen).cuda()
+    return {"linear_act": (w, lambda t: ho.linear_act(x, t, None, "silu")), "linear_act behind another node": (w, lambda t: ho.linear_act(x, t * 2)),
+            "label_log_probs": (logits, lambda t: ho.label_log_probs(t, y, top=2).log_prob), "distill_top_k": (logits, lambda t: ho.distill_top_k(t, index, value))}
+
+
+@pytest.mark.parametrize("name", list(_captured_calls()))
+def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves_is_refused(name):
+    """... before torch makes the eager graph's stream wait for the captured one; the capture goes on, and without that graph, or with
+    leaves of its own, the pass is captured and replays."""
+    data, call = _captured_calls()[name]
+    leaf = data.requires_grad_()
+    alive = call(leaf)
+    want, = torch.autograd.grad(call(leaf).sum(), leaf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(leaf)
+        with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+            torch.autograd.grad(out.sum(), leaf)
+        own = leaf.detach().requires_grad_()
+        got, = torch.autograd.grad(call(own).sum(), own)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    del alive, out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(call(leaf).sum(), leaf)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", list(_captured_calls()))
+def test_a_captured_backward_pass_over_two_streams(name):
+    """A stream that has joined the capture is part of it."""
+    data, call = _captured_calls()[name]
+    leaf = data.requires_grad_()
+    want, = torch.autograd.grad((call(leaf * 1) + call(leaf * 1)).sum(), leaf)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        a, b = leaf * 1, leaf * 1
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            one = call(b)
+        two = call(a)
+        main.wait_stream(side)
+        got, = torch.autograd.grad((one + two).sum(), leaf)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        torch.testing.assert_close(got, want, rtol=4 * 2.0 ** -24, atol=4 * 2.0 ** -24 * float(want.abs().max()))
