@@ -274,6 +274,9 @@ def test_alternatives_come_from_the_pass_that_made_the_triples(tmp_path, monkeyp
 
 
 # ------------------------------------------------------------------------- captured backward passes and what is alive outside of them
+CAPTURED = ["linear_act", "linear_act behind another node", "label_log_probs", "distill_top_k"]
+
+
 def _captured_calls():
     gen = torch.Generator().manual_seed(5)
     x, w = torch.randn(30, 40, generator=gen).cuda(), torch.randn(20, 40, generator=gen).cuda()
@@ -283,7 +286,7 @@ def _captured_calls():
             "label_log_probs": (logits, lambda t: ho.label_log_probs(t, y, top=2).log_prob), "distill_top_k": (logits, lambda t: ho.distill_top_k(t, index, value))}
 
 
-@pytest.mark.parametrize("name", list(_captured_calls()))
+@pytest.mark.parametrize("name", CAPTURED)
 def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves_is_refused(name):
     """... before torch makes the eager graph's stream wait for the captured one; the capture goes on, and without that graph, or with
     leaves of its own, the pass is captured and replays."""
@@ -315,7 +318,7 @@ def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves_is_re
         assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("name", list(_captured_calls()))
+@pytest.mark.parametrize("name", CAPTURED)
 def test_a_captured_backward_pass_over_two_streams(name):
     """A stream that has joined the capture is part of it."""
     data, call = _captured_calls()[name]
