@@ -90,7 +90,8 @@ def distill_top_k(logits, teacher_index, teacher_logits, temperature=1.0):
     differences count).  q = softmax(teacher_logits / temperature) over the row's k entries, p = softmax(logits / temperature) over
     all V.  -> (...) fp32, differentiable in the logits; the teacher is a constant (RuntimeError if it requires a gradient).
     A slot with a negative index or the value -inf is unused; a row without a used slot has loss 0 and gradient 0 (so padded rows
-    take teacher_index = -1).  An index >= V of a used slot makes its row NaN; an index may occur more than once."""
+    take teacher_index = -1).  An index >= V of a used slot makes its row NaN; an index may occur more than once.  Where the teacher has
+    an entry that is masked (-inf) for the student the loss is +inf; a student's row of nothing but -inf has gradient 0."""
     try:
         return _heads.distill_top_k(logits, teacher_index, teacher_logits, float(temperature), _timed())
     except TypeError:
