@@ -110,7 +110,7 @@ __device__ __forceinline__ float hd_wave_max(float v) {
 __device__ __forceinline__ float hd_exp2(float v) { return __builtin_amdgcn_exp2f(v); }   // v_exp_f32: 1 ulp, flushes below 2^-126
 
 // n workgroups of `threads` threads.  The launch packet counts an axis in 32-bit threads, and 2^32 of them wrap without an error (67
-// million short rows had 3 of their results): what passes that goes to the second axis.  hd_block(): this workgroup's number, which
+// million short rows got 4 of their results): what passes that goes to the second axis.  hd_block(): this workgroup's number, which
 // can then be n or more.
 inline dim3 hd_grid(long long n, unsigned threads) {
   const long long most = 0xffffffffLL / threads, y = (n + most - 1) / most;

@@ -108,3 +108,34 @@ def test_a_teacher_model_and_its_student():
     grads = torch.autograd.grad(loss, [p for p in student.rel_predictor.parameters()])
     assert all(g.isfinite().all() and g.any() for g in grads if g.numel())
     student.training_step(batch).backward()
+
+
+@pytest.mark.gpu
+def test_a_replayed_step_reads_its_batch_s_teacher():
+    """Whole steps on one batch of scans with learning rate 0 and no dropout: the eager first one, the captured one, replays with other
+    predicates of the teacher; every loss is the eager loss of its batch (atomics in the encoders' backward do not reach it)."""
+    from runtime import GraphedTrainStep
+    from scene_graph_prediction import main as runner
+    from scene_graph_prediction.scene_graph_helpers.dataset.synthetic import collate_scans
+    torch.manual_seed(4)
+    model = runner.SGPNModelWrapper(runner.config_loader("no_gt.json"), 12, 15, torch.ones(12), torch.ones(15), runner.RELATION_NAMES).cuda().train()
+    for m in model.modules():
+        if isinstance(m, torch.nn.Dropout):
+            m.p = 0.0
+    for n, p in model.named_parameters():
+        if ".backbone.fc_layer." in n:
+            p.requires_grad_(False)
+    opt = torch.optim.AdamW([p for p in model.parameters() if p.requires_grad], lr=0.0, weight_decay=0.0, capturable=True)
+    step = GraphedTrainStep(model.pure_training_step, model.parameters(), opt)
+
+    def batch(seed):
+        scans = [dict(synthetic_scan(n, 512, 1024, seed=n, scan_id=f"s{n}"), teacher_rels=scan(n, seed)["teacher_rels"]) for n in (4, 3)]
+        return to_device(collate_scans(scans), "cuda")
+    losses = []
+    for seed in (1, 1, 2, 3, 1):
+        b = batch(seed)
+        with torch.no_grad():
+            want = float(model.pure_training_step(b)[0])
+        losses.append(float(step(b)[0]))
+        assert abs(losses[-1] - want) <= 1e-5 * want
+    assert step.num_graphs == 1 and len({round(v, 4) for v in losses}) == 3
